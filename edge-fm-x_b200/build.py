@@ -31,8 +31,9 @@ CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-Wextra", "-Wno-unused-para
 CORE_CU = ["src/backends/b200/efm_b200.cu", "src/layers/gemm_launch.cu", "src/backends/b200/nccl_glue.cpp"]
 QWEN_CU = ["src/backends/b200/qwen_b200.cu", "src/layers/attention_launch.cu", "src/layers/qwen_text.cu", "src/backends/b200/ops_b200.cu", "src/backends/b200/vit_b200.cu"]
 VLA_CU = ["src/backends/b200/vla_b200.cu"]
+KV4_CU = ["src/backends/b200/kv4_b200.cu"]
 DECODER_CU = ["src/backends/b200/decoder_b200.cu", "src/layers/decoder.cu"]
-BACKEND_CU = CORE_CU + DECODER_CU + QWEN_CU + VLA_CU
+BACKEND_CU = CORE_CU + DECODER_CU + QWEN_CU + VLA_CU + KV4_CU
 ENGINE_CPP = sorted(glob.glob(os.path.join(HERE, "src", "engine", "*.cpp"))) + \
     [os.path.join(HERE, "src", "edge-fm.cpp"), os.path.join(HERE, "src", "tensor.cpp")]
 

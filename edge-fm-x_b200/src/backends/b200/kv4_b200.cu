@@ -1,0 +1,326 @@
+// Operators of the 4-bit key/value cache (include/efm_b200_kv4.h): checks of arguments, sizes, launches on the caller's stream.
+#include <efm_b200_kv4.h>
+
+#include <atomic>
+#include <exception>
+
+#include "../../operators/kv4_attention.cuh"
+#include "../../operators/kv4_cache.cuh"
+#include "../../operators/kv4_evict.cuh"
+#include "ctx_util.h"
+
+namespace efm {
+namespace {
+
+using kv4::kRows;
+
+efm_status bad(const char* call, const char* what) { return fail(nullptr, EFM_ERR_INVALID_ARGUMENT, std::string(call) + ": " + what); }
+bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
+
+efm_status check_cache(const char* call, const efm_kv4_cache* c) {
+    if (c == nullptr || c->struct_size != (int32_t)sizeof(efm_kv4_cache)) return bad(call, "cache: struct_size does not match this header");
+    if (c->dtype != EFM_BF16 && c->dtype != EFM_F16) return fail(nullptr, EFM_ERR_UNSUPPORTED, std::string(call) + ": dtype bf16 or fp16");
+    if (c->head_dim != 64 && c->head_dim != 128) return fail(nullptr, EFM_ERR_UNSUPPORTED, std::string(call) + ": head_dim 64 or 128");
+    if (c->kv_heads < 1 || c->q_heads < 1 || c->q_heads > 1024 || c->q_heads % c->kv_heads != 0) return bad(call, "q_heads a multiple of kv_heads, at most 1024");
+    if (c->n_pages < 1 || c->batch < 1 || c->batch > 65535 || c->max_pages < 1 || c->max_pages >= (1 << 24)) return bad(call, "n_pages, batch or max_pages out of range");
+    return EFM_OK;
+}
+efm_status check_buffers(const char* call, const efm_kv4_cache* c) {
+    if (c->pool == nullptr || c->page_table == nullptr || !aligned(c->pool, 16) || !aligned(c->page_table, 4) || !aligned(c->status, 4))
+        return bad(call, "pool (16-byte aligned) and page_table are needed");
+    return EFM_OK;
+}
+
+// The pool's GPU for the length of a call; what the thread had current comes back with it.
+class OnDevice {
+public:
+    efm_status enter(const char* call, const void* pool) {
+        cudaPointerAttributes at{};
+        cudaError_t e = cudaPointerGetAttributes(&at, pool);
+        if (e != cudaSuccess) { (void)cudaGetLastError(); return cuda_fail(nullptr, e, call); }
+        if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) return bad(call, "pool is not device memory");
+        e = cudaGetDevice(&before_);
+        if (e == cudaSuccess && before_ != at.device) { e = cudaSetDevice(at.device); moved_ = e == cudaSuccess; }
+        if (e != cudaSuccess) return cuda_fail(nullptr, e, call);
+        device = at.device;
+        return EFM_OK;
+    }
+    ~OnDevice() { if (moved_) (void)cudaSetDevice(before_); }
+    int device = 0;
+
+private:
+    int before_ = 0;
+    bool moved_ = false;
+};
+
+struct DeviceInfo { int sms = 0, smem = 0; };
+constexpr int kEvictSmemReserve = 12 * 1024;          // static shared memory of the ordering kernel, rounded up
+
+// Once per device: architecture, sizes, shared memory beyond the default.
+efm_status device_info(const char* call, int device, DeviceInfo& info) {
+    static std::atomic<int64_t> known[64];
+    if (device < 0 || device >= 64) return fail(nullptr, EFM_ERR_UNSUPPORTED, "device index above 63");
+    int64_t k = known[device].load(std::memory_order_acquire);
+    if (k == 0) {
+        int major = 0, minor = 0, sms = 0, smem = 0;
+        cudaError_t e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device);
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device);
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);
+        if (e != cudaSuccess) return cuda_fail(nullptr, e, call);
+        if (major != 10 || minor != 0) return fail(nullptr, EFM_ERR_CUDA, std::string(call) + ": needs an sm_100 device");
+        e = cudaFuncSetAttribute(kv4::evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem - kEvictSmemReserve);
+        if (e != cudaSuccess) return cuda_fail(nullptr, e, call);
+        k = ((int64_t)sms << 32) | smem;
+        known[device].store(k, std::memory_order_release);
+    }
+    info.sms = (int)(k >> 32);
+    info.smem = (int)(k & 0xffffffff);
+    return EFM_OK;
+}
+
+kv4::Cache device_cache(const efm_kv4_cache* c) {
+    return kv4::Cache{c->q_heads, c->kv_heads, c->n_pages, c->batch, c->max_pages, (uint8_t*)c->pool, c->page_table, c->status};
+}
+
+template <typename F>
+void by_type(const efm_kv4_cache* c, F&& f) {
+    if (c->dtype == EFM_BF16) { if (c->head_dim == 64) f(__nv_bfloat16(), std::integral_constant<int, 64>()); else f(__nv_bfloat16(), std::integral_constant<int, 128>()); }
+    else { if (c->head_dim == 64) f(__half(), std::integral_constant<int, 64>()); else f(__half(), std::integral_constant<int, 128>()); }
+}
+
+Launcher on_stream(void* stream) {
+    Launcher L;
+    L.stream = (cudaStream_t)stream;
+    L.pdl = false;
+    return L;
+}
+efm_status launched(const char* call, const Launcher& L) { return L.err == cudaSuccess ? EFM_OK : cuda_fail(nullptr, L.err, call); }
+
+template <typename F>
+efm_status guarded(F&& f) {
+    try { return f(); } catch (const std::exception&) { return EFM_ERR_OUT_OF_MEMORY; } catch (...) { return EFM_ERR_STATE; }
+}
+
+int64_t capacity(const efm_kv4_cache* c) { return (int64_t)c->max_pages * kRows; }
+int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+efm_status check_attention(const char* call, const efm_kv4_cache* c, const efm_kv4_attention* a) {
+    if (a == nullptr || a->struct_size != (int32_t)sizeof(efm_kv4_attention)) return bad(call, "struct_size does not match this header");
+    if (a->max_rows < 0 || a->max_rows > (1 << 30) || a->max_new < 0 || a->max_len < 0 || a->max_len > capacity(c)) return bad(call, "max_rows, max_new or max_len out of range");
+    if ((a->mass_in == nullptr) != (a->mass_out == nullptr)) return bad(call, "mass_in and mass_out: both or neither");
+    if (!(a->scale > 0.f) || !(a->scale < INFINITY)) return bad(call, "scale: positive and finite");
+    return EFM_OK;
+}
+int64_t attention_bytes(const efm_kv4_cache* c, const efm_kv4_attention* a) {
+    return a->mass_out != nullptr ? (int64_t)a->max_rows * c->q_heads * (int64_t)sizeof(float2) : 0;
+}
+
+efm_status check_evict(const char* call, const efm_kv4_evict* a) {
+    if (a == nullptr || a->struct_size != (int32_t)sizeof(efm_kv4_evict)) return bad(call, "struct_size does not match this header");
+    if (a->budget < 1 || a->limit < a->budget || a->keep_first < 0 || a->keep_last < 0) return bad(call, "budget >= 1, limit >= budget, keep_first and keep_last >= 0");
+    return EFM_OK;
+}
+int64_t most_moves(const efm_kv4_cache* c, const efm_kv4_evict* a) {
+    return std::max<int64_t>(0, std::min<int64_t>(a->budget, capacity(c) - a->budget));
+}
+int64_t evict_counts(const efm_kv4_cache* c) { return round_up((int64_t)c->batch * c->kv_heads * 4, 16); }
+int64_t evict_bytes(const efm_kv4_cache* c, const efm_kv4_evict* a) {
+    return evict_counts(c) + (int64_t)c->batch * c->kv_heads * most_moves(c, a) * (int64_t)sizeof(int2);
+}
+
+}  // namespace
+}  // namespace efm
+
+using namespace efm;
+
+extern "C" {
+
+efm_status efm_b200_kv4_tile_bytes(int32_t head_dim, int64_t* bytes) {
+    return guarded([&] {
+        if (bytes == nullptr || (head_dim != 64 && head_dim != 128)) return bad("kv4_tile_bytes", "head_dim 64 or 128");
+        *bytes = head_dim == 64 ? kv4::Tile<64>::BYTES : kv4::Tile<128>::BYTES;
+        return (efm_status)EFM_OK;
+    });
+}
+
+efm_status efm_b200_kv4_attention_workspace(const efm_kv4_cache* cache, const efm_kv4_attention* a, int64_t* bytes) {
+    return guarded([&] {
+        const char* call = "kv4_attention_workspace";
+        efm_status st = check_cache(call, cache);
+        if (st == EFM_OK) st = check_attention(call, cache, a);
+        if (st == EFM_OK && bytes == nullptr) st = bad(call, "bytes is null");
+        if (st == EFM_OK) *bytes = attention_bytes(cache, a);
+        return st;
+    });
+}
+
+efm_status efm_b200_kv4_evict_workspace(const efm_kv4_cache* cache, const efm_kv4_evict* a, int64_t* bytes) {
+    return guarded([&] {
+        const char* call = "kv4_evict_workspace";
+        efm_status st = check_cache(call, cache);
+        if (st == EFM_OK) st = check_evict(call, a);
+        if (st == EFM_OK && bytes == nullptr) st = bad(call, "bytes is null");
+        if (st == EFM_OK) *bytes = evict_bytes(cache, a);
+        return st;
+    });
+}
+
+efm_status efm_b200_op_kv4_append(const efm_kv4_cache* cache, const efm_kv4_append* a, void* stream) {
+    return guarded([&]() -> efm_status {
+        const char* call = "op_kv4_append";
+        efm_status st = check_cache(call, cache);
+        if (st == EFM_OK) st = check_buffers(call, cache);
+        if (st != EFM_OK) return st;
+        if (a == nullptr || a->struct_size != (int32_t)sizeof(efm_kv4_append)) return bad(call, "struct_size does not match this header");
+        const int64_t D = cache->head_dim, qd = cache->q_heads * D, kd = cache->kv_heads * D;
+        if (a->max_rows < 0 || a->max_rows > (1 << 30)) return bad(call, "max_rows out of range");
+        if (a->cu_rows == nullptr || a->lens_in == nullptr || a->lens_out == nullptr || a->lens_in == a->lens_out)
+            return bad(call, "cu_rows, lens_in and lens_out (two buffers) are needed");
+        if (a->max_rows > 0) {
+            if (a->k == nullptr || a->v == nullptr || (a->q == nullptr) != (a->q_out == nullptr)) return bad(call, "k and v are needed, q and q_out together");
+            if (a->k_stride < kd || a->v_stride < kd || a->k_stride % 8 || a->v_stride % 8 || (a->q != nullptr && (a->q_stride < qd || a->q_stride % 8)))
+                return bad(call, "strides: multiples of 8 elements, at least heads x head_dim");
+            for (const void* p : {a->q, a->k, a->v, a->q_norm, a->k_norm, (const void*)a->q_out, (const void*)a->k_held, (const void*)a->v_held})
+                if (!aligned(p, 16)) return bad(call, "q, k, v, norm weights and their outputs: 16-byte aligned");
+            for (const void* p : {(const void*)a->cu_rows, (const void*)a->lens_in, (const void*)a->lens_out, (const void*)a->positions, (const void*)a->token_index,
+                                  (const void*)a->index, (const void*)a->mass})
+                if (!aligned(p, 4)) return bad(call, "numbers: aligned to their size");
+            if (a->norm != 0 && a->norm != 1) return bad(call, "norm: 0 or 1");
+            if (a->norm == 1 && !(a->norm_eps >= 0.f)) return bad(call, "norm_eps: not negative");
+            if (a->rot_dims < 0 || a->rot_dims > D || a->rot_dims % 16) return bad(call, "rot_dims: a multiple of 16, at most head_dim");
+            if (a->rot_dims > 0) {
+                if (a->rot_kind != EFM_KV4_ROT_HALVES && a->rot_kind != EFM_KV4_ROT_NEIGHBOURS) return bad(call, "rot_kind");
+                if (a->axes != 1 && a->axes != 3) return bad(call, "axes: 1 or 3");
+                if (a->axes == 3) {
+                    int64_t sum = 0;
+                    for (int i = 0; i < 3; ++i) { if (a->sections[i] < 0) return bad(call, "sections: not negative"); sum += a->sections[i]; }
+                    if (sum != a->rot_dims / 2) return bad(call, "sections: their sum is rot_dims / 2");
+                }
+                if (a->inv_freq == nullptr || a->positions == nullptr || !aligned(a->inv_freq, 8)) return bad(call, "inv_freq and positions are needed to rotate");
+            }
+        }
+        OnDevice on;
+        DeviceInfo info;
+        if ((st = on.enter(call, cache->pool)) != EFM_OK || (st = device_info(call, on.device, info)) != EFM_OK) return st;
+        kv4::AppendParams p{};
+        p.max_rows = a->max_rows;
+        p.cu_rows = a->cu_rows; p.lens_in = a->lens_in; p.lens_out = a->lens_out;
+        p.q = a->q; p.k = a->k; p.v = a->v;
+        p.q_stride = a->q_stride; p.k_stride = a->k_stride; p.v_stride = a->v_stride;
+        p.norm = a->norm; p.eps = a->norm_eps; p.q_norm = a->q_norm; p.k_norm = a->k_norm;
+        p.rot_dims = a->rot_dims; p.neighbours = a->rot_kind == EFM_KV4_ROT_NEIGHBOURS; p.axes = a->axes;
+        p.section0 = a->sections[0]; p.section1 = a->sections[1];
+        p.inv_freq = a->inv_freq; p.positions = a->positions; p.token_index = a->token_index;
+        p.q_out = a->q_out; p.k_held = a->k_held; p.v_held = a->v_held;
+        p.index = a->index; p.mass = a->mass;
+        const int heads = cache->q_heads + 2 * cache->kv_heads, warps = kv4::kAppendThreads / 32;
+        // few rows: a head per warp, so that the row's heads are on as many SMs as there are; many rows: a block per row, one table of angles
+        const int per_block = a->max_rows * ((heads + warps - 1) / warps) <= 2 * info.sms ? warps : heads;
+        Launcher L = on_stream(stream);
+        by_type(cache, [&](auto t, auto d) {
+            L.launch(kv4::append_kernel<decltype(t), decltype(d)::value>, dim3(std::max(a->max_rows, 1), (heads + per_block - 1) / per_block), dim3(kv4::kAppendThreads), 0,
+                     device_cache(cache), p, per_block);
+        });
+        return launched(call, L);
+    });
+}
+
+efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_attention* a, void* stream) {
+    return guarded([&]() -> efm_status {
+        const char* call = "op_kv4_attention";
+        efm_status st = check_cache(call, cache);
+        if (st == EFM_OK) st = check_buffers(call, cache);
+        if (st == EFM_OK) st = check_attention(call, cache, a);
+        if (st != EFM_OK) return st;
+        if (a->cu_rows == nullptr || a->lens == nullptr || !aligned(a->cu_rows, 4) || !aligned(a->lens, 4)) return bad(call, "cu_rows and lens are needed");
+        if (a->max_rows > 0 && (a->q == nullptr || a->out == nullptr || !aligned(a->q, 16) || !aligned(a->out, 16))) return bad(call, "q and out are needed, 16-byte aligned");
+        if (!aligned(a->mass_in, 4) || !aligned(a->mass_out, 4)) return bad(call, "mass: aligned to 4 bytes");
+        const int64_t need = attention_bytes(cache, a);
+        if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need || !aligned(a->workspace, 16)))
+            return bad(call, "workspace: 16-byte aligned, as large as efm_b200_kv4_attention_workspace says");
+        OnDevice on;
+        DeviceInfo info;
+        if ((st = on.enter(call, cache->pool)) != EFM_OK || (st = device_info(call, on.device, info)) != EFM_OK) return st;
+        kv4::AttnParams p{};
+        p.max_rows = a->max_rows; p.max_new = std::min(a->max_new, a->max_rows);
+        p.max_len = a->max_len > 0 ? a->max_len : (int)capacity(cache);
+        p.cu_rows = a->cu_rows; p.lens = a->lens; p.q = a->q; p.out = a->out;
+        p.scale_log2 = a->scale * 1.4426950408889634f;
+        p.mass_in = a->mass_in; p.mass_out = a->mass_out;
+        p.stats = a->mass_out != nullptr ? (float2*)a->workspace : nullptr;
+        Launcher L = on_stream(stream);
+        by_type(cache, [&](auto t, auto d) {
+            using T = decltype(t);
+            constexpr int D = decltype(d)::value;
+            if (p.max_new > 0) L.launch(kv4::attend_plain_kernel<T, D>, dim3(p.max_new, cache->q_heads, cache->batch), dim3(128), 0, device_cache(cache), p);
+            if (p.mass_out != nullptr) L.launch(kv4::mass_plain_kernel<T, D>, dim3((p.max_len + 7) / 8, cache->kv_heads, cache->batch), dim3(256), 0, device_cache(cache), p);
+        });
+        return launched(call, L);
+    });
+}
+
+efm_status efm_b200_op_kv4_evict(const efm_kv4_cache* cache, const efm_kv4_evict* a, void* stream) {
+    return guarded([&]() -> efm_status {
+        const char* call = "op_kv4_evict";
+        efm_status st = check_cache(call, cache);
+        if (st == EFM_OK) st = check_buffers(call, cache);
+        if (st == EFM_OK) st = check_evict(call, a);
+        if (st != EFM_OK) return st;
+        if (a->lens_in == nullptr || a->lens_out == nullptr || a->lens_in == a->lens_out) return bad(call, "lens_in and lens_out (two buffers) are needed");
+        for (const void* p : {(const void*)a->index_in, (const void*)a->index_out, (const void*)a->mass_in, (const void*)a->mass_out})
+            if (p == nullptr || !aligned(p, 4)) return bad(call, "index and mass, in and out, are needed");
+        if (!aligned(a->lens_in, 4) || !aligned(a->lens_out, 4)) return bad(call, "lens: aligned to 4 bytes");
+        if (a->workspace == nullptr || a->workspace_bytes < evict_bytes(cache, a) || !aligned(a->workspace, 16))
+            return bad(call, "workspace: 16-byte aligned, as large as efm_b200_kv4_evict_workspace says");
+        OnDevice on;
+        DeviceInfo info;
+        if ((st = on.enter(call, cache->pool)) != EFM_OK || (st = device_info(call, on.device, info)) != EFM_OK) return st;
+        kv4::EvictParams p{};
+        p.budget = a->budget; p.limit = a->limit; p.keep_first = a->keep_first; p.keep_last = a->keep_last;
+        p.lens_in = a->lens_in; p.lens_out = a->lens_out; p.index_in = a->index_in; p.index_out = a->index_out; p.mass_in = a->mass_in; p.mass_out = a->mass_out;
+        p.n_moves = (int32_t*)a->workspace;
+        p.moves = (int2*)((char*)a->workspace + evict_counts(cache));
+        p.most_moves = (int)most_moves(cache, a);
+        p.keys_cap = (int)std::min<int64_t>(capacity(cache), (info.smem - kEvictSmemReserve) / 4);
+        Launcher L = on_stream(stream);
+        const kv4::Cache c = device_cache(cache);
+        L.launch(kv4::evict_select_kernel, dim3(cache->kv_heads, cache->batch), dim3(kv4::kEvictThreads), (size_t)p.keys_cap * 4, c, p);
+        if (p.most_moves > 0) {
+            const int per = kv4::kMoveThreads / 16, all = (p.most_moves + per - 1) / per;
+            const int parts = (int)std::min<int64_t>(all, std::max<int64_t>(1, (int64_t)16 * info.sms / ((int64_t)cache->batch * cache->kv_heads)));
+            if (cache->head_dim == 64) L.launch(kv4::evict_move_kernel<64>, dim3(parts, cache->kv_heads, cache->batch), dim3(kv4::kMoveThreads), 0, c, p);
+            else L.launch(kv4::evict_move_kernel<128>, dim3(parts, cache->kv_heads, cache->batch), dim3(kv4::kMoveThreads), 0, c, p);
+        }
+        return launched(call, L);
+    });
+}
+
+efm_status efm_b200_op_kv4_read(const efm_kv4_cache* cache, const efm_kv4_read* a, void* stream) {
+    return guarded([&]() -> efm_status {
+        const char* call = "op_kv4_read";
+        efm_status st = check_cache(call, cache);
+        if (st == EFM_OK) st = check_buffers(call, cache);
+        if (st != EFM_OK) return st;
+        if (a == nullptr || a->struct_size != (int32_t)sizeof(efm_kv4_read)) return bad(call, "struct_size does not match this header");
+        if (a->first < 0 || a->rows < 0 || (int64_t)a->first + a->rows > (1 << 30)) return bad(call, "first and rows out of range");
+        if (a->lens == nullptr || !aligned(a->lens, 4) || (a->k_out == nullptr && a->v_out == nullptr) || !aligned(a->k_out, 16) || !aligned(a->v_out, 16))
+            return bad(call, "lens and k_out or v_out (16-byte aligned) are needed");
+        OnDevice on;
+        DeviceInfo info;
+        if ((st = on.enter(call, cache->pool)) != EFM_OK || (st = device_info(call, on.device, info)) != EFM_OK) return st;
+        const int64_t end = std::min<int64_t>(capacity(cache), (int64_t)a->first + a->rows);
+        const int64_t pages = end > a->first ? (end + kRows - 1) / kRows - a->first / kRows : 0;
+        if (pages == 0) return EFM_OK;
+        if (pages * cache->kv_heads > 0x7fffffff) return bad(call, "too many rows");
+        Launcher L = on_stream(stream);
+        by_type(cache, [&](auto t, auto d) {
+            using T = decltype(t);
+            L.launch(kv4::read_kernel<T, decltype(d)::value>, dim3((unsigned)(pages * cache->kv_heads), cache->batch), dim3(kv4::kReadThreads), 0, device_cache(cache),
+                     a->lens, a->first, a->rows, (T*)a->k_out, (T*)a->v_out);
+        });
+        return launched(call, L);
+    });
+}
+
+}  // extern "C"

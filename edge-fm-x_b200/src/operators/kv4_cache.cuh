@@ -1,0 +1,281 @@
+// A key/value cache in 4 bits (include/efm_b200_kv4.h has the layout): appending rows and reading them back.
+//
+// append: y = x r w with r = 1 / sqrt(mean(x^2) + eps), channels turned by their position's angle, q rounded once, k and v snapped to
+// min + scale * code.  Codes are whole numbers, so what is done to x before them is fixed operation by operation (squares summed in
+// 64 bits, every other product and sum rounded to 32 bits on its own, angles and their sine and cosine in 64 bits): the same input
+// gives the same cache whatever the launch shape.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace efm {
+namespace kv4 {
+
+constexpr int kRows = 64, kGroup = 64;
+constexpr int kBadPage = 1, kFull = 2, kBadCount = 4, kWait = 8;      // EFM_KV4_*
+
+template <int D>
+struct Tile {
+    static constexpr int G = D / kGroup;                     // groups of a row
+    static constexpr int CODES = kRows * D / 2, PARAMS = kRows * G * 4;
+    static constexpr int K_CODES = 0, K_PARAMS = CODES, V_CODES = CODES + PARAMS, V_PARAMS = 2 * CODES + PARAMS;
+    static constexpr int BYTES = 2 * (CODES + PARAMS);
+    static constexpr int WORDS = D / 8;                      // 32-bit words of a row's codes
+};
+
+struct Cache {
+    int q_heads, kv_heads, n_pages, batch, max_pages;
+    uint8_t* pool;
+    const int32_t* page_table;
+    int32_t* status;
+};
+
+__device__ __forceinline__ void raise(const Cache& c, int bit) {
+    if (c.status != nullptr) atomicOr(c.status, bit);
+}
+// Page that holds cache rows [64 k, 64 k + 64) of sequence b, -1 where its number is not one of the pool's.
+__device__ __forceinline__ int page_of(const Cache& c, int b, int k) {
+    const int p = c.page_table[(size_t)b * c.max_pages + k];
+    if ((unsigned)p < (unsigned)c.n_pages) return p;
+    raise(c, kBadPage);
+    return -1;
+}
+template <int D>
+__device__ __forceinline__ uint8_t* tile_of(const Cache& c, int page, int head) {
+    return c.pool + ((size_t)page * c.kv_heads + head) * Tile<D>::BYTES;
+}
+__device__ __forceinline__ size_t row_slot(const Cache& c, int page, int head, int r) { return ((size_t)page * c.kv_heads + head) * kRows + r; }
+__device__ __forceinline__ int held(const Cache& c, const int32_t* lens, int b, int most) {
+    const int n = lens[b];
+    if ((unsigned)n <= (unsigned)most) return n;
+    raise(c, kBadCount);
+    return n < 0 ? 0 : most;
+}
+
+// nibble of channel i of a word's eight
+__host__ __device__ constexpr int nibble(int i) { return (i >> 1) + 4 * (i & 1); }
+// word of a key row that holds channels 8 w .. 8 w + 7
+template <int D>
+__host__ __device__ constexpr int key_word(int w) { return (w & 7) / 2 * (2 * Tile<D>::G) + (w >> 3) * 2 + (w & 1); }
+
+template <typename T> struct Num;
+template <> struct Num<__nv_bfloat16> {
+    static __device__ __forceinline__ float2 two(uint32_t v) { return make_float2(bf16lo(v), bf16hi(v)); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16(a, b); }
+};
+template <> struct Num<__half> {
+    static __device__ __forceinline__ float2 two(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        __half2 p = __floats2half2_rn(a, b);
+        return *reinterpret_cast<uint32_t*>(&p);
+    }
+};
+
+struct AppendParams {
+    int max_rows;
+    const int32_t *cu_rows, *lens_in;
+    int32_t* lens_out;
+    const void *q, *k, *v;
+    int64_t q_stride, k_stride, v_stride;
+    int norm;
+    float eps;
+    const void *q_norm, *k_norm;
+    int rot_dims, neighbours, axes, section0, section1;
+    const double* inv_freq;
+    const int32_t *positions, *token_index;
+    void *q_out, *k_held, *v_held;
+    int32_t* index;
+    float* mass;
+};
+
+constexpr int kAppendThreads = 256;
+
+// Channels turned: (a, b) -> (a cos - b sin, b cos + a sin), three roundings each.
+__device__ __forceinline__ float turn(float a, float c, float b, float s, bool plus) {
+    const float x = __fmul_rn(a, c), y = __fmul_rn(b, s);
+    return plus ? __fadd_rn(x, y) : __fsub_rn(x, y);
+}
+
+// grid (rows, parts of the row's heads); a warp has one head at a time, a lane D / 32 neighbouring channels of it.
+template <typename T, int D>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const Cache c, const AppendParams p, int heads_per_block) {
+    constexpr int E = D / 32;
+    using L = Tile<D>;
+    __shared__ float2 rot[D / 2];
+    __shared__ int owner;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int cap = c.max_pages * kRows;
+    if (tid == 0) owner = -1;
+    __syncthreads();
+    for (int b = tid; b < c.batch; b += kAppendThreads) {
+        const int lo = p.cu_rows[b], hi = p.cu_rows[b + 1];
+        if (row >= lo && row < hi && row < p.max_rows) owner = b;
+        if (row == 0 && blockIdx.y == 0) {
+            const int n = max(0, min(hi, p.max_rows) - max(min(lo, p.max_rows), 0)), have = held(c, p.lens_in, b, cap);
+            p.lens_out[b] = min(cap - have, n) + have;
+            if (n > cap - have) raise(c, kFull);
+        }
+    }
+    if (p.rot_dims > 0 && row < p.max_rows)
+        for (int i = tid; i < p.rot_dims / 2; i += kAppendThreads) {
+            const int axis = p.axes == 1 || i < p.section0 ? 0 : i < p.section0 + p.section1 ? 1 : 2;
+            double s, co;
+            sincos((double)p.positions[(size_t)axis * p.max_rows + row] * p.inv_freq[i], &s, &co);
+            rot[i] = make_float2((float)co, (float)s);
+        }
+    __syncthreads();
+    if (owner < 0) return;
+    const int b = owner;
+    const int64_t behind = held(c, p.lens_in, b, cap) + ((int64_t)row - p.cu_rows[b]);
+    const int place = behind < cap ? (int)behind : cap, page = place < cap ? page_of(c, b, place / kRows) : -1, r = place % kRows;
+    const int heads = c.q_heads + 2 * c.kv_heads, last = min(heads, ((int)blockIdx.y + 1) * heads_per_block);
+    for (int h = blockIdx.y * heads_per_block + warp; h < last; h += kAppendThreads / 32) {
+        const int kind = h < c.q_heads ? 0 : h < c.q_heads + c.kv_heads ? 1 : 2;      // q, k, v
+        const int hh = kind == 0 ? h : kind == 1 ? h - c.q_heads : h - c.q_heads - c.kv_heads;
+        if (kind == 0 && p.q == nullptr) continue;
+        const T* src = kind == 0 ? (const T*)p.q + row * p.q_stride : kind == 1 ? (const T*)p.k + row * p.k_stride : (const T*)p.v + row * p.v_stride;
+        src += (size_t)hh * D + lane * E;
+        float x[E];
+        if constexpr (E == 4) {
+            const uint2 w = *reinterpret_cast<const uint2*>(src);
+            const float2 lo = Num<T>::two(w.x), hi = Num<T>::two(w.y);
+            x[0] = lo.x; x[1] = lo.y; x[2] = hi.x; x[3] = hi.y;
+        } else {
+            const float2 lo = Num<T>::two(*reinterpret_cast<const uint32_t*>(src));
+            x[0] = lo.x; x[1] = lo.y;
+        }
+        if (kind < 2 && p.norm) {
+            double sq = 0.0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) sq += (double)x[e] * (double)x[e];
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+            const float f = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn((float)(sq / D), p.eps)));
+            const T* w = (const T*)(kind == 0 ? p.q_norm : p.k_norm);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                x[e] = __fmul_rn(x[e], f);
+                if (w != nullptr) x[e] = __fmul_rn(x[e], (float)w[lane * E + e]);
+            }
+        }
+        if (kind < 2 && p.rot_dims > 0) {
+            const int c0 = lane * E, half = p.rot_dims / 2;
+            if (p.neighbours) {
+                if (c0 < p.rot_dims) {
+#pragma unroll
+                    for (int e = 0; e < E; e += 2) {
+                        const float2 cs = rot[(c0 + e) / 2];
+                        const float a = x[e], bb = x[e + 1];
+                        x[e] = turn(a, cs.x, bb, cs.y, false);
+                        x[e + 1] = turn(bb, cs.x, a, cs.y, true);
+                    }
+                }
+            } else {
+                const bool second = c0 >= half;
+                const int from = second ? lane - half / E : lane + half / E;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float o = __shfl_sync(0xffffffffu, x[e], from & 31);
+                    if (c0 < p.rot_dims) {
+                        const float2 cs = rot[(second ? c0 - half : c0) + e];
+                        x[e] = turn(x[e], cs.x, o, cs.y, second);
+                    }
+                }
+            }
+        }
+        auto put = [&](void* out, int n_heads) {
+            T* dst = (T*)out + ((size_t)row * n_heads + hh) * D + lane * E;
+            if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(Num<T>::pack(x[0], x[1]), Num<T>::pack(x[2], x[3]));
+            else *reinterpret_cast<uint32_t*>(dst) = Num<T>::pack(x[0], x[1]);
+        };
+        if (kind == 0) { put(p.q_out, c.q_heads); continue; }
+        float lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            x[e] = x[e] != x[e] ? 0.0f : fminf(fmaxf(x[e], -65504.0f), 65504.0f);
+            lo = fminf(lo, x[e]);
+            hi = fmaxf(hi, x[e]);
+        }
+#pragma unroll
+        for (int o = kGroup / E / 2; o > 0; o >>= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        const __half sh = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f)), mh = __float2half_rn(lo);
+        const float s = __half2float(sh), m = __half2float(mh);
+        uint32_t word = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float code = s > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[e], m), s)), 0.0f), 15.0f) : 0.0f;
+            x[e] = __fadd_rn(m, __fmul_rn(s, code));
+            const int i = (lane * E + e) & 7;
+            word |= (uint32_t)(int)code << (4 * ((i >> 1) + 4 * (i & 1)));
+        }
+        word |= __shfl_xor_sync(0xffffffffu, word, 1);
+        if constexpr (E == 2) word |= __shfl_xor_sync(0xffffffffu, word, 2);
+        void* want = kind == 1 ? p.k_held : p.v_held;
+        if (want != nullptr) put(want, c.kv_heads);
+        if (page < 0) continue;
+        uint8_t* tile = tile_of<D>(c, page, hh);
+        const int w = lane * E / 8;
+        if (lane * E % 8 == 0) {
+            uint32_t* codes = reinterpret_cast<uint32_t*>(tile + (kind == 1 ? L::K_CODES : L::V_CODES)) + r * L::WORDS;
+            codes[kind == 1 ? key_word<D>(w) : w] = word;
+        }
+        if (lane * E % kGroup == 0) {
+            __half2* par = reinterpret_cast<__half2*>(tile + (kind == 1 ? L::K_PARAMS : L::V_PARAMS)) + r * L::G;
+            par[lane * E / kGroup] = __halves2half2(sh, mh);
+        }
+        if (kind == 1 && lane == 0) {
+            if (p.index != nullptr) p.index[row_slot(c, page, hh, r)] = p.token_index != nullptr ? p.token_index[row] : place;
+            if (p.mass != nullptr) p.mass[row_slot(c, page, hh, r)] = 0.0f;
+        }
+    }
+}
+
+// What a word of codes stands for: eight channels, rounded once.
+template <typename T>
+__device__ __forceinline__ uint4 word_values(uint32_t w, __half2 par) {
+    const float s = __low2float(par), m = __high2float(par);
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(m, __fmul_rn(s, (float)((w >> (4 * nibble(i))) & 15u)));
+    return make_uint4(Num<T>::pack(x[0], x[1]), Num<T>::pack(x[2], x[3]), Num<T>::pack(x[4], x[5]), Num<T>::pack(x[6], x[7]));
+}
+
+constexpr int kReadThreads = 256;
+
+// grid (pages of the range x kv heads, batch); a thread has one word of keys or values at a time, in the order of the output.
+template <typename T, int D>
+__global__ void __launch_bounds__(kReadThreads) read_kernel(const Cache c, const int32_t* lens, int first, int rows, T* k_out, T* v_out) {
+    using L = Tile<D>;
+    constexpr int PER = kRows * L::WORDS / kReadThreads;
+    const int b = blockIdx.y, h = blockIdx.x % c.kv_heads, k = first / kRows + blockIdx.x / c.kv_heads;
+    const int n = min(held(c, lens, b, c.max_pages * kRows), first + rows);
+    if (k * kRows >= n) return;
+    const int page = page_of(c, b, k);
+    if (page < 0) return;
+    const uint8_t* tile = tile_of<D>(c, page, h);
+    const uint32_t *kc = reinterpret_cast<const uint32_t*>(tile + L::K_CODES), *vc = reinterpret_cast<const uint32_t*>(tile + L::V_CODES);
+    const __half2 *kp = reinterpret_cast<const __half2*>(tile + L::K_PARAMS), *vp = reinterpret_cast<const __half2*>(tile + L::V_PARAMS);
+    uint32_t kw[PER], vw[PER];
+    __half2 ks[PER], vs[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int at = i * kReadThreads + threadIdx.x, r = at / L::WORDS, w = at % L::WORDS;
+        if (k_out != nullptr) { kw[i] = kc[r * L::WORDS + key_word<D>(w)]; ks[i] = kp[r * L::G + w / 8]; }
+        if (v_out != nullptr) { vw[i] = vc[r * L::WORDS + w]; vs[i] = vp[r * L::G + w / 8]; }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int at = i * kReadThreads + threadIdx.x, r = at / L::WORDS, w = at % L::WORDS, row = k * kRows + r;
+        if (row < first || row >= n) continue;
+        const size_t dst = (((size_t)b * rows + (row - first)) * c.kv_heads + h) * D + w * 8;
+        if (k_out != nullptr) *reinterpret_cast<uint4*>(k_out + dst) = word_values<T>(kw[i], ks[i]);
+        if (v_out != nullptr) *reinterpret_cast<uint4*>(v_out + dst) = word_values<T>(vw[i], vs[i]);
+    }
+}
+
+}  // namespace kv4
+}  // namespace efm
