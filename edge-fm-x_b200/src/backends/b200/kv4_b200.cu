@@ -56,6 +56,13 @@ private:
 struct DeviceInfo { int sms = 0, smem = 0; };
 constexpr int kEvictSmemReserve = 12 * 1024;          // static shared memory of the ordering kernel, rounded up
 
+template <typename T, int D>
+cudaError_t more_smem() {
+    cudaError_t e = cudaFuncSetAttribute(kv4::attend_few_kernel<T, D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::FewCfg<D, 1>::SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_few_kernel<T, D, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::FewCfg<D, 2>::SMEM);
+    return e;
+}
+
 // Once per device: architecture, sizes, shared memory beyond the default.
 efm_status device_info(const char* call, int device, DeviceInfo& info) {
     static std::atomic<int64_t> known[64];
@@ -70,6 +77,10 @@ efm_status device_info(const char* call, int device, DeviceInfo& info) {
         if (e != cudaSuccess) return cuda_fail(nullptr, e, call);
         if (major != 10 || minor != 0) return fail(nullptr, EFM_ERR_CUDA, std::string(call) + ": needs an sm_100 device");
         e = cudaFuncSetAttribute(kv4::evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem - kEvictSmemReserve);
+        if (e == cudaSuccess) e = more_smem<__nv_bfloat16, 64>();
+        if (e == cudaSuccess) e = more_smem<__nv_bfloat16, 128>();
+        if (e == cudaSuccess) e = more_smem<__half, 64>();
+        if (e == cudaSuccess) e = more_smem<__half, 128>();
         if (e != cudaSuccess) return cuda_fail(nullptr, e, call);
         k = ((int64_t)sms << 32) | smem;
         known[device].store(k, std::memory_order_release);
@@ -112,9 +123,31 @@ efm_status check_attention(const char* call, const efm_kv4_cache* c, const efm_k
     if (!(a->scale > 0.f) || !(a->scale < INFINITY)) return bad(call, "scale: positive and finite");
     return EFM_OK;
 }
-int64_t attention_bytes(const efm_kv4_cache* c, const efm_kv4_attention* a) {
-    return a->mass_out != nullptr ? (int64_t)a->max_rows * c->q_heads * (int64_t)sizeof(float2) : 0;
+
+// How a call's work is dealt: tiles of 8 nt query rows, blocks of `chunk` pages.
+struct AttnPlan {
+    int max_new, max_len, nt, tiles, chunk, chunks;
+    int64_t stats, part;                              // floats: maxima and sums, weighted values of the blocks of a row
+};
+constexpr int kSms = 148, kWaves = 2;                  // of the one GPU these kernels are built for
+
+AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
+    AttnPlan p{};
+    p.max_new = std::min(a->max_new, a->max_rows);
+    p.max_len = a->max_len > 0 ? a->max_len : (int)capacity(c);
+    const int64_t rows = (int64_t)p.max_new * (c->q_heads / c->kv_heads);
+    p.nt = rows <= 8 ? 1 : 2;
+    p.tiles = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
+    const int64_t pages = std::max(1, (p.max_len + kRows - 1) / kRows), base = std::max<int64_t>(1, (int64_t)c->batch * c->kv_heads * p.tiles);
+    const int64_t blocks = (int64_t)kSms * (p.nt == 1 ? 3 : 2) * kWaves;
+    p.chunk = (int)std::min<int64_t>(kv4::kMaxChunk, std::max<int64_t>(kv4::kWarps, round_up((pages * base + blocks - 1) / blocks, kv4::kWarps)));
+    p.chunks = (int)((pages + p.chunk - 1) / p.chunk);
+    const int64_t all = (int64_t)p.chunks * c->batch * p.max_new * c->q_heads;
+    p.stats = p.chunks > 1 || a->mass_out != nullptr ? round_up(2 * all, 4) : 0;
+    p.part = p.chunks > 1 ? all * c->head_dim : 0;
+    return p;
 }
+int64_t attention_bytes(const AttnPlan& p) { return 4 * (p.stats + p.part); }
 
 efm_status check_evict(const char* call, const efm_kv4_evict* a) {
     if (a == nullptr || a->struct_size != (int32_t)sizeof(efm_kv4_evict)) return bad(call, "struct_size does not match this header");
@@ -150,7 +183,7 @@ efm_status efm_b200_kv4_attention_workspace(const efm_kv4_cache* cache, const ef
         efm_status st = check_cache(call, cache);
         if (st == EFM_OK) st = check_attention(call, cache, a);
         if (st == EFM_OK && bytes == nullptr) st = bad(call, "bytes is null");
-        if (st == EFM_OK) *bytes = attention_bytes(cache, a);
+        if (st == EFM_OK) *bytes = attention_bytes(plan_attention(cache, a));
         return st;
     });
 }
@@ -236,25 +269,37 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
         if (a->cu_rows == nullptr || a->lens == nullptr || !aligned(a->cu_rows, 4) || !aligned(a->lens, 4)) return bad(call, "cu_rows and lens are needed");
         if (a->max_rows > 0 && (a->q == nullptr || a->out == nullptr || !aligned(a->q, 16) || !aligned(a->out, 16))) return bad(call, "q and out are needed, 16-byte aligned");
         if (!aligned(a->mass_in, 4) || !aligned(a->mass_out, 4)) return bad(call, "mass: aligned to 4 bytes");
-        const int64_t need = attention_bytes(cache, a);
+        const AttnPlan plan = plan_attention(cache, a);
+        const int64_t need = attention_bytes(plan);
         if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need || !aligned(a->workspace, 16)))
             return bad(call, "workspace: 16-byte aligned, as large as efm_b200_kv4_attention_workspace says");
+        if ((int64_t)plan.tiles * plan.chunks > 0x7fffffff) return bad(call, "too many rows");
         OnDevice on;
         DeviceInfo info;
         if ((st = on.enter(call, cache->pool)) != EFM_OK || (st = device_info(call, on.device, info)) != EFM_OK) return st;
         kv4::AttnParams p{};
-        p.max_rows = a->max_rows; p.max_new = std::min(a->max_new, a->max_rows);
-        p.max_len = a->max_len > 0 ? a->max_len : (int)capacity(cache);
+        p.max_rows = a->max_rows; p.max_new = plan.max_new; p.max_len = plan.max_len;
         p.cu_rows = a->cu_rows; p.lens = a->lens; p.q = a->q; p.out = a->out;
         p.scale_log2 = a->scale * 1.4426950408889634f;
         p.mass_in = a->mass_in; p.mass_out = a->mass_out;
-        p.stats = a->mass_out != nullptr ? (float2*)a->workspace : nullptr;
+        p.chunk = plan.chunk; p.chunks = plan.chunks; p.rows = plan.max_new;
+        p.stats = plan.stats > 0 ? (float2*)a->workspace : nullptr;
+        p.part = plan.part > 0 ? (float*)a->workspace + plan.stats : nullptr;
         Launcher L = on_stream(stream);
         by_type(cache, [&](auto t, auto d) {
             using T = decltype(t);
             constexpr int D = decltype(d)::value;
-            if (p.max_new > 0) L.launch(kv4::attend_plain_kernel<T, D>, dim3(p.max_new, cache->q_heads, cache->batch), dim3(128), 0, device_cache(cache), p);
-            if (p.mass_out != nullptr) L.launch(kv4::mass_plain_kernel<T, D>, dim3((p.max_len + 7) / 8, cache->kv_heads, cache->batch), dim3(256), 0, device_cache(cache), p);
+            const dim3 grid(plan.tiles * plan.chunks, cache->kv_heads, cache->batch), block(kv4::kWarps * 32);
+            const kv4::Cache c = device_cache(cache);
+            if (plan.tiles > 0 && plan.nt == 1) L.launch(kv4::attend_few_kernel<T, D, 1>, grid, block, kv4::FewCfg<D, 1>::SMEM, c, p);
+            if (plan.tiles > 0 && plan.nt == 2) L.launch(kv4::attend_few_kernel<T, D, 2>, grid, block, kv4::FewCfg<D, 2>::SMEM, c, p);
+            const int groups = p.mass_out != nullptr ? (plan.max_len + kRows * kv4::kWarps - 1) / (kRows * kv4::kWarps) : 0;
+            const int64_t rows = (int64_t)plan.max_new * (cache->q_heads / cache->kv_heads);
+            const int merges = plan.chunks > 1 ? (int)std::min<int64_t>(64, (rows + kv4::kWarps - 1) / kv4::kWarps) : 0;
+            if (groups + merges > 0) {
+                L.pdl = true;
+                L.launch(kv4::attend_finish_kernel<T, D>, dim3(groups + merges, cache->kv_heads, cache->batch), block, kv4::FinishCfg<D>::SMEM, c, p, groups);
+            }
         });
         return launched(call, L);
     });

@@ -122,8 +122,9 @@ def normed(x, eps, w):
     return x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * w
 
 
-def attend(q, k, v, scale):
-    """q [n, heads, d], k / v [kv heads, L, d] (float64), row i sees L - n + i + 1 rows.  -> out, weights [heads, n, L], sum of p |v|."""
+def attend(q, k, v, scale, spread=None):
+    """q [n, heads, d], k / v [kv heads, L, d] (float64), row i sees L - n + i + 1 rows.  -> out, weights [heads, n, L], sum of p max(|v|, spread)."""
+    big = np.abs(v) if spread is None else np.maximum(np.abs(v), spread)
     n, qh, d = q.shape
     L, g = k.shape[1], qh // k.shape[0]
     out, size, w = np.zeros((n, qh, d)), np.zeros((n, qh, d)), np.zeros((qh, n, L))
@@ -134,7 +135,7 @@ def attend(q, k, v, scale):
             p = np.exp(s - s.max())
             p /= p.sum()
             w[h, i, :see] = p
-            out[i, h], size[i, h] = p @ v[h // g, :see], p @ np.abs(v[h // g, :see])
+            out[i, h], size[i, h] = p @ v[h // g, :see], p @ big[h // g, :see]
     return out, w, size
 
 
@@ -239,6 +240,14 @@ class KV4:
         pages = self.np_table[b, :-(-n // ROWS)]
         tiles = self.pool[self.torch.from_numpy(pages.astype(np.int64)).to(self.dev)].cpu().numpy()
         return [values(*u).swapaxes(0, 1).reshape(self.kh, -1, self.d)[:, :n] for u in unpack(tiles, self.d)]
+
+    def spread(self, b, n):
+        """|scale (code - 8)| of sequence b's values: what a weight multiplies once the centre of the codes is taken out."""
+        if n == 0:
+            return np.zeros((self.kh, 0, self.d))
+        tiles = self.pool[self.torch.from_numpy(self.np_table[b, :-(-n // ROWS)].astype(np.int64)).to(self.dev)].cpu().numpy()
+        codes, scale, _ = unpack(tiles, self.d)[1]
+        return np.abs(np.repeat(scale, GROUP, -1) * (codes - 8)).swapaxes(0, 1).reshape(self.kh, -1, self.d)[:, :n]
 
     def rows_of(self, t, b, n):
         """t [pages, kv heads, 64] -> [kv heads, n] of sequence b."""

@@ -1,9 +1,11 @@
 """GPU: the operators of the 4-bit cache through the C ABI against the plain 64-bit statement in kv4_util.
 
 Tolerances.  An output rounded to bf16 or fp16 is off by half a step, eps/2 of its value.  Before that, attention's weights may be rounded to
-fp16 (2^-11 of each, so 2^-11 of sum p |v| at most) and everything else is 32 bits: scores of up to some tens come out within 2^-18, which
-multiplies a weight by at most 1 + 2^-17.  Where many rows share tiles the dequantised k and v are rounded to fp16 as well: another 2^-11 of
-sum p |v|, and a score is off by 2^-11 sum |q k| scale at most.  attention_bound() is that sum."""
+fp16, 2^-11 of each.  With v = c + scale (code - 8), c = min + 8 scale, a rounded weight p (1 + e) may stand before all of v, which is off by
+e p |v|, or before scale (code - 8) alone while c keeps the unrounded one, which is off by e p |scale (code - 8)|: at most 2^-11 times the sum
+of p max(|v|, |scale (code - 8)|).  Everything else is 32 bits: scores of up to some tens come out within 2^-18, which multiplies a weight by
+at most 1 + 2^-17.  Where many rows share tiles the dequantised k and v are rounded to fp16 as well: another 2^-11 of sum p |v|, and a score
+is off by 2^-11 sum |q k| scale at most.  attention_bound() is that sum."""
 import ctypes as C
 import math
 
@@ -228,7 +230,7 @@ def run_attention(c, counts, lens, dtype, mass=False, pad=2, max_len=0, shared_t
     for b, (m, L) in enumerate(zip(counts, lens)):
         k, v = c.held(b, L)
         x = host(q[row:row + m])
-        ref, w, size = kv.attend(x, k, v, scale)
+        ref, w, size = kv.attend(x, k, v, scale, c.spread(b, L))
         if m and L:
             off = np.abs(got[row:row + m] - ref)
             bound = attention_bound(dtype, ref, size, x, k, scale, shared_tiles)
@@ -300,7 +302,7 @@ def test_attention_large_and_small_queries():
         out = torch.zeros_like(q)
         lens = c.ints([100])
         c.do("attention", c.attention_args([1], lens, q, out, 1))
-        ref, _, size = kv.attend(host(q), *c.held(0, 100), 1.0 / math.sqrt(128))
+        ref, _, size = kv.attend(host(q), *c.held(0, 100), 1.0 / math.sqrt(128), c.spread(0, 100))
         if s < 1000:                                       # scores of thousands: only the order of the two largest counts
             slack = 2.0 ** -18 * max(1.0, s * 30)
             assert (np.abs(host(out) - ref) <= HALF_STEP["bf16"] * np.abs(ref) + (2.0 ** -11 + 2 * slack) * size).all()
@@ -565,7 +567,7 @@ def test_decoding_under_a_budget_eager_and_captured():
             assert got == (eager.budget if n > eager.limit else n)
             if got == n and t % 10 == 0:
                 k, v = c.held(b, n)
-                ref, _, size = kv.attend(q[b:b + 1], k, v, 1 / 8)
+                ref, _, size = kv.attend(q[b:b + 1], k, v, 1 / 8, c.spread(b, n))
                 assert (np.abs(host(eager.out)[b:b + 1] - ref) <= attention_bound("bf16", ref, size, q[b:b + 1], k, 1 / 8)).all()
     n = eager.a.tolist()
     assert eager.c.status.item() == 0 and n == [100 + (230 - 141) % 41] * 3
@@ -628,7 +630,7 @@ def test_portions_and_decoded_tokens_of_one_prompt_agree():
         outs.append(host(out))
         pools.append(c.pool.clone())
         k, v = c.held(0, n)
-        ref, _, size = kv.attend(host(q), k, v, 1 / math.sqrt(d))
+        ref, _, size = kv.attend(host(q), k, v, 1 / math.sqrt(d), c.spread(0, n))
         assert (np.abs(outs[-1] - ref) <= attention_bound("bf16", ref, size, host(q), k, 1 / math.sqrt(d), True)).all()
     assert torch.equal(pools[0], pools[1]) and torch.equal(pools[0], pools[2])
 
