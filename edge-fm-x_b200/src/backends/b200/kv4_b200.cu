@@ -124,12 +124,14 @@ efm_status check_attention(const char* call, const efm_kv4_cache* c, const efm_k
     return EFM_OK;
 }
 
-// How a call's work is dealt: tiles of 8 nt query rows, blocks of `chunk` pages.
+// What a call needs: tiles of 8 nt packed query rows, and the parts of its workspace, in floats.
 struct AttnPlan {
-    int max_new, max_len, nt, tiles, chunk, chunks;
-    int64_t stats, part;                              // floats: maxima and sums, weighted values of the blocks of a row
+    int max_new, max_len, nt, blocks;
+    bool scores;                                      // attend_few leaves its scores for the summed weights
+    int64_t stats, part_stats, part, score_ld, score;
+    int64_t bytes() const { return 4 * (stats + part_stats + part + score); }
 };
-constexpr int kSms = 148, kWaves = 2;                  // of the one GPU these kernels are built for
+constexpr int kSms = 148;                              // of the GPU these kernels are built for
 
 AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
     AttnPlan p{};
@@ -137,17 +139,16 @@ AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
     p.max_len = a->max_len > 0 ? a->max_len : (int)capacity(c);
     const int64_t rows = (int64_t)p.max_new * (c->q_heads / c->kv_heads);
     p.nt = rows <= 8 ? 1 : 2;
-    p.tiles = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
-    const int64_t pages = std::max(1, (p.max_len + kRows - 1) / kRows), base = std::max<int64_t>(1, (int64_t)c->batch * c->kv_heads * p.tiles);
-    const int64_t blocks = (int64_t)kSms * (p.nt == 1 ? 3 : 2) * kWaves;
-    p.chunk = (int)std::min<int64_t>(kv4::kMaxChunk, std::max<int64_t>(kv4::kWarps, round_up((pages * base + blocks - 1) / blocks, kv4::kWarps)));
-    p.chunks = (int)((pages + p.chunk - 1) / p.chunk);
-    const int64_t all = (int64_t)p.chunks * c->batch * p.max_new * c->q_heads;
-    p.stats = p.chunks > 1 || a->mass_out != nullptr ? round_up(2 * all, 4) : 0;
-    p.part = p.chunks > 1 ? all * c->head_dim : 0;
+    const int64_t R = 8 * p.nt, tiles = (rows + R - 1) / R, units = std::max(1, (p.max_len + kRows - 1) / kRows) * tiles * c->kv_heads * (int64_t)c->batch;
+    p.blocks = (int)std::max<int64_t>(1, std::min<int64_t>(kSms * (p.nt == 1 ? 3 : 2), (units + kv4::kWarps - 1) / kv4::kWarps));
+    p.scores = a->mass_out != nullptr && rows <= R;
+    p.stats = a->mass_out != nullptr ? round_up(2 * (int64_t)c->batch * p.max_new * c->q_heads, 4) : 0;
+    p.part_stats = 2 * 2 * (int64_t)p.blocks * R;
+    p.part = 2 * (int64_t)p.blocks * R * c->head_dim;
+    p.score_ld = round_up(p.max_len, kRows);
+    p.score = p.scores ? (int64_t)c->batch * c->kv_heads * R * p.score_ld : 0;
     return p;
 }
-int64_t attention_bytes(const AttnPlan& p) { return 4 * (p.stats + p.part); }
 
 efm_status check_evict(const char* call, const efm_kv4_evict* a) {
     if (a == nullptr || a->struct_size != (int32_t)sizeof(efm_kv4_evict)) return bad(call, "struct_size does not match this header");
@@ -183,7 +184,7 @@ efm_status efm_b200_kv4_attention_workspace(const efm_kv4_cache* cache, const ef
         efm_status st = check_cache(call, cache);
         if (st == EFM_OK) st = check_attention(call, cache, a);
         if (st == EFM_OK && bytes == nullptr) st = bad(call, "bytes is null");
-        if (st == EFM_OK) *bytes = attention_bytes(plan_attention(cache, a));
+        if (st == EFM_OK) *bytes = plan_attention(cache, a).bytes();
         return st;
     });
 }
@@ -270,10 +271,8 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
         if (a->max_rows > 0 && (a->q == nullptr || a->out == nullptr || !aligned(a->q, 16) || !aligned(a->out, 16))) return bad(call, "q and out are needed, 16-byte aligned");
         if (!aligned(a->mass_in, 4) || !aligned(a->mass_out, 4)) return bad(call, "mass: aligned to 4 bytes");
         const AttnPlan plan = plan_attention(cache, a);
-        const int64_t need = attention_bytes(plan);
-        if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need || !aligned(a->workspace, 16)))
+        if (a->workspace == nullptr || a->workspace_bytes < plan.bytes() || !aligned(a->workspace, 16))
             return bad(call, "workspace: 16-byte aligned, as large as efm_b200_kv4_attention_workspace says");
-        if ((int64_t)plan.tiles * plan.chunks > 0x7fffffff) return bad(call, "too many rows");
         OnDevice on;
         DeviceInfo info;
         if ((st = on.enter(call, cache->pool)) != EFM_OK || (st = device_info(call, on.device, info)) != EFM_OK) return st;
@@ -282,24 +281,30 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
         p.cu_rows = a->cu_rows; p.lens = a->lens; p.q = a->q; p.out = a->out;
         p.scale_log2 = a->scale * 1.4426950408889634f;
         p.mass_in = a->mass_in; p.mass_out = a->mass_out;
-        p.chunk = plan.chunk; p.chunks = plan.chunks; p.rows = plan.max_new;
-        p.stats = plan.stats > 0 ? (float2*)a->workspace : nullptr;
-        p.part = plan.part > 0 ? (float*)a->workspace + plan.stats : nullptr;
+        p.few_rows = 0x7fffffff; p.blocks = plan.blocks; p.rows = plan.max_new;
+        float* ws = (float*)a->workspace;
+        p.stats = plan.stats > 0 ? (float2*)ws : nullptr;
+        p.part_stats = (float2*)(ws + plan.stats);
+        p.part = ws + plan.stats + plan.part_stats;
+        p.scores = plan.scores ? p.part + plan.part : nullptr;
+        p.score_ld = plan.score_ld;
         Launcher L = on_stream(stream);
         by_type(cache, [&](auto t, auto d) {
             using T = decltype(t);
             constexpr int D = decltype(d)::value;
-            const dim3 grid(plan.tiles * plan.chunks, cache->kv_heads, cache->batch), block(kv4::kWarps * 32);
+            const dim3 block(kv4::kWarps * 32);
             const kv4::Cache c = device_cache(cache);
-            if (plan.tiles > 0 && plan.nt == 1) L.launch(kv4::attend_few_kernel<T, D, 1>, grid, block, kv4::FewCfg<D, 1>::SMEM, c, p);
-            if (plan.tiles > 0 && plan.nt == 2) L.launch(kv4::attend_few_kernel<T, D, 2>, grid, block, kv4::FewCfg<D, 2>::SMEM, c, p);
-            const int groups = p.mass_out != nullptr ? (plan.max_len + kRows * kv4::kWarps - 1) / (kRows * kv4::kWarps) : 0;
             const int64_t rows = (int64_t)plan.max_new * (cache->q_heads / cache->kv_heads);
-            const int merges = plan.chunks > 1 ? (int)std::min<int64_t>(64, (rows + kv4::kWarps - 1) / kv4::kWarps) : 0;
-            if (groups + merges > 0) {
-                L.pdl = true;
-                L.launch(kv4::attend_finish_kernel<T, D>, dim3(groups + merges, cache->kv_heads, cache->batch), block, kv4::FinishCfg<D>::SMEM, c, p, groups);
-            }
+            const int merges = plan.blocks > 1 ? (int)std::min<int64_t>(64, rows) : 0, masses = plan.scores ? (plan.max_len + kv4::kMassTokens - 1) / kv4::kMassTokens : 0;
+            const dim3 join(merges + masses, cache->kv_heads, cache->batch);
+            if (rows > 0 && plan.nt == 1) L.launch(kv4::attend_few_kernel<T, D, 1>, dim3(plan.blocks), block, kv4::FewCfg<D, 1>::SMEM, c, p);
+            if (rows > 0 && plan.nt == 2) L.launch(kv4::attend_few_kernel<T, D, 2>, dim3(plan.blocks), block, kv4::FewCfg<D, 2>::SMEM, c, p);
+            L.pdl = rows > 0;
+            if (join.x > 0 && plan.nt == 1) L.launch(kv4::attend_merge_kernel<T, D, 8>, join, block, 0, c, p, masses);
+            if (join.x > 0 && plan.nt == 2) L.launch(kv4::attend_merge_kernel<T, D, 16>, join, block, 0, c, p, masses);
+            if (p.mass_out != nullptr && !plan.scores)
+                L.launch(kv4::attend_mass_kernel<T, D>, dim3((plan.max_len + kRows * kv4::kWarps - 1) / (kRows * kv4::kWarps), cache->kv_heads, cache->batch), block,
+                         kv4::MassCfg<D>::SMEM, c, p);
         });
         return launched(call, L);
     });

@@ -20,11 +20,14 @@ struct AttnParams {
     float scale_log2;         // scale * log2(e): scores in units of log2
     const float* mass_in;
     float* mass_out;
-    int chunk;                // pages a block takes
-    int chunks;               // blocks of the longest sequence
-    int rows;                 // new rows a sequence has in the buffers below
-    float2* stats;            // [chunks, batch, rows, q_heads] (maximum, sum) of a row's weights in a chunk; null: not wanted
-    float* part;              // [chunks, batch, rows, q_heads, D] its weighted values
+    int few_rows;             // sequences with at most this many packed rows (new rows x heads of a group) are attend_few's
+    int blocks;               // attend_few's blocks
+    float2* stats;            // [batch, rows, q_heads] (maximum, sum) of a row's weights, where one block had all its keys; null: not wanted
+    int rows;                 // new rows a sequence has in stats
+    float2* part_stats;       // [2 blocks][8 nt] the same of the keys a block had, and
+    float* part;              // [2 blocks][8 nt][D] its weighted values: slot 0 is the piece its range begins with, slot 1 the one it ends with
+    float* scores;            // [batch, kv_heads, 8 nt][score_ld] scores in units of log2; null: not wanted
+    int64_t score_ld;
 };
 
 // New rows and cache rows of sequence b, cut to what the call was given.
@@ -39,11 +42,30 @@ __device__ __forceinline__ Entry entry_of(const Cache& c, const AttnParams& p, i
     e.len = held(c, p.lens, b, min(p.max_len, c.max_pages * kRows));
     return e;
 }
-__device__ __forceinline__ size_t part_row(const Cache& c, const AttnParams& p, int chunk, int b, int i, int head) {
-    return (((size_t)chunk * c.batch + b) * p.rows + i) * c.q_heads + head;
+__device__ __forceinline__ size_t stat_row(const Cache& c, const AttnParams& p, int b, int i, int head) {
+    return ((size_t)b * p.rows + i) * c.q_heads + head;
 }
 
-constexpr int kWarps = 4, kMaxChunk = 32 * kWarps;      // a lane knows one page of its warp's
+constexpr int kWarps = 4;
+
+// How attend_few's work is dealt: every page of every (sequence, kv head, tile of R packed rows) is a unit, in that order; block w has the
+// units [w step, (w + 1) step).  Lengths are known on the device only, so every block adds them up for itself.
+struct Deal { int64_t before, all; };          // units ahead of sequence b, and altogether
+struct Share { int64_t units; int tiles, pages; };
+template <int R>
+__device__ __forceinline__ Share share_of(const Cache& c, const AttnParams& p, int b, int group) {
+    const Entry e = entry_of(c, p, b);
+    const int rows = e.n * group;
+    Share s;
+    s.pages = max(1, (e.len + kRows - 1) / kRows);                               // a row that sees nothing is somebody's to clear
+    s.tiles = rows <= p.few_rows ? (rows + R - 1) / R : 0;
+    s.units = (int64_t)s.tiles * s.pages * c.kv_heads;
+    return s;
+}
+__device__ __forceinline__ int64_t step_of(const AttnParams& p, int64_t all) {
+    const int64_t even = (all + p.blocks - 1) / p.blocks;
+    return even > kWarps ? even : kWarps;
+}
 
 // ---- fragments -------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -130,7 +152,7 @@ struct QueryTile {
             for (int k = 0; k < 2; ++k) sum[g][k] = __shfl_sync(0xffffffffu, s[g], (2 * j + k) * 4);
         }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) unit[k] = __shfl_sync(0xffffffffu, down * scale_log2, (2 * j + k) * 4);
+        for (int k = 0; k < 2; ++k) unit[k] = __shfl_sync(0xffffffffu, fmaxf(down * scale_log2, 1.2e-38f), (2 * j + k) * 4);     // times -inf: -inf
     }
 };
 
@@ -138,16 +160,28 @@ struct QueryTile {
 // next to each other.
 __device__ __forceinline__ int token_of(int l) { return (l & 8) + ((l & 7) >> 1) + 4 * (l & 1); }
 
-// Parameters of a row and group: scale and centre of the codes; nothing where the row is not held.
-__device__ __forceinline__ float2 centred(uint32_t par, bool have) {
-    const float2 t = Num<__half>::two(have ? par : 0u);
+// Parameters of a row and group: scale and centre of the codes.
+__device__ __forceinline__ float2 centred(uint32_t par) {
+    const float2 t = Num<__half>::two(par);
     return make_float2(t.x, fmaf(8.0f, t.x, t.y));
+}
+// Rows of a page in shared memory that are not held: parameters of nothing, whatever bits were there (the whole warp calls).
+template <int D>
+__device__ __forceinline__ void clear_rows(uint8_t* page, int valid, bool values) {
+    using L = Tile<D>;
+    __syncwarp();
+    for (int i = valid * L::G + (threadIdx.x & 31); i < kRows * L::G; i += 32) {
+        reinterpret_cast<uint32_t*>(page + L::K_PARAMS)[i] = 0u;
+        if (values) reinterpret_cast<uint32_t*>(page + L::V_PARAMS)[i] = 0u;
+    }
+    __syncwarp();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");                  // ahead of the next copy into this place
 }
 
 // Scores, unscaled, of the 16 tokens of tile u of a page against NT query tiles: s[t][0..1] of token token_of(lane / 4) and the lane's
-// two columns, s[t][2..3] of the token 8 behind.  valid: rows of the page that are held.
+// two columns, s[t][2..3] of the token 8 behind.
 template <int D, int NT>
-__device__ __forceinline__ void score_tile(const uint8_t* page, int u, int valid, const QueryTile<D> (&q)[NT], float (&s)[NT][4]) {
+__device__ __forceinline__ void score_tile(const uint8_t* page, int u, const QueryTile<D> (&q)[NT], float (&s)[NT][4]) {
     using L = Tile<D>;
     constexpr int G = L::G;
     const int lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3;
@@ -181,42 +215,16 @@ __device__ __forceinline__ void score_tile(const uint8_t* page, int u, int valid
                 mma16816(acc[t], a1, q[t].f[g][2 * w + 1][0], q[t].f[g][2 * w + 1][1]);
             }
         }
-        const float2 a = centred(pa[g], ta < valid), b = centred(pb[g], tb < valid);
+        const float2 a = centred(pa[g]), b = centred(pb[g]);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const float x = fmaf(a.x, acc[t][k], a.y * q[t].sum[g][k]), y = fmaf(b.x, acc[t][2 + k], b.y * q[t].sum[g][k]);
-                s[t][k] = g == 0 ? x : s[t][k] + x;
-                s[t][2 + k] = g == 0 ? y : s[t][2 + k] + y;
+                s[t][k] = fmaf(a.x, acc[t][k], g == 0 ? a.y * q[t].sum[g][k] : fmaf(a.y, q[t].sum[g][k], s[t][k]));
+                s[t][2 + k] = fmaf(b.x, acc[t][2 + k], g == 0 ? b.y * q[t].sum[g][k] : fmaf(b.y, q[t].sum[g][k], s[t][2 + k]));
             }
     }
 }
-
-// Pages of a warp through a ring of its own in shared memory, one bulk copy each.
-template <int BYTES, int STAGES>
-struct PageRing {
-    uint32_t base, bars;
-    int lane_page;               // of the warp's page number `lane`, -1: not a page of the pool
-    __device__ __forceinline__ void init(unsigned char* smem, uint64_t* bar) {
-        base = tc::smem_u32(smem);
-        bars = tc::smem_u32(bar);
-        if ((threadIdx.x & 31) == 0) {
-            for (int i = 0; i < STAGES; ++i) tc::mbar_init(bars + 8 * i, 1);
-            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        }
-        __syncwarp();
-    }
-    template <int D>
-    __device__ __forceinline__ int request(const Cache& c, int head, int i) {      // returns the page, by the whole warp
-        const int page = __shfl_sync(0xffffffffu, lane_page, i & 31);
-        if (page >= 0 && (threadIdx.x & 31) == 0) {
-            tc::mbar_expect_tx(bars + 8 * (i % STAGES), BYTES);
-            bulk_copy(base + (i % STAGES) * BYTES, tile_of<D>(c, page, head), BYTES, bars + 8 * (i % STAGES));
-        }
-        return page;
-    }
-};
 
 template <int D, int NT>
 struct FewCfg {
@@ -225,341 +233,497 @@ struct FewCfg {
     static constexpr size_t RING = (size_t)kWarps * STAGES * Tile<D>::BYTES;
     static constexpr int LD = D + 4;                                             // floats of a row in the merge of the warps
     static constexpr size_t MERGE = (size_t)kWarps * 8 * NT * LD * 4;
-    static constexpr size_t SMEM = (RING > MERGE ? RING : MERGE) + kWarps * STAGES * 8 + kWarps * 8 * NT * 8 + 16;
+    static constexpr size_t BARS = RING > MERGE ? RING : MERGE;                  // the merge takes the place of the rings, which are idle then
+    static constexpr size_t SMEM = BARS + kWarps * STAGES * 8 + kWarps * 8 * NT * 8 + 16;
 };
 
-// Few query rows.  grid (chunks x row tiles, kv heads, batch); a warp takes every fourth page of the chunk.  The MMA's 16 rows are
-// tokens (channels in P V) and its 8 columns query rows -- the heads of a group, times the new rows -- so that a single token of up to 8
-// heads per kv head fills it: m16n8k16 the other way round would leave half of it empty.
+// Few query rows.  A warp takes every fourth page of its block's units, each page (one kv head's tile) one bulk copy into the warp's own
+// ring.  The MMA's 16 rows are tokens (channels in P V) and its 8 columns query rows -- the heads of a group, times the new rows -- so
+// that a single token of up to 8 heads per kv head fills it: m16n8k16 the other way round would leave half of it empty.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few_kernel(const Cache c, const AttnParams p) {
     using L = Tile<D>;
     using C = FewCfg<D, NT>;
     constexpr int G = L::G, R = 8 * NT;
     extern __shared__ __align__(128) unsigned char smem[];
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (C::RING > C::MERGE ? C::RING : C::MERGE));
+    __shared__ int64_t sums[kWarps], before_s[2];
+    __shared__ int first_s;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
     float2* ml_s = reinterpret_cast<float2*>(bars + kWarps * C::STAGES);         // [warps][R]
     volatile int* abort_s = reinterpret_cast<volatile int*>(ml_s + kWarps * R);
-    const int chunk = blockIdx.x % p.chunks, tile = blockIdx.x / p.chunks, h = blockIdx.y, b = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3, group = c.q_heads / c.kv_heads;
+    unsigned char* ring = smem + (size_t)warp * C::STAGES * L::BYTES;
+    const uint32_t bar0 = tc::smem_u32(bars + warp * C::STAGES);
+    if (lane == 0) {
+        for (int i = 0; i < C::STAGES; ++i) tc::mbar_init(bar0 + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (threadIdx.x == 0) { *abort_s = 0; first_s = -1; }
     pdl_wait();
     pdl_launch_dependents();
-    const int col = chunk * p.chunk + warp + kWarps * lane;                      // this lane's page of the warp's
-    const int raw = col < c.max_pages && kWarps * lane + warp < p.chunk ? c.page_table[(size_t)b * c.max_pages + col] : -1;
-    const Entry e = entry_of(c, p, b);
-    const int rows = e.n * group;                                                // packed: new row x head of the group
-    if (tile * R >= rows) return;
-    const int pages = (e.len + kRows - 1) / kRows, p0 = chunk * p.chunk, mine = max(0, min(pages - p0, p.chunk) - warp + kWarps - 1) / kWarps;
-    if (p0 >= pages && chunk > 0) return;
-    PageRing<L::BYTES, C::STAGES> ring;
-    ring.lane_page = (unsigned)raw < (unsigned)c.n_pages ? raw : -1;
-    if (lane < mine && ring.lane_page < 0) raise(c, kBadPage);
-    ring.init(smem + (size_t)warp * C::STAGES * L::BYTES, bars + warp * C::STAGES);
-    if (threadIdx.x == 0) *abort_s = 0;
-    for (int i = 0; i < min(mine, C::STAGES); ++i) ring.template request<D>(c, h, i);
-
-    QueryTile<D> q[NT];
-    int see[NT][2], least = INT32_MAX;                                           // cached rows that the lane's columns see
+    // this block's range of the units, and the sequence it begins in
+    const int per = (c.batch + kWarps * 32 - 1) / (kWarps * 32), b_lo = min(c.batch, (int)threadIdx.x * per), b_hi = min(c.batch, b_lo + per);
+    int64_t own = 0;
+    for (int b = b_lo; b < b_hi; ++b) own += share_of<R>(c, p, b, group).units;
+    int64_t upto = own;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int row = tile * R + t * 8 + r;
-        q[t].load((const T*)p.q + ((size_t)(e.row0 + row / group) * c.q_heads + h * group + row % group) * D, row < rows, p.scale_log2);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int cr = tile * R + t * 8 + 2 * j + k;
-            see[t][k] = cr < rows ? max(0, min(e.len, e.len - e.n + cr / group + 1)) : 0;
-            if (cr < rows) least = min(least, see[t][k]);
-        }
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
     }
-    least = min(least, __shfl_xor_sync(0xffffffffu, least, 1));
-    least = min(least, __shfl_xor_sync(0xffffffffu, least, 2));
-    float o[G][4][NT][4], pc[G][NT][2], m[NT][2], l[NT][2];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) { m[t][k] = -INFINITY; l[t][k] = 0.f; for (int g = 0; g < G; ++g) pc[g][t][k] = 0.f; }
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) o[g][x][t][k] = 0.f;
-    int ev = -40;                                                                // exponent of the largest value scale seen
+    if (lane == 31) sums[warp] = upto;
     __syncthreads();
+    int64_t all = 0;
+    for (int w = 0; w < kWarps; ++w) { if (w < warp) upto += sums[w]; all += sums[w]; }
+    const int64_t step = step_of(p, all), u0 = blockIdx.x * step, u1 = min(all, u0 + step);
+    if (u0 >= all) return;
+    if (upto - own <= u0 && u0 < upto) {
+        int64_t at = upto - own;
+        int b = b_lo;
+        for (int64_t n; at + (n = share_of<R>(c, p, b, group).units) <= u0; ++b) at += n;
+        first_s = b;
+        before_s[0] = at;
+    }
+    __syncthreads();
+    int b = first_s, slot = 0;                                                   // slot: of the copies and their barriers
+    int64_t start = before_s[0];                                                 // unit that sequence b begins with
 
-    for (int i = 0; i < mine; ++i) {
-        const int first = (p0 + warp + kWarps * i) * kRows, valid = min(kRows, e.len - first);
-        const int page_no = __shfl_sync(0xffffffffu, ring.lane_page, i & 31);
-        if (page_no >= 0) {
-            if (!__all_sync(0xffffffffu, tc::mbar_wait(ring.bars + 8 * (i % C::STAGES), (uint32_t)(i / C::STAGES) & 1u, abort_s))) { *abort_s = 1; break; }
-            const uint8_t* page = smem + ((size_t)warp * C::STAGES + i % C::STAGES) * L::BYTES;
-            float s[4][NT][4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) score_tile<D, NT>(page, u, valid, q, s[u]);
-            const bool whole = first + kRows <= least;
-            float top[NT][2];
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    top[t][k] = -INFINITY;
-#pragma unroll
-                    for (int u = 0; u < 4; ++u)
-#pragma unroll
-                        for (int hf = 0; hf < 2; ++hf) {
-                            float& x = s[u][t][2 * hf + k];
-                            x *= q[t].unit[k];
-                            if (!whole && first + u * 16 + token_of(r) + 8 * hf >= see[t][k]) x = -INFINITY;
-                            top[t][k] = fmaxf(top[t][k], x);
-                        }
-                }
-            // parameters of the values, and the largest scale (positive halves order like whole numbers)
-            uint32_t vp[4][2][G];
-            int big = 0;
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const int tk = u * 16 + token_of(r) + 8 * hf;
-#pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        vp[u][hf][g] = tk < valid ? reinterpret_cast<const uint32_t*>(page + L::V_PARAMS)[tk * G + g] : 0u;
-                        big = max(big, (int)(vp[u][hf][g] & 0x7fffu));
-                    }
-                }
-#pragma unroll
-            for (int off = 4; off < 32; off <<= 1) {
-                big = max(big, __shfl_xor_sync(0xffffffffu, big, off));
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) top[t][k] = fmaxf(top[t][k], __shfl_xor_sync(0xffffffffu, top[t][k], off));
+    for (int64_t at = u0; at < u1;) {
+        const Share sh = share_of<R>(c, p, b, group);
+        if (at >= start + sh.units) { start += sh.units; ++b; continue; }
+        const Entry e = entry_of(c, p, b);
+        const int rows = e.n * group, pages = (e.len + kRows - 1) / kRows;
+        const int piece = (int)((at - start) / sh.pages), h = piece / sh.tiles, tile = piece % sh.tiles, p0 = (int)((at - start) % sh.pages);
+        const int p1 = (int)min((int64_t)sh.pages, p0 + (u1 - at));              // pages [p0, p1) of this piece
+        const bool from_start = p0 == 0, to_end = p1 == sh.pages;
+        at += p1 - p0;
+        const int mine = max(0, min(p1, pages) - p0 - warp + kWarps - 1) / kWarps;
+        int lane_page = -1;
+        uint32_t there = 0;                                                      // bit per stage: its page is one of the pool's
+        auto request = [&](int i) {
+            if ((i & 31) == 0) {
+                const int col = p0 + warp + kWarps * (i + lane);
+                const bool in = i + lane < mine;
+                lane_page = in ? c.page_table[(size_t)b * c.max_pages + col] : -1;
+                if ((unsigned)lane_page >= (unsigned)c.n_pages) { if (in) raise(c, kBadPage); lane_page = -1; }
             }
-            const int en = max(ev, big > 0 ? max(big >> 10, 1) - 15 : -40);
-            const float fold = __uint_as_float((uint32_t)(127 + ev - en) << 23);
-            float alpha[NT][2], base[NT][2];
-            bool same = ev == en;
-            ev = en;
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const float mn = fmaxf(m[t][k], top[t][k]);
-                    base[t][k] = mn == -INFINITY ? 0.f : mn;
-                    alpha[t][k] = m[t][k] == -INFINITY ? 0.f : ex2f(m[t][k] - base[t][k]);
-                    same = same && (mn == m[t][k]);
-                    m[t][k] = mn;
+            const int page = __shfl_sync(0xffffffffu, lane_page, i & 31), st = (slot + i) % C::STAGES;
+            there = page >= 0 ? there | 1u << st : there & ~(1u << st);
+            if (lane == 0) {
+                if (page >= 0) {
+                    tc::mbar_expect_tx(bar0 + 8 * st, L::BYTES);
+                    bulk_copy(tc::smem_u32(ring) + st * L::BYTES, tile_of<D>(c, page, h), L::BYTES, bar0 + 8 * st);
+                } else {
+                    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar0 + 8 * st) : "memory");
                 }
-            if (!__all_sync(0xffffffffu, same)) {
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        l[t][k] *= alpha[t][k];
-                        const float f = alpha[t][k] * fold;
-#pragma unroll
-                        for (int g = 0; g < G; ++g) {
-                            pc[g][t][k] *= alpha[t][k];
-#pragma unroll
-                            for (int x = 0; x < 4; ++x) { o[g][x][t][k] *= f; o[g][x][t][2 + k] *= f; }
-                        }
-                    }
             }
-            const float unit = __uint_as_float((uint32_t)(127 + 14 - en) << 23);
+        };
+        for (int i = 0; i < min(mine, C::STAGES); ++i) request(i);
+
+        QueryTile<D> q[NT];
+        int see[NT][2], least = INT32_MAX;                                       // cached rows that the lane's columns see
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                uint32_t b0[G][NT], b1[G][NT];
+        for (int t = 0; t < NT; ++t) {
+            const int row = tile * R + t * 8 + r;
+            q[t].load((const T*)p.q + ((size_t)(e.row0 + row / group) * c.q_heads + h * group + row % group) * D, row < rows, p.scale_log2);
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        s[u][t][k] = ex2f(s[u][t][k] - base[t][k & 1]);
-                        l[t][k & 1] += s[u][t][k];
-                    }
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const float2 a = centred(vp[u][0][g], true), bb = centred(vp[u][1][g], true);
-                    const float sa = a.x * unit, sb = bb.x * unit;
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const float(&w)[4] = s[u][t];
-                        pc[g][t][0] = fmaf(w[0], a.y, fmaf(w[2], bb.y, pc[g][t][0]));
-                        pc[g][t][1] = fmaf(w[1], a.y, fmaf(w[3], bb.y, pc[g][t][1]));
-                        b0[g][t] = transposed(half_pair(w[0] * sa, w[1] * sa));
-                        b1[g][t] = transposed(half_pair(w[2] * sb, w[3] * sb));
-                    }
-                }
-                // columns 2 j, 2 j + 1 (and 8 behind) of the operand are the tokens j, j + 4 (j + 8, j + 12)
-                const uint32_t* codes = reinterpret_cast<const uint32_t*>(page + L::V_CODES) + (u * 16 + j) * L::WORDS + r;
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const uint32_t w0 = codes[g * 8], w1 = codes[4 * L::WORDS + g * 8], w2 = codes[8 * L::WORDS + g * 8], w3 = codes[12 * L::WORDS + g * 8];
-#pragma unroll
-                    for (int hl = 0; hl < 2; ++hl) {
-                        const uint32_t x = __byte_perm(w0, w1, hl ? 0x7632 : 0x5410), y = __byte_perm(w2, w3, hl ? 0x7632 : 0x5410);
-                        const uint32_t a0[4] = {low_pair(x), high_pair(x), low_pair(y), high_pair(y)};
-                        const uint32_t a1[4] = {low_pair(x >> 8), high_pair(x >> 8), low_pair(y >> 8), high_pair(y >> 8)};
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            mma16816(o[g][2 * hl][t], a0, b0[g][t], b1[g][t]);
-                            mma16816(o[g][2 * hl + 1][t], a1, b0[g][t], b1[g][t]);
-                        }
-                    }
-                }
+            for (int k = 0; k < 2; ++k) {
+                const int cr = tile * R + t * 8 + 2 * j + k;
+                see[t][k] = cr < rows ? max(0, min(e.len, e.len - e.n + cr / group + 1)) : 0;
+                if (cr < rows) least = min(least, see[t][k]);
             }
         }
-        __syncwarp();                                                            // every lane has read the page
-        if (i + C::STAGES < mine) ring.template request<D>(c, h, i + C::STAGES);
-    }
-    if (*abort_s != 0 && lane == 0)                                              // given up: let the copies in flight land (bounded)
-        for (int i = 0; i < min(mine, C::STAGES); ++i) { volatile int go_on = 0; (void)tc::mbar_wait(ring.bars + 8 * i, 0, &go_on); (void)tc::mbar_wait(ring.bars + 8 * i, 1, &go_on); }
-
-    // the warps' results: maxima first, then values relative to the block's
-#pragma unroll
-    for (int off = 4; off < 32; off <<= 1)
+        least = min(least, __shfl_xor_sync(0xffffffffu, least, 1));
+        least = min(least, __shfl_xor_sync(0xffffffffu, least, 2));
+        float o[G][4][NT][4], pc[G][NT][2], m[NT][2], l[NT][2];                  // m: maximum, in units of log2
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                l[t][k] += __shfl_xor_sync(0xffffffffu, l[t][k], off);
+                m[t][k] = -INFINITY;
+                l[t][k] = 0.f;
 #pragma unroll
-                for (int g = 0; g < G; ++g) pc[g][t][k] += __shfl_xor_sync(0xffffffffu, pc[g][t][k], off);
+                for (int g = 0; g < G; ++g) pc[g][t][k] = 0.f;
             }
-    if (r == 0)
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o[g][x][t][k] = 0.f;
+        int ev = -40;                                                            // exponent of the largest value scale seen
+
+        for (int i = 0; i < mine; ++i) {
+            const int st = (slot + i) % C::STAGES, first = (p0 + warp + kWarps * i) * kRows;
+            if (!__all_sync(0xffffffffu, tc::mbar_wait(bar0 + 8 * st, (uint32_t)((slot + i) / C::STAGES) & 1u, abort_s))) { *abort_s = 1; break; }
+            if (there >> st & 1u) {
+                uint8_t* page = ring + (size_t)st * L::BYTES;
+                if (e.len - first < kRows) clear_rows<D>(page, e.len - first, true);
+                float s[4][NT][4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) score_tile<D, NT>(page, u, q, s[u]);
+                if (first + kRows > least) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if (first + u * 16 + token_of(r) + 8 * (k >> 1) >= see[t][k & 1]) s[u][t][k] = -INFINITY;
+                }
+                if (p.scores != nullptr) {
+                    float* to = p.scores + ((size_t)b * c.kv_heads + h) * R * p.score_ld + first + token_of(r);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            if (t * 8 + 2 * j + k < rows)
+#pragma unroll
+                                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                                    for (int hf = 0; hf < 2; ++hf) to[(t * 8 + 2 * j + k) * p.score_ld + u * 16 + 8 * hf] = s[u][t][2 * hf + k] * q[t].unit[k];
+                }
+                float top[NT][2];
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        top[t][k] = fmaxf(s[0][t][k], s[0][t][2 + k]);
+#pragma unroll
+                        for (int u = 1; u < 4; ++u) top[t][k] = fmaxf(top[t][k], fmaxf(s[u][t][k], s[u][t][2 + k]));
+                    }
+                // parameters of the values; the largest scale is the low half of the largest pair
+                uint32_t vp[4][2][G], big2 = 0;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const uint8_t* par = page + L::V_PARAMS + (u * 16 + token_of(r) + 8 * hf) * G * 4;
+                        if constexpr (G == 2) {
+                            const uint2 w = *reinterpret_cast<const uint2*>(par);
+                            vp[u][hf][0] = w.x;
+                            vp[u][hf][1] = w.y;
+                        } else {
+                            vp[u][hf][0] = *reinterpret_cast<const uint32_t*>(par);
+                        }
+#pragma unroll
+                        for (int g = 0; g < G; ++g) asm("max.f16x2 %0, %0, %1;" : "+r"(big2) : "r"(vp[u][hf][g]));
+                    }
+                int big = (int)(big2 & 0x7fffu);
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) {
+                    big = max(big, __shfl_xor_sync(0xffffffffu, big, off));
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) top[t][k] = fmaxf(top[t][k], __shfl_xor_sync(0xffffffffu, top[t][k], off));
+                }
+                const int en = max(ev, big > 0 ? max(big >> 10, 1) - 15 : -40);
+                float base[NT][2];
+                bool same = ev == en;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        base[t][k] = fmaxf(m[t][k], top[t][k] * q[t].unit[k]);
+                        same = same && base[t][k] == m[t][k];
+                    }
+                if (!__all_sync(0xffffffffu, same)) {
+                    const float fold = __uint_as_float((uint32_t)(127 + ev - en) << 23);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const float alpha = m[t][k] == -INFINITY ? 0.f : ex2f(m[t][k] - base[t][k]), f = alpha * fold;
+                            m[t][k] = base[t][k];
+                            l[t][k] *= alpha;
+#pragma unroll
+                            for (int g = 0; g < G; ++g) {
+                                pc[g][t][k] *= alpha;
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) { o[g][x][t][k] *= f; o[g][x][t][2 + k] *= f; }
+                            }
+                        }
+                    ev = en;
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        if (base[t][k] == -INFINITY) base[t][k] = 0.f;
+                const float unit = __uint_as_float((uint32_t)(127 + 14 - ev) << 23);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    uint32_t b0[G][NT], b1[G][NT];
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            s[u][t][k] = ex2f(fmaf(s[u][t][k], q[t].unit[k & 1], -base[t][k & 1]));
+                            l[t][k & 1] += s[u][t][k];
+                        }
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const float2 a = centred(vp[u][0][g]), bb = centred(vp[u][1][g]);
+                        const float sa = a.x * unit, sb = bb.x * unit;
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            const float(&w)[4] = s[u][t];
+                            pc[g][t][0] = fmaf(w[0], a.y, fmaf(w[2], bb.y, pc[g][t][0]));
+                            pc[g][t][1] = fmaf(w[1], a.y, fmaf(w[3], bb.y, pc[g][t][1]));
+                            b0[g][t] = transposed(half_pair(w[0] * sa, w[1] * sa));
+                            b1[g][t] = transposed(half_pair(w[2] * sb, w[3] * sb));
+                        }
+                    }
+                    // columns 2 j, 2 j + 1 (and 8 behind) of the operand are the tokens j, j + 4 (j + 8, j + 12)
+                    const uint32_t* codes = reinterpret_cast<const uint32_t*>(page + L::V_CODES) + (u * 16 + j) * L::WORDS + r;
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const uint32_t w0 = codes[g * 8], w1 = codes[4 * L::WORDS + g * 8], w2 = codes[8 * L::WORDS + g * 8], w3 = codes[12 * L::WORDS + g * 8];
+#pragma unroll
+                        for (int hl = 0; hl < 2; ++hl) {
+                            const uint32_t x = __byte_perm(w0, w1, hl ? 0x7632 : 0x5410), y = __byte_perm(w2, w3, hl ? 0x7632 : 0x5410);
+                            const uint32_t a0[4] = {low_pair(x), high_pair(x), low_pair(y), high_pair(y)};
+                            const uint32_t a1[4] = {low_pair(x >> 8), high_pair(x >> 8), low_pair(y >> 8), high_pair(y >> 8)};
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) {
+                                mma16816(o[g][2 * hl][t], a0, b0[g][t], b1[g][t]);
+                                mma16816(o[g][2 * hl + 1][t], a1, b0[g][t], b1[g][t]);
+                            }
+                        }
+                    }
+                }
+            }
+            __syncwarp();                                                        // every lane has read the page
+            if (i + C::STAGES < mine) request(i + C::STAGES);
+        }
+        if (*abort_s != 0 && lane == 0)                                          // given up: let the copies in flight land (bounded)
+            for (int i = 0; i < C::STAGES; ++i) { volatile int go_on = 0; (void)tc::mbar_wait(bar0 + 8 * i, 0, &go_on); (void)tc::mbar_wait(bar0 + 8 * i, 1, &go_on); }
+        slot += mine;
+
+        // the warps' results: maxima first, then values relative to the block's
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    l[t][k] += __shfl_xor_sync(0xffffffffu, l[t][k], off);
+#pragma unroll
+                    for (int g = 0; g < G; ++g) pc[g][t][k] += __shfl_xor_sync(0xffffffffu, pc[g][t][k], off);
+                }
+        if (r == 0)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) ml_s[warp * R + t * 8 + 2 * j + k] = make_float2(m[t][k], l[t][k]);
+        __syncthreads();
+        if (*abort_s != 0) { if (threadIdx.x == 0) raise(c, kWait); return; }
+        float* merge = reinterpret_cast<float*>(smem);
+        const float back = __uint_as_float((uint32_t)(127 + ev - 14) << 23);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) ml_s[warp * R + t * 8 + 2 * j + k] = make_float2(m[t][k], l[t][k]);
-    __syncthreads();                                                             // the rings are free
-    float* merge = reinterpret_cast<float*>(smem);
-    const float back = __uint_as_float((uint32_t)(127 + ev - 14) << 23);
+            for (int k = 0; k < 2; ++k) {
+                const int rr = t * 8 + 2 * j + k;
+                float top = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+                for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml_s[w * R + rr].x);
+                const float f = m[t][k] == -INFINITY ? 0.f : ex2f(m[t][k] - top);
+                float* dst = merge + ((size_t)warp * R + rr) * C::LD + 8 * r;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int rr = t * 8 + 2 * j + k;
-            float top = -INFINITY;
+                for (int g = 0; g < G; ++g) {
+                    float v[8];                                                  // channels of word r of the group, see the nibbles' order
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int ch = (x & 1) * 4 + (x >> 1);
+                        v[ch] = fmaf(o[g][x][t][k], back, pc[g][t][k]) * f;
+                        v[ch + 2] = fmaf(o[g][x][t][2 + k], back, pc[g][t][k]) * f;
+                    }
+                    *reinterpret_cast<float4*>(dst + g * 64) = make_float4(v[0], v[1], v[2], v[3]);
+                    *reinterpret_cast<float4*>(dst + g * 64 + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                }
+            }
+        __syncthreads();
+        const bool alone = from_start && to_end;
+        const size_t piece_row = ((size_t)2 * blockIdx.x + (from_start ? 1 : 0)) * R;
+        for (int i = threadIdx.x; i < R * (D / 4); i += kWarps * 32) {
+            const int rr = i / (D / 4), d = i % (D / 4) * 4, row = tile * R + rr;
+            if (row >= rows) continue;
+            float top = -INFINITY, sum = 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml_s[w * R + rr].x);
-            const float f = m[t][k] == -INFINITY ? 0.f : ex2f(m[t][k] - top);
-            float* dst = merge + ((size_t)warp * R + rr) * C::LD + 8 * r;
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-                float v[8];                                                      // channels of word r of the group, see the nibbles' order
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const int at = (x & 1) * 4 + (x >> 1);
-                    v[at] = fmaf(o[g][x][t][k], back, pc[g][t][k]) * f;
-                    v[at + 2] = fmaf(o[g][x][t][2 + k], back, pc[g][t][k]) * f;
-                }
-                *reinterpret_cast<float4*>(dst + g * 64) = make_float4(v[0], v[1], v[2], v[3]);
-                *reinterpret_cast<float4*>(dst + g * 64 + 4) = make_float4(v[4], v[5], v[6], v[7]);
+            for (int w = 0; w < kWarps; ++w) {
+                const float2 ml = ml_s[w * R + rr];
+                if (ml.x != -INFINITY) sum = fmaf(ml.y, ex2f(ml.x - top), sum);
+                const float4 x = *reinterpret_cast<const float4*>(merge + ((size_t)w * R + rr) * C::LD + d);
+                v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+            }
+            const int head = h * group + row % group;
+            if (alone) {
+                const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+                T* dst = (T*)p.out + ((size_t)(e.row0 + row / group) * c.q_heads + head) * D + d;
+                *reinterpret_cast<uint2*>(dst) = make_uint2(Num<T>::pack(v.x * inv, v.y * inv), Num<T>::pack(v.z * inv, v.w * inv));
+                if (p.stats != nullptr && d == 0) p.stats[stat_row(c, p, b, row / group, head)] = make_float2(top, sum);
+            } else {
+                *reinterpret_cast<float4*>(p.part + (piece_row + rr) * D + d) = v;
+                if (d == 0) p.part_stats[piece_row + rr] = make_float2(top, sum);
             }
         }
-    __syncthreads();
-    if (*abort_s != 0) { if (threadIdx.x == 0) raise(c, kWait); return; }
-    const bool alone = pages <= p.chunk;
-    for (int i = threadIdx.x; i < R * (D / 4); i += kWarps * 32) {
-        const int rr = i / (D / 4), d = i % (D / 4) * 4, row = tile * R + rr;
-        if (row >= rows) continue;
-        float top = -INFINITY, sum = 0.f;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml_s[w * R + rr].x);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float2 s = ml_s[w * R + rr];
-            if (s.x != -INFINITY) sum = fmaf(s.y, ex2f(s.x - top), sum);
-            const float4 x = *reinterpret_cast<const float4*>(merge + ((size_t)w * R + rr) * C::LD + d);
-            v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+        if (at < u1) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");         // the merge is over ahead of copies into the rings
+            __syncthreads();
         }
-        const int head = h * group + row % group;
-        if (alone) {
-            const float inv = sum > 0.f ? 1.0f / sum : 0.f;
-            T* dst = (T*)p.out + ((size_t)(e.row0 + row / group) * c.q_heads + head) * D + d;
-            *reinterpret_cast<uint2*>(dst) = make_uint2(Num<T>::pack(v.x * inv, v.y * inv), Num<T>::pack(v.z * inv, v.w * inv));
-        } else {
-            *reinterpret_cast<float4*>(p.part + part_row(c, p, chunk, b, row / group, head) * D + d) = v;
-        }
-        if (p.stats != nullptr && d == 0) p.stats[part_row(c, p, chunk, b, row / group, head)] = make_float2(top, sum);
     }
 }
 
-// Maximum and 1 / sum over the chunks of a row's weights.
-__device__ __forceinline__ float2 row_stats(const Cache& c, const AttnParams& p, int n_chunks, int b, int i, int head) {
+// Where the keys of a tile of packed rows were dealt: to one block, which finished the rows itself, or to blocks [w0, w1].
+struct Pieces { int64_t w0, w1; };
+__device__ __forceinline__ Pieces pieces_of(const AttnParams& p, const Share& s, const Deal& d, int h, int tile) {
+    const int64_t step = step_of(p, d.all), at = d.before + ((int64_t)h * s.tiles + tile) * s.pages;
+    return Pieces{at / step, (at + s.pages - 1) / step};
+}
+__device__ __forceinline__ size_t piece_row(int64_t w, const Pieces& x, int R, int rr) { return ((size_t)2 * w + (w == x.w0 ? 1 : 0)) * R + rr; }
+
+// Maximum and sum of packed row rr of a tile over its pieces, by a warp.
+__device__ __forceinline__ float2 merged_stats(const AttnParams& p, const Pieces& x, int R, int rr) {
+    const int lane = threadIdx.x & 31;
     float top = -INFINITY, sum = 0.f;
-    for (int k = 0; k < n_chunks; ++k) top = fmaxf(top, p.stats[part_row(c, p, k, b, i, head)].x);
-    if (top == -INFINITY) return make_float2(0.f, 0.f);
-    for (int k = 0; k < n_chunks; ++k) {
-        const float2 s = p.stats[part_row(c, p, k, b, i, head)];
-        if (s.x != -INFINITY) sum = fmaf(s.y, ex2f(s.x - top), sum);
+    for (int64_t w = x.w0 + lane; w <= x.w1; w += 32) {
+        const float2 s = p.part_stats[piece_row(w, x, R, rr)];
+        const float mx = fmaxf(top, s.x);
+        if (mx != -INFINITY) sum = (top == -INFINITY ? 0.f : sum * ex2f(top - mx)) + (s.x == -INFINITY ? 0.f : s.y * ex2f(s.x - mx));
+        top = mx;
     }
-    return make_float2(top, 1.0f / sum);
+    const float all = warp_max(top);
+    return make_float2(all, warp_sum(top == -INFINITY ? 0.f : sum * ex2f(top - all)));
+}
+
+constexpr int kMassTokens = 512;      // cached rows of a block that sums weights from scores
+
+// What needs the whole row.  grid (mass blocks + merging blocks, kv heads, batch): merging blocks join the pieces of rows that attend_few
+// dealt over several blocks, a row at a time; mass blocks sum the weights of 512 cached rows from the scores it left.
+template <typename T, int D, int R>
+__global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c, const AttnParams p, int mass_blocks) {
+    __shared__ int64_t sums[2][kWarps];
+    __shared__ float2 st_s[R];
+    __shared__ float4 v_s[kWarps * 32];
+    const int h = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = c.q_heads / c.kv_heads;
+    pdl_launch_dependents();
+    // lengths are not attend_few's to write: where the units lie is known before the wait
+    int64_t before = 0, all = 0;
+    for (int i = threadIdx.x; i < c.batch; i += kWarps * 32) {
+        const int64_t n = share_of<R>(c, p, i, group).units;
+        all += n;
+        if (i < b) before += n;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) { all += __shfl_xor_sync(0xffffffffu, all, o); before += __shfl_xor_sync(0xffffffffu, before, o); }
+    if (lane == 0) { sums[0][warp] = before; sums[1][warp] = all; }
+    __syncthreads();
+    Deal deal{0, 0};
+    for (int w = 0; w < kWarps; ++w) { deal.before += sums[0][w]; deal.all += sums[1][w]; }
+    const Entry e = entry_of(c, p, b);
+    const Share sh = share_of<R>(c, p, b, group);
+    const int rows = sh.tiles > 0 ? e.n * group : 0;
+    if ((int)blockIdx.x < mass_blocks) {
+        const int t0 = blockIdx.x * kMassTokens;
+        pdl_wait();
+        if (t0 >= e.len) return;
+        const Pieces x = rows > 0 ? pieces_of(p, sh, deal, h, 0) : Pieces{0, 0};
+        for (int row = warp; row < rows; row += kWarps) {
+            const float2 s = x.w0 == x.w1 ? p.stats[stat_row(c, p, b, row / group, h * group + row % group)] : merged_stats(p, x, R, row);
+            if (lane == 0) st_s[row] = s.x == -INFINITY ? make_float2(0.f, 0.f) : make_float2(s.x, 1.0f / s.y);
+        }
+        __syncthreads();
+        constexpr int PER = kMassTokens / (kWarps * 32);
+        float w[PER];
+        const float* from = p.scores + ((size_t)b * c.kv_heads + h) * R * p.score_ld + t0 + threadIdx.x;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) w[k] = 0.f;
+        for (int row = 0; row < rows; ++row) {
+            const float2 s = st_s[row];
+#pragma unroll
+            for (int k = 0; k < PER; ++k)
+                if (t0 + (int)threadIdx.x + k * kWarps * 32 < e.len) w[k] = fmaf(ex2f(from[row * p.score_ld + k * kWarps * 32] - s.x), s.y, w[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int tk = t0 + threadIdx.x + k * kWarps * 32;
+            const int page = tk < e.len ? page_of(c, b, tk / kRows) : -1;
+            if (page < 0) continue;
+            const size_t at = row_slot(c, page, h, tk % kRows);
+            p.mass_out[at] = p.mass_in[at] + w[k];
+        }
+        return;
+    }
+    pdl_wait();
+    for (int row = (int)blockIdx.x - mass_blocks; row < rows; row += (int)gridDim.x - mass_blocks) {
+        const Pieces x = pieces_of(p, sh, deal, h, row / R);
+        if (x.w0 == x.w1) continue;
+        const int i = row / group, head = h * group + row % group, rr = row % R;
+        const float2 st = merged_stats(p, x, R, rr);
+        constexpr int Q = D / 4, LANES = kWarps * 32 / Q;        // threads side by side, each with four channels of every LANES-th piece
+        const int d = threadIdx.x % Q * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int64_t w = x.w0 + threadIdx.x / Q; w <= x.w1; w += LANES) {
+            const size_t at = piece_row(w, x, R, rr);
+            const float m = p.part_stats[at].x, f = m == -INFINITY ? 0.f : ex2f(m - st.x);
+            const float4 y = *reinterpret_cast<const float4*>(p.part + at * D + d);
+            v.x = fmaf(y.x, f, v.x); v.y = fmaf(y.y, f, v.y); v.z = fmaf(y.z, f, v.z); v.w = fmaf(y.w, f, v.w);
+        }
+        v_s[threadIdx.x] = v;
+        __syncthreads();
+        if ((int)threadIdx.x < Q) {
+            for (int k = 1; k < LANES; ++k) { const float4 y = v_s[k * Q + threadIdx.x]; v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w; }
+            const float inv = st.y > 0.f ? 1.0f / st.y : 0.f;
+            *reinterpret_cast<uint2*>((T*)p.out + ((size_t)(e.row0 + i) * c.q_heads + head) * D + d) = make_uint2(Num<T>::pack(v.x * inv, v.y * inv), Num<T>::pack(v.z * inv, v.w * inv));
+            if (threadIdx.x == 0 && p.stats != nullptr && mass_blocks == 0) p.stats[stat_row(c, p, b, i, head)] = st;
+        }
+        __syncthreads();
+    }
 }
 
 template <int D>
-struct FinishCfg {
+struct MassCfg {
     static constexpr int K_BYTES = Tile<D>::V_CODES;                             // codes and parameters of the keys
     static constexpr size_t SMEM = (size_t)kWarps * K_BYTES + kWarps * 8 + 16;
 };
 
-// What needs the whole row: outputs of rows whose keys were dealt over several blocks, and the summed weights.  grid (page groups +
-// merging blocks, kv heads, batch); in a page group a warp has a page of its own and walks the new rows in order.
+// Summed weights where scores were not kept (more packed rows than a tile): the keys once more.  grid (groups of pages, kv heads, batch); a
+// warp has a page of its own and walks the new rows in order, eight packed rows at a time, so that sums need no atomics.
 template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32) attend_finish_kernel(const Cache c, const AttnParams p, int page_groups) {
-    using L = Tile<D>;
-    using C = FinishCfg<D>;
+__global__ void __launch_bounds__(kWarps * 32) attend_mass_kernel(const Cache c, const AttnParams p) {
+    using C = MassCfg<D>;
     extern __shared__ __align__(128) unsigned char smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (size_t)kWarps * C::K_BYTES);
     volatile int* abort_s = reinterpret_cast<volatile int*>(bars + kWarps);
     const int h = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3, group = c.q_heads / c.kv_heads;
     pdl_launch_dependents();
-    if ((int)blockIdx.x >= page_groups) {                                        // merge: a warp per new row and head
-        pdl_wait();
-        const Entry e = entry_of(c, p, b);
-        const int pages = (e.len + kRows - 1) / kRows, n_chunks = (pages + p.chunk - 1) / p.chunk;
-        if (n_chunks <= 1) return;
-        for (int row = ((int)blockIdx.x - page_groups) * kWarps + warp; row < e.n * group; row += ((int)gridDim.x - page_groups) * kWarps) {
-            const int i = row / group, head = h * group + row % group;
-            const float2 st = row_stats(c, p, n_chunks, b, i, head);
-            constexpr int E = D / 32;
-            float v[E];
-#pragma unroll
-            for (int k = 0; k < E; ++k) v[k] = 0.f;
-            for (int k = 0; k < n_chunks; ++k) {
-                const size_t at = part_row(c, p, k, b, i, head);
-                const float f = ex2f(p.stats[at].x - st.x);                      // 0 where the chunk has nothing to see
-                const float* src = p.part + at * D + lane * E;
-#pragma unroll
-                for (int d = 0; d < E; ++d) v[d] = fmaf(src[d], f, v[d]);
-            }
-            T* dst = (T*)p.out + ((size_t)(e.row0 + i) * c.q_heads + head) * D + lane * E;
-#pragma unroll
-            for (int d = 0; d < E; d += 2) *reinterpret_cast<uint32_t*>(dst + d) = Num<T>::pack(v[d] * st.y, v[d + 1] * st.y);
-        }
-        return;
-    }
     const Entry e = entry_of(c, p, b);
-    const int pages = (e.len + kRows - 1) / kRows, pg = blockIdx.x * kWarps + warp, n_chunks = max(1, (pages + p.chunk - 1) / p.chunk);
+    const int pages = (e.len + kRows - 1) / kRows, pg = blockIdx.x * kWarps + warp;
     if (threadIdx.x == 0) *abort_s = 0;
     __syncthreads();
-    if (pg >= pages) { pdl_wait(); return; }
-    const int page = page_of(c, b, pg);
+    const int page = pg < pages ? page_of(c, b, pg) : -1;
     if (page < 0) { pdl_wait(); return; }
     const uint32_t bar = tc::smem_u32(bars + warp);
+    uint8_t* tile = smem + (size_t)warp * C::K_BYTES;
     if (lane == 0) {
         tc::mbar_init(bar, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         tc::mbar_expect_tx(bar, C::K_BYTES);
-        bulk_copy(tc::smem_u32(smem) + warp * C::K_BYTES, tile_of<D>(c, page, h), C::K_BYTES, bar);
+        bulk_copy(tc::smem_u32(tile), tile_of<D>(c, page, h), C::K_BYTES, bar);
     }
     __syncwarp();
     pdl_wait();
     if (!__all_sync(0xffffffffu, tc::mbar_wait(bar, 0, abort_s))) { if (lane == 0) raise(c, kWait); return; }
-    const uint8_t* tile = smem + (size_t)warp * C::K_BYTES;
     const int first = pg * kRows, valid = min(kRows, e.len - first), rows = e.n * group;
+    if (valid < kRows) clear_rows<D>(tile, valid, false);
     float w[4][2];
 #pragma unroll
     for (int u = 0; u < 4; ++u) w[u][0] = w[u][1] = 0.f;
@@ -568,20 +732,21 @@ __global__ void __launch_bounds__(kWarps * 32) attend_finish_kernel(const Cache 
         QueryTile<D> q[1];
         const int row = r0 + r;
         q[0].load((const T*)p.q + ((size_t)(e.row0 + row / group) * c.q_heads + h * group + row % group) * D, row < rows, p.scale_log2);
-        const float2 mine = row < rows ? row_stats(c, p, n_chunks, b, row / group, h * group + row % group) : make_float2(0.f, 0.f);
+        const float2 st = row < rows ? p.stats[stat_row(c, p, b, row / group, h * group + row % group)] : make_float2(-INFINITY, 0.f);
+        const float mine = st.x == -INFINITY ? 0.f : st.x, one = st.x == -INFINITY ? 0.f : 1.0f / st.y;
         float top[2], inv[2];
         int see[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            top[k] = __shfl_sync(0xffffffffu, mine.x, (2 * j + k) * 4);
-            inv[k] = __shfl_sync(0xffffffffu, mine.y, (2 * j + k) * 4);
+            top[k] = __shfl_sync(0xffffffffu, mine, (2 * j + k) * 4);
+            inv[k] = __shfl_sync(0xffffffffu, one, (2 * j + k) * 4);
             const int cr = r0 + 2 * j + k;
             see[k] = cr < rows ? min(e.len, e.len - e.n + cr / group + 1) : 0;
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             float s[1][4];
-            score_tile<D, 1>(tile, u, valid, q, s);
+            score_tile<D, 1>(tile, u, q, s);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const float x = ex2f(fmaf(s[0][k], q[0].unit[k & 1], -top[k & 1])) * inv[k & 1];
