@@ -1,7 +1,7 @@
 // Attention over a 4-bit cache (kv4_cache.cuh): new rows of a ragged batch against the pages of their sequences.
 //
 // The codes go to the tensor cores as they are: a key is min + scale * code = c + scale * (code - 8) with c = min + 8 scale, so that
-//     q . k = sum over groups g of  scale_g (q_g . (code - 8)_g) + c_g (sum of q_g),
+//     q . k = sum over groups g of  scale_g (q_g . (code - 8)_g + 8 (sum of q_g)) + min_g (sum of q_g),
 // and code - 8 is exact in fp16.  q is scaled by a power of two per row and is exact there too (bf16 has fewer bits): scores carry fp32
 // rounding only.  Values: o = sum over tokens of (p scale_g) (code - 8) + sum of p c_g, with p scale_g rounded to fp16 below a power of
 // two that keeps the largest scale seen at 2^14 .. 2^15, so that neither large nor small scales leave its range.
@@ -21,7 +21,7 @@ struct AttnParams {
     const float* mass_in;
     float* mass_out;
     int few_rows;             // sequences with at most this many packed rows (new rows x heads of a group) are attend_few's
-    int blocks;               // attend_few's blocks
+    int blocks, unit;         // attend_few's blocks; pages of a unit of work
     float2* stats;            // [batch, rows, q_heads] (maximum, sum) of a row's weights, where one block had all its keys; null: not wanted
     int rows;                 // new rows a sequence has in stats
     float2* part_stats;       // [2 blocks][8 nt] the same of the keys a block had, and
@@ -48,28 +48,30 @@ __device__ __forceinline__ size_t stat_row(const Cache& c, const AttnParams& p, 
 
 constexpr int kWarps = 4;
 
-// How attend_few's work is dealt: every page of every (sequence, kv head, tile of R packed rows) is a unit, in that order; block w has the
-// units [w step, (w + 1) step).  Lengths are known on the device only, so every block adds them up for itself.
-struct Deal { int64_t before, all; };          // units ahead of sequence b, and altogether
-struct Share { int64_t units; int tiles, pages; };
+// How attend_few's work is dealt: the pages of every (sequence, kv head, tile of R packed rows) in units of p.unit, in that order; block w
+// has the units [w step, (w + 1) step).  Lengths are known on the device only, so every block adds them up for itself.
+struct Deal { int before, all; };          // units ahead of sequence b, and altogether
+struct Share { int units, tiles, each; };      // of a sequence; row tiles; units of a tile and head
 template <int R>
 __device__ __forceinline__ Share share_of(const Cache& c, const AttnParams& p, int b, int group) {
     const Entry e = entry_of(c, p, b);
     const int rows = e.n * group;
     Share s;
-    s.pages = max(1, (e.len + kRows - 1) / kRows);                               // a row that sees nothing is somebody's to clear
+    s.each = max(1, ((e.len + kRows - 1) / kRows + p.unit - 1) / p.unit);        // a row that sees nothing is somebody's to clear
     s.tiles = rows <= p.few_rows ? (rows + R - 1) / R : 0;
-    s.units = (int64_t)s.tiles * s.pages * c.kv_heads;
+    s.units = s.tiles * s.each * c.kv_heads;
     return s;
 }
-__device__ __forceinline__ int64_t step_of(const AttnParams& p, int64_t all) {
-    const int64_t even = (all + p.blocks - 1) / p.blocks;
-    return even > kWarps ? even : kWarps;
-}
+__device__ __forceinline__ int step_of(const AttnParams& p, int all) { return max(1, (all + p.blocks - 1) / p.blocks); }
 
 // ---- fragments -------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+// d = a b + (c0, c1, c0, c1)
+__device__ __forceinline__ void mma16816_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -87,12 +89,14 @@ __device__ __forceinline__ float ex2f(float x) {
 }
 // Nibbles at bits 0 and 16 (4 and 20) of w as a pair of fp16 code - 8: 1024 + n (1024 + 16 n) by setting the exponent, then exact arithmetic.
 __device__ __forceinline__ uint32_t low_pair(uint32_t w) {
-    uint32_t v = (w & 0x000f000fu) | 0x64006400u;
+    uint32_t v;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w), "r"(0x000f000fu), "r"(0x64006400u));     // (w & mask) | 1024 in one instruction
     asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(v) : "r"(0x64086408u));                       // 1032
     return v;
 }
 __device__ __forceinline__ uint32_t high_pair(uint32_t w) {
-    uint32_t v = (w & 0x00f000f0u) | 0x64006400u;
+    uint32_t v;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w), "r"(0x00f000f0u), "r"(0x64006400u));
     asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(v) : "r"(0x2c002c00u), "r"(0xd480d480u));   // / 16, - 72
     return v;
 }
@@ -107,7 +111,7 @@ template <int D>
 struct QueryTile {
     static constexpr int G = D / kGroup;
     uint32_t f[G][4][2];
-    float sum[G][2], unit[2];      // of the lane's two columns 2 j, 2 j + 1: sums of the scaled q, and what a score is multiplied with
+    float sum[G][2], eight[G][2], unit[2];      // of the lane's two columns 2 j, 2 j + 1: sums of the scaled q, 8 times those, what a score is multiplied with
 
     template <typename T>
     __device__ __forceinline__ void load(const T* row, bool have, float scale_log2) {       // row: of column lane / 4
@@ -149,7 +153,7 @@ struct QueryTile {
             s[g] += __shfl_xor_sync(0xffffffffu, s[g], 1);
             s[g] += __shfl_xor_sync(0xffffffffu, s[g], 2);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) sum[g][k] = __shfl_sync(0xffffffffu, s[g], (2 * j + k) * 4);
+            for (int k = 0; k < 2; ++k) { sum[g][k] = __shfl_sync(0xffffffffu, s[g], (2 * j + k) * 4); eight[g][k] = 8.0f * sum[g][k]; }
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) unit[k] = __shfl_sync(0xffffffffu, fmaxf(down * scale_log2, 1.2e-38f), (2 * j + k) * 4);     // times -inf: -inf
@@ -202,20 +206,19 @@ __device__ __forceinline__ void score_tile(const uint8_t* page, int u, const Que
     }
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-        float acc[NT][4];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+        float acc[NT][4];                                        // begin with 8 (sum of q): products with the codes themselves
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             const uint32_t a0[4] = {low_pair(ka[g][w]), low_pair(kb[g][w]), high_pair(ka[g][w]), high_pair(kb[g][w])};
             const uint32_t a1[4] = {low_pair(ka[g][w] >> 8), low_pair(kb[g][w] >> 8), high_pair(ka[g][w] >> 8), high_pair(kb[g][w] >> 8)};
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                mma16816(acc[t], a0, q[t].f[g][2 * w][0], q[t].f[g][2 * w][1]);
+                if (w == 0) mma16816_from(acc[t], a0, q[t].f[g][0][0], q[t].f[g][0][1], q[t].eight[g][0], q[t].eight[g][1]);
+                else mma16816(acc[t], a0, q[t].f[g][2][0], q[t].f[g][2][1]);
                 mma16816(acc[t], a1, q[t].f[g][2 * w + 1][0], q[t].f[g][2 * w + 1][1]);
             }
         }
-        const float2 a = centred(pa[g]), b = centred(pb[g]);
+        const float2 a = Num<__half>::two(pa[g]), b = Num<__half>::two(pb[g]);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -246,8 +249,7 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
     using C = FewCfg<D, NT>;
     constexpr int G = L::G, R = 8 * NT;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ int64_t sums[kWarps], before_s[2];
-    __shared__ int first_s;
+    __shared__ int sums[kWarps], before_s, first_s;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
     float2* ml_s = reinterpret_cast<float2*>(bars + kWarps * C::STAGES);         // [warps][R]
     volatile int* abort_s = reinterpret_cast<volatile int*>(ml_s + kWarps * R);
@@ -263,41 +265,40 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
     pdl_launch_dependents();
     // this block's range of the units, and the sequence it begins in
     const int per = (c.batch + kWarps * 32 - 1) / (kWarps * 32), b_lo = min(c.batch, (int)threadIdx.x * per), b_hi = min(c.batch, b_lo + per);
-    int64_t own = 0;
+    int own = 0;
     for (int b = b_lo; b < b_hi; ++b) own += share_of<R>(c, p, b, group).units;
-    int64_t upto = own;
+    int upto = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += v;
     }
     if (lane == 31) sums[warp] = upto;
     __syncthreads();
-    int64_t all = 0;
+    int all = 0;
     for (int w = 0; w < kWarps; ++w) { if (w < warp) upto += sums[w]; all += sums[w]; }
-    const int64_t step = step_of(p, all), u0 = blockIdx.x * step, u1 = min(all, u0 + step);
+    const int step = step_of(p, all), u0 = min((int64_t)all, (int64_t)blockIdx.x * step), u1 = min(all - u0, step) + u0;
     if (u0 >= all) return;
     if (upto - own <= u0 && u0 < upto) {
-        int64_t at = upto - own;
-        int b = b_lo;
-        for (int64_t n; at + (n = share_of<R>(c, p, b, group).units) <= u0; ++b) at += n;
+        int at = upto - own, b = b_lo;
+        for (int n; at + (n = share_of<R>(c, p, b, group).units) <= u0; ++b) at += n;
         first_s = b;
-        before_s[0] = at;
+        before_s = at;
     }
     __syncthreads();
     int b = first_s, slot = 0;                                                   // slot: of the copies and their barriers
-    int64_t start = before_s[0];                                                 // unit that sequence b begins with
+    int start = before_s;                                                 // unit that sequence b begins with
 
-    for (int64_t at = u0; at < u1;) {
+    for (int at = u0; at < u1;) {
         const Share sh = share_of<R>(c, p, b, group);
         if (at >= start + sh.units) { start += sh.units; ++b; continue; }
         const Entry e = entry_of(c, p, b);
         const int rows = e.n * group, pages = (e.len + kRows - 1) / kRows;
-        const int piece = (int)((at - start) / sh.pages), h = piece / sh.tiles, tile = piece % sh.tiles, p0 = (int)((at - start) % sh.pages);
-        const int p1 = (int)min((int64_t)sh.pages, p0 + (u1 - at));              // pages [p0, p1) of this piece
-        const bool from_start = p0 == 0, to_end = p1 == sh.pages;
-        at += p1 - p0;
-        const int mine = max(0, min(p1, pages) - p0 - warp + kWarps - 1) / kWarps;
+        const int piece = (at - start) / sh.each, h = piece / sh.tiles, tile = piece % sh.tiles, first_unit = (at - start) % sh.each;
+        const int last_unit = min(sh.each, first_unit + (u1 - at)), p0 = first_unit * p.unit;
+        const bool from_start = first_unit == 0, to_end = last_unit == sh.each;
+        at += last_unit - first_unit;
+        const int mine = max(0, min(last_unit * p.unit, pages) - p0 - warp + kWarps - 1) / kWarps;      // of the pages from p0 on
         int lane_page = -1;
         uint32_t there = 0;                                                      // bit per stage: its page is one of the pool's
         auto request = [&](int i) {
@@ -582,18 +583,18 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
 }
 
 // Where the keys of a tile of packed rows were dealt: to one block, which finished the rows itself, or to blocks [w0, w1].
-struct Pieces { int64_t w0, w1; };
+struct Pieces { int w0, w1; };
 __device__ __forceinline__ Pieces pieces_of(const AttnParams& p, const Share& s, const Deal& d, int h, int tile) {
-    const int64_t step = step_of(p, d.all), at = d.before + ((int64_t)h * s.tiles + tile) * s.pages;
-    return Pieces{at / step, (at + s.pages - 1) / step};
+    const int step = step_of(p, d.all), at = d.before + (h * s.tiles + tile) * s.each;
+    return Pieces{at / step, (at + s.each - 1) / step};
 }
-__device__ __forceinline__ size_t piece_row(int64_t w, const Pieces& x, int R, int rr) { return ((size_t)2 * w + (w == x.w0 ? 1 : 0)) * R + rr; }
+__device__ __forceinline__ size_t piece_row(int w, const Pieces& x, int R, int rr) { return ((size_t)2 * w + (w == x.w0 ? 1 : 0)) * R + rr; }
 
 // Maximum and sum of packed row rr of a tile over its pieces, by a warp.
 __device__ __forceinline__ float2 merged_stats(const AttnParams& p, const Pieces& x, int R, int rr) {
     const int lane = threadIdx.x & 31;
     float top = -INFINITY, sum = 0.f;
-    for (int64_t w = x.w0 + lane; w <= x.w1; w += 32) {
+    for (int w = x.w0 + lane; w <= x.w1; w += 32) {
         const float2 s = p.part_stats[piece_row(w, x, R, rr)];
         const float mx = fmaxf(top, s.x);
         if (mx != -INFINITY) sum = (top == -INFINITY ? 0.f : sum * ex2f(top - mx)) + (s.x == -INFINITY ? 0.f : s.y * ex2f(s.x - mx));
@@ -609,15 +610,15 @@ constexpr int kMassTokens = 512;      // cached rows of a block that sums weight
 // dealt over several blocks, a row at a time; mass blocks sum the weights of 512 cached rows from the scores it left.
 template <typename T, int D, int R>
 __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c, const AttnParams p, int mass_blocks) {
-    __shared__ int64_t sums[2][kWarps];
+    __shared__ int sums[2][kWarps];
     __shared__ float2 st_s[R];
     __shared__ float4 v_s[kWarps * 32];
     const int h = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = c.q_heads / c.kv_heads;
     pdl_launch_dependents();
     // lengths are not attend_few's to write: where the units lie is known before the wait
-    int64_t before = 0, all = 0;
+    int before = 0, all = 0;
     for (int i = threadIdx.x; i < c.batch; i += kWarps * 32) {
-        const int64_t n = share_of<R>(c, p, i, group).units;
+        const int n = share_of<R>(c, p, i, group).units;
         all += n;
         if (i < b) before += n;
     }
@@ -671,7 +672,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
         const int d = threadIdx.x % Q * 4;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-        for (int64_t w = x.w0 + threadIdx.x / Q; w <= x.w1; w += LANES) {
+        for (int w = x.w0 + threadIdx.x / Q; w <= x.w1; w += LANES) {
             const size_t at = piece_row(w, x, R, rr);
             const float m = p.part_stats[at].x, f = m == -INFINITY ? 0.f : ex2f(m - st.x);
             const float4 y = *reinterpret_cast<const float4*>(p.part + at * D + d);

@@ -106,6 +106,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const Cache c, c
     __shared__ int owner;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int cap = c.max_pages * kRows;
+    pdl_launch_dependents();
+    pdl_wait();
     if (tid == 0) owner = -1;
     __syncthreads();
     for (int b = tid; b < c.batch; b += kAppendThreads) {
@@ -252,6 +254,8 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const Cache c, const
     using L = Tile<D>;
     constexpr int PER = kRows * L::WORDS / kReadThreads;
     const int b = blockIdx.y, h = blockIdx.x % c.kv_heads, k = first / kRows + blockIdx.x / c.kv_heads;
+    pdl_launch_dependents();
+    pdl_wait();
     const int n = min(held(c, lens, b, c.max_pages * kRows), first + rows);
     if (k * kRows >= n) return;
     const int page = page_of(c, b, k);

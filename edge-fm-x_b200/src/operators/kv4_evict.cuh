@@ -65,6 +65,8 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Cache
     extern __shared__ uint32_t keys[];
     __shared__ int hist[kBins], sums[32], found[2], newest_s;
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+    pdl_launch_dependents();
+    pdl_wait();
     const int n = held(c, p.lens_in, b, c.max_pages * kRows);
     const bool over = n > p.limit;
     const int left = over ? p.budget : n;
@@ -169,6 +171,8 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const Cache c,
     using L = Tile<D>;
     constexpr int Q = D / 32;                                    // 16-byte pieces of a row's codes
     const int h = blockIdx.y, b = blockIdx.z;
+    pdl_launch_dependents();
+    pdl_wait();
     const int n = p.n_moves[b * c.kv_heads + h];
     const int2* moves = p.moves + (size_t)(b * c.kv_heads + h) * p.most_moves;
     const int part = threadIdx.x & 15;
