@@ -5,6 +5,7 @@
 #include <exception>
 
 #include "../../operators/kv4_attention.cuh"
+#include "../../operators/kv4_attention_tc.cuh"
 #include "../../operators/kv4_cache.cuh"
 #include "../../operators/kv4_evict.cuh"
 #include "ctx_util.h"
@@ -60,6 +61,9 @@ template <typename T, int D>
 cudaError_t more_smem() {
     cudaError_t e = cudaFuncSetAttribute(kv4::attend_few_kernel<T, D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::FewCfg<D, 1>::SMEM);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_few_kernel<T, D, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::FewCfg<D, 2>::SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_many_kernel<T, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::ManyCfg<D, true>::SMEM);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_many_kernel<T, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::ManyCfg<D, false>::SMEM);
     return e;
 }
 
@@ -128,13 +132,14 @@ efm_status check_attention(const char* call, const efm_kv4_cache* c, const efm_k
 
 // What a call needs: tiles of 8 nt packed query rows, and the parts of its workspace, in floats.
 struct AttnPlan {
-    int max_new, max_len, nt, blocks, unit;
+    int max_new, max_len, nt, blocks, unit, few_rows, many_tiles;      // many_tiles: blocks of 256 packed rows a sequence may have
     bool joined;                                      // pieces of a row may lie in several blocks
     bool scores;                                      // attend_few leaves its scores for the summed weights
     int64_t units, stats, part_stats, part, score_ld, score;
     int64_t bytes() const { return 4 * (stats + part_stats + part + score); }
 };
 constexpr int kSms = 148;                              // of the GPU these kernels are built for
+constexpr int kFewRows = 32;                           // packed rows of a sequence up to which attend_few takes it
 
 AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
     AttnPlan p{};
@@ -142,7 +147,9 @@ AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
     p.max_len = a->max_len > 0 ? a->max_len : (int)capacity(c);
     const int64_t rows = (int64_t)p.max_new * (c->q_heads / c->kv_heads);
     p.nt = rows <= 8 ? 1 : 2;
-    const int64_t R = 8 * p.nt, tiles = (rows + R - 1) / R, pages = std::max(1, (p.max_len + kRows - 1) / kRows);
+    p.few_rows = kFewRows;
+    p.many_tiles = rows > p.few_rows ? (int)((rows + 2 * kv4::kTileRows - 1) / (2 * kv4::kTileRows)) : 0;
+    const int64_t R = 8 * p.nt, tiles = (std::min<int64_t>(rows, p.few_rows) + R - 1) / R, pages = std::max(1, (p.max_len + kRows - 1) / kRows);
     // a page for each warp, or short caches whole: nothing is left to join then
     p.unit = pages <= 2 * kv4::kWarps ? 2 * kv4::kWarps : kv4::kWarps;
     p.units = (pages + p.unit - 1) / p.unit * tiles * c->kv_heads * c->batch;
@@ -289,7 +296,7 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
         p.cu_rows = a->cu_rows; p.lens = a->lens; p.q = a->q; p.out = a->out;
         p.scale_log2 = a->scale * 1.4426950408889634f;
         p.mass_in = a->mass_in; p.mass_out = a->mass_out;
-        p.few_rows = 0x7fffffff; p.blocks = plan.blocks; p.unit = plan.unit; p.rows = plan.max_new;
+        p.few_rows = plan.few_rows; p.blocks = plan.blocks; p.unit = plan.unit; p.rows = plan.max_new;
         float* ws = (float*)a->workspace;
         p.stats = plan.stats > 0 ? (float2*)ws : nullptr;
         p.part_stats = (float2*)(ws + plan.stats);
@@ -303,10 +310,15 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
             const dim3 block(kv4::kWarps * 32);
             const kv4::Cache c = device_cache(cache);
             const int64_t rows = (int64_t)plan.max_new * (cache->q_heads / cache->kv_heads);
-            const int merges = plan.joined ? (int)std::min<int64_t>(64, rows) : 0, masses = plan.scores ? (plan.max_len + kv4::kMassTokens - 1) / kv4::kMassTokens : 0;
+            const int merges = plan.joined ? (int)std::min<int64_t>(64, std::min<int64_t>(rows, plan.few_rows)) : 0, masses = plan.scores ? (plan.max_len + kv4::kMassTokens - 1) / kv4::kMassTokens : 0;
             const dim3 join(merges + masses, cache->kv_heads, cache->batch);
             if (rows > 0 && plan.nt == 1) L.launch(kv4::attend_few_kernel<T, D, 1>, dim3(plan.blocks), block, kv4::FewCfg<D, 1>::SMEM, c, p);
             if (rows > 0 && plan.nt == 2) L.launch(kv4::attend_few_kernel<T, D, 2>, dim3(plan.blocks), block, kv4::FewCfg<D, 2>::SMEM, c, p);
+            const dim3 many(plan.many_tiles, cache->kv_heads, cache->batch);
+            if (plan.many_tiles > 0) {
+                if (cache->dtype == EFM_F16 || p.mass_out != nullptr) L.launch(kv4::attend_many_kernel<T, D, true>, many, dim3(kv4::kManyThreads), kv4::ManyCfg<D, true>::SMEM, c, p);
+                else if constexpr (std::is_same<T, __nv_bfloat16>::value) L.launch(kv4::attend_many_kernel<T, D, false>, many, dim3(kv4::kManyThreads), kv4::ManyCfg<D, false>::SMEM, c, p);
+            }
             if (join.x > 0 && plan.nt == 1) L.launch(kv4::attend_merge_kernel<T, D, 8>, join, block, 0, c, p, masses);
             if (join.x > 0 && plan.nt == 2) L.launch(kv4::attend_merge_kernel<T, D, 16>, join, block, 0, c, p, masses);
             if (p.mass_out != nullptr && !plan.scores)

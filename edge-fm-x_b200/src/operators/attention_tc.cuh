@@ -82,6 +82,16 @@ __device__ __forceinline__ void umma_d(uint32_t tmem_d, uint64_t adesc, uint64_t
         "}\n"
         ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
+// D = A . B with A in tensor memory (pairs of 16-bit values along K in 32-bit columns) and B by shared-memory descriptor
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "}\n"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
 // MN-major operand tile written by TMA with the 128-byte swizzle (rows = K index, 128 bytes = 64 MN elements per row):
 // leading byte offset = distance between 64-element blocks along MN, stride byte offset = distance between 8-row groups
 // along K.

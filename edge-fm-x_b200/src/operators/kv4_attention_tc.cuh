@@ -1,0 +1,425 @@
+// Many query rows against a 4-bit cache on the 5th-generation tensor cores.
+//
+// Block = 256 packed rows (new rows x heads of a group) of one sequence and kv head, as two tiles of 128 that share the keys and values;
+// 13 warps:
+//   warps 0-3, 4-7   softmax of a tile, a thread per row: S from tensor memory, p = 2^(s - m), P back into tensor memory as fp16, where the
+//                    product takes it as its A operand.  O stays in tensor memory; it is scaled only when a row's maximum has grown by
+//                    more than 2^8 since it was last, which a row's first pages see and later ones hardly;
+//   warps 8-11       pages by bulk copies (a ring of three), codes to fp16 values (min + scale * code, rounded once), written in the
+//                    operands' 128-byte-swizzled layout: K-major rows of K, and the same rows of V read MN-major;
+//   warp 12          one lane issues the products: S = Q K^T (M 128, N 64, K = head size), O += P V (M 128, N = head size, K 64).  S has two
+//                    buffers a tile and runs two pages ahead of P V; weights take the place of the scores they came from.
+// q is scaled by a power of two per row to be exact in fp16.  k, v and p are rounded to fp16 (2^-11), well below the half step of a bf16
+// output (2^-8).  Where that would show (X: fp16 outputs, and row sums that weights are divided by) each is a pair high + low instead:
+// S = Q (Kh + Kl), O += Ph Vh + Pl Vh + Ph Vl.
+// A barrier is waited for by parity, which tells a phase from its neighbours only: every barrier here is either waited for in each of its
+// phases by whoever its next phase needs, or (o_done) has a copy per page parity, whose next phase needs the waiting thread's weights of
+// two pages later.
+// Bound: tensor pipe (4 rows keys D flops), and close to it the exponentials and the conversion of the codes.
+#pragma once
+#include <type_traits>
+
+#include "attention_tc.cuh"
+#include "kv4_attention.cuh"
+
+namespace efm {
+namespace kv4 {
+
+constexpr int kTileRows = 128, kManyThreads = 13 * 32;
+
+template <int D, bool X>
+struct ManyCfg {
+    static constexpr int G = D / 64;
+    static constexpr int KS = X ? 2 : 3, VS = 2, LEAD = KS - 1, RAW = LEAD + 2;          // K is converted LEAD pages ahead of V; pages in the ring of raw ones
+    static constexpr int Q_BYTES = kTileRows * 128 * G, LOW = kRows * 128 * G;           // of one tile; of K or V of a page, and where its low half begins
+    static constexpr int KV_BYTES = X ? 2 * LOW : LOW;
+    static constexpr int Q_AT = 0, K_AT = 2 * Q_BYTES, V_AT = K_AT + KS * KV_BYTES, RAW_AT = V_AT + VS * KV_BYTES, BARS = RAW_AT + RAW * Tile<D>::BYTES;
+    static constexpr int S_COL = 0, O_COL = 256;                                         // S of (tile, page parity): 64 columns each, P in its place; O: 128 a tile
+    static constexpr size_t SMEM = BARS + 304 + 1024;
+};
+
+// Pairs of fp16 codes of a word, in the order of the channels: as in low_pair / high_pair, without the 8.
+__device__ __forceinline__ void half_codes(uint32_t w, __half2 (&n)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t x;
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(i < 2 ? w : w >> 8), "r"((i & 1) ? 0x00f000f0u : 0x000f000fu), "r"(0x64006400u));
+        if (i & 1) asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(x) : "r"(0x2c002c00u), "r"(0xd400d400u));
+        else asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0x64006400u));
+        n[i] = *reinterpret_cast<__half2*>(&x);
+    }
+}
+__device__ __forceinline__ uint4 four(const __half2 (&x)[4]) {
+    const uint32_t* u = reinterpret_cast<const uint32_t*>(x);
+    return make_uint4(u[0], u[1], u[2], u[3]);
+}
+// min + scale * code of a word's eight codes, rounded once
+__device__ __forceinline__ uint4 half_values(uint32_t w, __half2 par) {
+    const __half2 s = __low2half2(par), m = __high2half2(par);
+    __half2 n[4];
+    half_codes(w, n);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n[i] = __hfma2(n[i], s, m);
+    return four(n);
+}
+// the same as high + low: the product's and the sum's rounding errors, both exact, added up
+__device__ __forceinline__ void half_pairs(uint32_t w, __half2 par, uint4& high, uint4& low) {
+    const __half2 s = __low2half2(par), m = __high2half2(par);
+    __half2 n[4], h[4];
+    half_codes(w, n);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 x = __hmul2_rn(n[i], s), xl = __hfma2(n[i], s, __hneg2(x));
+        h[i] = __hadd2_rn(m, x);
+        const __half2 back = __hsub2_rn(h[i], m);
+        n[i] = __hadd2_rn(__hadd2_rn(__hsub2_rn(m, __hsub2_rn(h[i], back)), __hsub2_rn(x, back)), xl);
+    }
+    high = four(h);
+    low = four(n);
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+        "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&r)[64]) {
+#pragma unroll
+    for (int i = 0; i < 64; i += 32)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+            "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+            : "=f"(r[i]), "=f"(r[i + 1]), "=f"(r[i + 2]), "=f"(r[i + 3]), "=f"(r[i + 4]), "=f"(r[i + 5]), "=f"(r[i + 6]), "=f"(r[i + 7]), "=f"(r[i + 8]), "=f"(r[i + 9]), "=f"(r[i + 10]),
+              "=f"(r[i + 11]), "=f"(r[i + 12]), "=f"(r[i + 13]), "=f"(r[i + 14]), "=f"(r[i + 15]), "=f"(r[i + 16]), "=f"(r[i + 17]), "=f"(r[i + 18]), "=f"(r[i + 19]), "=f"(r[i + 20]),
+              "=f"(r[i + 21]), "=f"(r[i + 22]), "=f"(r[i + 23]), "=f"(r[i + 24]), "=f"(r[i + 25]), "=f"(r[i + 26]), "=f"(r[i + 27]), "=f"(r[i + 28]), "=f"(r[i + 29]), "=f"(r[i + 30]),
+              "=f"(r[i + 31])
+            : "r"(taddr + i) : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// grid (tiles of 256 packed rows, kv heads, batch); late rows see the most keys and come first
+template <typename T, int D, bool X>
+__global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cache c, const AttnParams p) {
+    using C = ManyCfg<D, X>;
+    using L = Tile<D>;
+    constexpr int G = C::G;
+    constexpr float kGrow = 8.0f, kLift = 7.0f;                  // p is up to 2^(8 + 7): fp16 keeps weights down to 2^-21 of the largest whole
+    extern __shared__ unsigned char many_smem[];
+    const uint32_t raw_base = tc::smem_u32(many_smem), base = (raw_base + 1023u) & ~1023u;
+    unsigned char* sm = many_smem + (base - raw_base);
+    const uint32_t bars = base + C::BARS;
+    const uint32_t q_full = bars, raw_full = bars + 8, raw_empty = bars + 40, k_full = bars + 72, k_empty = bars + 96, v_full = bars + 120, v_empty = bars + 136,
+                   s_full = bars + 152, p_full = bars + 184, o_done = bars + 216, drain = bars + 248;     // s_full, p_full, o_done: [tile][page parity]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::BARS + 256);
+    volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* there = reinterpret_cast<volatile int*>(tmem_slot + 2);        // [8] page j % 8 is one of the pool's
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y, b = blockIdx.z, group = c.q_heads / c.kv_heads;
+
+    pdl_wait();
+    const Entry e = entry_of(c, p, b);
+    const int rows = e.n * group, r0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * 2 * kTileRows;
+    if (rows <= p.few_rows || r0 >= rows) return;
+    const int nt = rows - r0 > kTileRows ? 2 : 1;                                // tiles in use
+    const int last = min(rows, r0 + 2 * kTileRows) - 1;
+    const int n = (max(0, min(e.len, e.len - e.n + last / group + 1)) + kRows - 1) / kRows;      // pages that any of the rows sees
+    if (tid == 0) {
+        tc::mbar_init(q_full, 128 * nt);
+        for (int i = 0; i < C::RAW; ++i) { tc::mbar_init(raw_full + 8 * i, 1); tc::mbar_init(raw_empty + 8 * i, 4); }
+        tc::mbar_init(drain, 1);
+        for (int i = 0; i < C::KS; ++i) { tc::mbar_init(k_full + 8 * i, 4); tc::mbar_init(k_empty + 8 * i, 1); }
+        for (int i = 0; i < C::VS; ++i) { tc::mbar_init(v_full + 8 * i, 4); tc::mbar_init(v_empty + 8 * i, 1); }
+        for (int i = 0; i < 4; ++i) { tc::mbar_init(s_full + 8 * i, 1); tc::mbar_init(p_full + 8 * i, 128); tc::mbar_init(o_done + 8 * i, 1); }
+        *abort_s = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    pdl_launch_dependents();                                     // not before this block has its tensor memory
+
+    if (warp < 8) {
+        const int t = warp >> 2, tr = (warp & 3) * 32 + lane, row = r0 + t * kTileRows + tr;
+        if (t < nt) {
+            const bool have = row < rows;
+            const size_t at = ((size_t)(e.row0 + row / group) * c.q_heads + h * group + row % group) * D;
+            const T* q = (const T*)p.q + at;
+            const int see = have ? max(0, min(e.len, e.len - e.n + row / group + 1)) : 0;
+            int least = have ? see : INT32_MAX;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
+            // the row into its operand, scaled by a power of two
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                if (have) w = *reinterpret_cast<const uint4*>(q + 8 * i);
+                const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) { const float2 x = Num<T>::two(v[k]); top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y))); }
+            }
+            const int bits = (int)(__float_as_uint(top) >> 23), ex = bits == 255 ? 3 : max(bits - 127, -100);
+            const float up = __uint_as_float((uint32_t)(130 - ex) << 23), unit = fmaxf(__uint_as_float((uint32_t)(ex + 124) << 23) * p.scale_log2, 1.2e-38f);
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                if (have) w = *reinterpret_cast<const uint4*>(q + 8 * i);
+                uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) { const float2 x = Num<T>::two(v[k]); v[k] = half_pair(x.x * up, x.y * up); }
+                *reinterpret_cast<uint4*>(sm + C::Q_AT + t * C::Q_BYTES + (i >> 3) * (kTileRows * 128) + tr * 128 + (((i & 7) ^ (tr & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(q_full);
+
+            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+            const uint32_t o_at = tmem + lanes + (uint32_t)(C::O_COL + t * 128);
+            float m = -INFINITY, l = 0.f;                        // m: what the row's weights are relative to
+            int j = 0;
+            for (; j < n; ++j) {
+                const int buf = t * 2 + (j & 1);
+                const uint32_t s_at = tmem + lanes + (uint32_t)(C::S_COL + buf * 64);
+                if (!__all_sync(0xffffffffu, tc::mbar_wait(s_full + 8 * buf, (uint32_t)(j >> 1) & 1u, abort_s))) { *abort_s = 1; break; }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                float s[64];
+                tmem_ld64(s_at, s);
+                const int seen = there[j & 7] ? see - j * kRows : 0;             // keys of the page that the row sees
+                if (there[j & 7] == 0 || (j + 1) * kRows > least) {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) if (i >= seen) s[i] = -INFINITY;
+                }
+                float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int i = 4; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+                const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * unit;
+                const bool grow = mn > m + kGrow || (m == -INFINITY && mn != -INFINITY);
+                float alpha = 1.0f;
+                if (grow) { alpha = at::ex2(m - mn); l *= alpha; m = mn; }
+                const float off = m == -INFINITY ? kLift : kLift - m;
+                uint32_t pk[32], pl[X ? 32 : 1];
+                float sum[2] = {0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < 64; i += 2) {
+                    const float a = at::ex2(fmaf(s[i], unit, off)), bb = at::ex2(fmaf(s[i + 1], unit, off));
+                    sum[0] += a;
+                    sum[1] += bb;
+                    pk[i >> 1] = half_pair(a, bb);
+                    if constexpr (X) {
+                        const float2 r = Num<__half>::two(pk[i >> 1]);
+                        pl[i >> 1] = half_pair(a - r.x, bb - r.y);
+                    }
+                }
+                l += sum[0] + sum[1];
+                if (j > 0 && __any_sync(0xffffffffu, grow)) {    // O once P V of the page before is through
+                    if (!__all_sync(0xffffffffu, tc::mbar_wait(o_done + 8 * (buf ^ 1), (uint32_t)((j - 1) >> 1) & 1u, abort_s))) { *abort_s = 1; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                    for (int d = 0; d < D; d += 32) {
+                        uint32_t x[32];
+                        tc::tmem_ld32(o_at + d, x);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * alpha);
+                        tmem_st32(o_at + d, x);
+                    }
+                }
+                tmem_st32(s_at, pk);
+                if constexpr (X) tmem_st32(s_at + 32, pl);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                mbar_arrive(p_full + 8 * buf);
+            }
+            const bool done = j == n && (n == 0 || __all_sync(0xffffffffu, tc::mbar_wait(o_done + 8 * (t * 2 + ((n - 1) & 1)), (uint32_t)((n - 1) >> 1) & 1u, abort_s)));
+            if (!done) *abort_s = 1;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (done) {
+                const float inv = l > 0.f ? 1.0f / l : l != l ? l : 0.f;
+                T* out = (T*)p.out + at;
+#pragma unroll 1
+                for (int d = 0; d < D; d += 32) {
+                    uint32_t x[32];
+                    if (n > 0) tc::tmem_ld32(o_at + d, x);
+                    else
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) x[i] = 0u;
+                    if (have)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            uint32_t y[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) y[k] = Num<T>::pack(__uint_as_float(x[i + 2 * k]) * inv, __uint_as_float(x[i + 2 * k + 1]) * inv);
+                            *reinterpret_cast<uint4*>(out + d + i) = make_uint4(y[0], y[1], y[2], y[3]);
+                        }
+                }
+                if (have && p.stats != nullptr) p.stats[stat_row(c, p, b, row / group, h * group + row % group)] = make_float2(m == -INFINITY ? m : m - kLift, l);
+            }
+        }
+    } else if (warp < 12) {
+        const int dw = warp - 8, dt = tid - 8 * 32;
+        int lane_page = -1;
+        auto request = [&](int j) {                              // by warp 8
+            if ((j & 31) == 0) {
+                const bool in = j + lane < n;
+                lane_page = in ? c.page_table[(size_t)b * c.max_pages + j + lane] : -1;
+                if ((unsigned)lane_page >= (unsigned)c.n_pages) { if (in) raise(c, kBadPage); lane_page = -1; }
+            }
+            const int page = __shfl_sync(0xffffffffu, lane_page, j & 31);
+            const uint32_t bar = raw_full + 8 * (j % C::RAW);
+            if (lane == 0) {
+                there[j & 7] = page >= 0;
+                if (page >= 0) {
+                    tc::mbar_expect_tx(bar, L::BYTES);
+                    bulk_copy(base + C::RAW_AT + (j % C::RAW) * L::BYTES, tile_of<D>(c, page, h), L::BYTES, bar);
+                } else {
+                    mbar_arrive(bar);
+                }
+            }
+        };
+        auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_s)); };
+        auto convert = [&](auto values, int j, uint32_t full) {  // K or V of page j, by all four warps
+            constexpr bool V = decltype(values)::value;
+            const uint8_t* page = sm + C::RAW_AT + (j % C::RAW) * L::BYTES;
+            const int valid = there[j & 7] ? min(kRows, e.len - j * kRows) : 0;
+            unsigned char* to = sm + (V ? C::V_AT + (j % C::VS) * C::KV_BYTES : C::K_AT + (j % C::KS) * C::KV_BYTES);
+            const uint32_t* codes = reinterpret_cast<const uint32_t*>(page + (V ? L::V_CODES : L::K_CODES));
+            const __half2* pars = reinterpret_cast<const __half2*>(page + (V ? L::V_PARAMS : L::K_PARAMS));
+#pragma unroll
+            for (int it = 0; it < 2; ++it) {
+                const int r = it * 32 + (dt >> 2), x = dt & 3;                   // row, quarter of its groups
+                uint32_t w[G][2];
+                if constexpr (G == 2 && !V) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(codes + r * L::WORDS + x * 4);
+                    w[0][0] = v.x; w[0][1] = v.y; w[1][0] = v.z; w[1][1] = v.w;
+                } else {
+#pragma unroll
+                    for (int g = 0; g < G; ++g) { const uint2 v = *reinterpret_cast<const uint2*>(codes + r * L::WORDS + g * 8 + x * 2); w[g][0] = v.x; w[g][1] = v.y; }
+                }
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    __half2 par = pars[r * G + g];
+                    if (r >= valid) par = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        uint4* dst = reinterpret_cast<uint4*>(to + g * (kRows * 128) + r * 128 + (((2 * x + i) ^ (r & 7)) << 4));
+                        if constexpr (X) {
+                            uint4 high, low;
+                            half_pairs(w[g][i], par, high, low);
+                            *dst = high;
+                            dst[C::LOW / 16] = low;
+                        } else {
+                            *dst = half_values(w[g][i], par);
+                        }
+                    }
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full);
+        };
+        int asked = 0;
+        if (dw == 0) for (; asked < min(n, C::RAW); ++asked) request(asked);
+        int i = 0;
+        for (; i < n + C::LEAD; ++i) {
+            if (i < n) {
+                if (!wait(raw_full + 8 * (i % C::RAW), (uint32_t)(i / C::RAW) & 1u)) break;
+                if (i >= C::KS && !wait(k_empty + 8 * (i % C::KS), (uint32_t)(i / C::KS - 1) & 1u)) break;
+                convert(std::false_type(), i, k_full + 8 * (i % C::KS));
+            }
+            const int j = i - C::LEAD;
+            if (j < 0) continue;
+            if (j >= C::VS && !wait(v_empty + 8 * (j % C::VS), (uint32_t)(j / C::VS - 1) & 1u)) break;
+            convert(std::true_type(), j, v_full + 8 * (j % C::VS));
+            if (lane == 0) mbar_arrive(raw_empty + 8 * (j % C::RAW));
+            if (dw == 0 && asked < n) {                          // once all four warps have read page j
+                if (!wait(raw_empty + 8 * (j % C::RAW), (uint32_t)(j / C::RAW) & 1u)) break;
+                request(asked++);
+            }
+        }
+        if (i < n + C::LEAD) *abort_s = 1;
+    } else {
+        // The whole warp walks the loop, so that addresses and descriptors stay in uniform registers; one lane issues.  With a loop of that
+        // lane alone the issue of 24 products a page took 2500 cycles, more than everything else.
+        constexpr uint32_t kDescS = at::instr_desc_f16(kTileRows, kRows), kDescO = at::instr_desc_f16(kTileRows, D) | (1u << 16);
+        uint32_t lead;
+        asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(lead));
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint64_t qd = tc::umma_desc(base + C::Q_AT), kd = tc::umma_desc(base + C::K_AT), vd = at::umma_desc_mn(base + C::V_AT, (uint32_t)(kRows * 128), 1024u);
+        auto issue_s = [&](int t, int j) {                       // into the buffer of the page's parity
+            if (lead) {
+                const int st = j % C::KS, buf = t * 2 + (j & 1);
+                const uint64_t qt = qd + (uint64_t)(t * (C::Q_BYTES >> 4)), kt = kd + (uint64_t)(st * (C::KV_BYTES >> 4));
+                const uint32_t to = tm + (uint32_t)(C::S_COL + buf * 64);
+#pragma unroll
+                for (int i = 0; i < (X ? 2 : 1) * (D / 16); ++i) {
+                    const int k = i % (D / 16), low = i / (D / 16);
+                    at::umma_d(to, qt + (uint64_t)((k >> 2) * (kTileRows * 128 >> 4) + (k & 3) * 2), kt + (uint64_t)((low * C::LOW + (k >> 2) * (kRows * 128)) / 16 + (k & 3) * 2), kDescS, i != 0 ? 1u : 0u);
+                }
+                tc::umma_commit(s_full + 8 * buf);
+                if (t == nt - 1) tc::umma_commit(k_empty + 8 * st);
+            }
+            __syncwarp();
+        };
+        auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_s)); };
+        bool ok = n > 0 && wait(q_full, 0);
+        for (int j = 0; j < min(n, 2) && ok; ++j) {
+            ok = wait(k_full + 8 * j, 0);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int t = 0; t < nt; ++t) issue_s(t, j);
+        }
+        for (int j = 0; j < n && ok; ++j) {
+            const int st = j & 1;
+            const uint32_t ph = (uint32_t)(j >> 1) & 1u;
+            // what the products need besides the weights first: it is there long before them
+            ok = wait(v_full + 8 * st, ph) && (j + 2 >= n || wait(k_full + 8 * ((j + 2) % C::KS), (uint32_t)((j + 2) / C::KS) & 1u));
+            for (int t = 0; t < nt && ok; ++t) {
+                ok = wait(p_full + 8 * (t * 2 + st), ph);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (lead) {
+                    const uint64_t vt = vd + (uint64_t)(st * (C::KV_BYTES >> 4));
+                    const uint32_t to = tm + (uint32_t)(C::O_COL + t * 128), from = tm + (uint32_t)(C::S_COL + (t * 2 + st) * 64);
+#pragma unroll
+                    for (int i = 0; i < (X ? 3 : 1) * (kRows / 16); ++i) {
+                        const int k = i % (kRows / 16), part = i / (kRows / 16);                   // Ph Vh, Pl Vh, Ph Vl
+                        at::umma_ts(to, from + (uint32_t)((part == 1 ? 32 : 0) + 8 * k), vt + (uint64_t)((part == 2 ? C::LOW : 0) / 16 + k * (2048 >> 4)), kDescO, i != 0 || j > 0 ? 1u : 0u);
+                    }
+                    tc::umma_commit(o_done + 8 * (t * 2 + st));
+                    if (t == nt - 1) tc::umma_commit(v_empty + 8 * st);
+                }
+                __syncwarp();
+                if (j + 2 < n) issue_s(t, j + 2);                // behind P V, which reads the weights in that place
+            }
+        }
+        if (n > 0 && !ok) {                                      // given up: the products issued end before the block leaves (bounded)
+            *abort_s = 1;
+            volatile int go_on = 0;
+            if (lead) tc::umma_commit(drain);
+            __syncwarp();
+            (void)tc::mbar_wait(drain, 0, &go_on);
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (*abort_s != 0 && tid == 0) {                             // and the copies land
+        volatile int go_on = 0;
+        for (int i = 0; i < C::RAW; ++i) { (void)tc::mbar_wait(raw_full + 8 * i, 0, &go_on); (void)tc::mbar_wait(raw_full + 8 * i, 1, &go_on); }
+        raise(c, kWait);
+    }
+    __syncthreads();
+    if (warp == 12) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+}  // namespace kv4
+}  // namespace efm
