@@ -62,6 +62,7 @@ cudaError_t more_smem() {
     cudaError_t e = cudaFuncSetAttribute(kv4::attend_few_kernel<T, D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::FewCfg<D, 1>::SMEM);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_few_kernel<T, D, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::FewCfg<D, 2>::SMEM);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_many_kernel<T, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::ManyCfg<D, true>::SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_weights_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::WeightsCfg<D>::SMEM);
     if constexpr (std::is_same<T, __nv_bfloat16>::value)
         if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_many_kernel<T, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::ManyCfg<D, false>::SMEM);
     return e;
@@ -319,11 +320,12 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
                 if (cache->dtype == EFM_F16 || p.mass_out != nullptr) L.launch(kv4::attend_many_kernel<T, D, true>, many, dim3(kv4::kManyThreads), kv4::ManyCfg<D, true>::SMEM, c, p);
                 else if constexpr (std::is_same<T, __nv_bfloat16>::value) L.launch(kv4::attend_many_kernel<T, D, false>, many, dim3(kv4::kManyThreads), kv4::ManyCfg<D, false>::SMEM, c, p);
             }
+            L.pdl = rows > 0;                          // what follows reads lengths ahead of its wait: not as a call's first launch
             if (join.x > 0 && plan.nt == 1) L.launch(kv4::attend_merge_kernel<T, D, 8>, join, block, 0, c, p, masses);
             if (join.x > 0 && plan.nt == 2) L.launch(kv4::attend_merge_kernel<T, D, 16>, join, block, 0, c, p, masses);
             if (p.mass_out != nullptr && !plan.scores)
-                L.launch(kv4::attend_mass_kernel<T, D>, dim3((plan.max_len + kRows * kv4::kWarps - 1) / (kRows * kv4::kWarps), cache->kv_heads, cache->batch), block,
-                         kv4::MassCfg<D>::SMEM, c, p);
+                L.launch(kv4::attend_weights_kernel<T, D>, dim3((plan.max_len + kv4::WeightsCfg<D>::KEYS - 1) / kv4::WeightsCfg<D>::KEYS, cache->kv_heads, cache->batch),
+                         dim3(kv4::kWeightThreads), kv4::WeightsCfg<D>::SMEM, c, p);
         });
         return launched(call, L);
     });

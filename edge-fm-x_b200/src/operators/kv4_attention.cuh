@@ -690,85 +690,5 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
     }
 }
 
-template <int D>
-struct MassCfg {
-    static constexpr int K_BYTES = Tile<D>::V_CODES;                             // codes and parameters of the keys
-    static constexpr size_t SMEM = (size_t)kWarps * K_BYTES + kWarps * 8 + 16;
-};
-
-// Summed weights where scores were not kept (more packed rows than a tile): the keys once more.  grid (groups of pages, kv heads, batch); a
-// warp has a page of its own and walks the new rows in order, eight packed rows at a time, so that sums need no atomics.
-template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32) attend_mass_kernel(const Cache c, const AttnParams p) {
-    using C = MassCfg<D>;
-    extern __shared__ __align__(128) unsigned char smem[];
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (size_t)kWarps * C::K_BYTES);
-    volatile int* abort_s = reinterpret_cast<volatile int*>(bars + kWarps);
-    const int h = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3, group = c.q_heads / c.kv_heads;
-    pdl_launch_dependents();
-    const Entry e = entry_of(c, p, b);
-    const int pages = (e.len + kRows - 1) / kRows, pg = blockIdx.x * kWarps + warp;
-    if (threadIdx.x == 0) *abort_s = 0;
-    __syncthreads();
-    const int page = pg < pages ? page_of(c, b, pg) : -1;
-    if (page < 0) { pdl_wait(); return; }
-    const uint32_t bar = tc::smem_u32(bars + warp);
-    uint8_t* tile = smem + (size_t)warp * C::K_BYTES;
-    if (lane == 0) {
-        tc::mbar_init(bar, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        tc::mbar_expect_tx(bar, C::K_BYTES);
-        bulk_copy(tc::smem_u32(tile), tile_of<D>(c, page, h), C::K_BYTES, bar);
-    }
-    __syncwarp();
-    pdl_wait();
-    if (!__all_sync(0xffffffffu, tc::mbar_wait(bar, 0, abort_s))) { if (lane == 0) raise(c, kWait); return; }
-    const int first = pg * kRows, valid = min(kRows, e.len - first), rows = e.n * group;
-    if (valid < kRows) clear_rows<D>(tile, valid, false);
-    float w[4][2];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) w[u][0] = w[u][1] = 0.f;
-    const int row_first = max(0, first - (e.len - e.n)) * group;                 // earlier rows do not see the page
-    for (int r0 = row_first & ~7; r0 < rows; r0 += 8) {
-        QueryTile<D> q[1];
-        const int row = r0 + r;
-        q[0].load((const T*)p.q + ((size_t)(e.row0 + row / group) * c.q_heads + h * group + row % group) * D, row < rows, p.scale_log2);
-        const float2 st = row < rows ? p.stats[stat_row(c, p, b, row / group, h * group + row % group)] : make_float2(-INFINITY, 0.f);
-        const float mine = st.x == -INFINITY ? 0.f : st.x, one = st.x == -INFINITY ? 0.f : 1.0f / st.y;
-        float top[2], inv[2];
-        int see[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            top[k] = __shfl_sync(0xffffffffu, mine, (2 * j + k) * 4);
-            inv[k] = __shfl_sync(0xffffffffu, one, (2 * j + k) * 4);
-            const int cr = r0 + 2 * j + k;
-            see[k] = cr < rows ? min(e.len, e.len - e.n + cr / group + 1) : 0;
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            float s[1][4];
-            score_tile<D, 1>(tile, u, q, s);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float x = ex2f(fmaf(s[0][k], q[0].unit[k & 1], -top[k & 1])) * inv[k & 1];
-                if (first + u * 16 + token_of(r) + 8 * (k >> 1) < see[k & 1]) w[u][k >> 1] += x;
-            }
-        }
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-            float x = w[u][hf];
-            x += __shfl_xor_sync(0xffffffffu, x, 1);
-            x += __shfl_xor_sync(0xffffffffu, x, 2);
-            const int tk = u * 16 + token_of(r) + 8 * hf;
-            if (j == 0 && tk < valid) {
-                const size_t at = row_slot(c, page, h, tk);
-                p.mass_out[at] = p.mass_in[at] + x;
-            }
-        }
-}
-
 }  // namespace kv4
 }  // namespace efm

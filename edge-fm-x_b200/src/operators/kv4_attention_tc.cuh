@@ -101,6 +101,49 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&r)[64]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t lead;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(lead));
+    return lead;
+}
+// A query row into row r of a K-major operand of 128 rows, as fp16 scaled by a power of two; returns what a score is to be multiplied with.
+template <typename T, int D>
+__device__ __forceinline__ float query_row(const T* q, bool have, unsigned char* to, int r, float scale_log2) {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (have) w = *reinterpret_cast<const uint4*>(q + 8 * i);
+        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { const float2 x = Num<T>::two(v[k]); top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y))); }
+    }
+    const int bits = (int)(__float_as_uint(top) >> 23), ex = bits == 255 ? 3 : max(bits - 127, -100);
+    const float up = __uint_as_float((uint32_t)(130 - ex) << 23);
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (have) w = *reinterpret_cast<const uint4*>(q + 8 * i);
+        uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { const float2 x = Num<T>::two(v[k]); v[k] = half_pair(x.x * up, x.y * up); }
+        *reinterpret_cast<uint4*>(to + (i >> 3) * (kTileRows * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+    return fmaxf(__uint_as_float((uint32_t)(ex + 124) << 23) * scale_log2, 1.2e-38f);
+}
+// The two words of a key row's quarter x of each group
+template <int D, bool V>
+__device__ __forceinline__ void quarter_words(const uint32_t* codes, int r, int x, uint32_t (&w)[D / 64][2]) {
+    constexpr int W = D / 8;
+    if constexpr (D == 128 && !V) {
+        const uint4 v = *reinterpret_cast<const uint4*>(codes + r * W + x * 4);
+        w[0][0] = v.x; w[0][1] = v.y; w[1][0] = v.z; w[1][1] = v.w;
+    } else {
+#pragma unroll
+        for (int g = 0; g < D / 64; ++g) { const uint2 v = *reinterpret_cast<const uint2*>(codes + r * W + g * 8 + x * 2); w[g][0] = v.x; w[g][1] = v.y; }
+    }
+}
+
 // grid (tiles of 256 packed rows, kv heads, batch); late rows see the most keys and come first
 template <typename T, int D, bool X>
 __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cache c, const AttnParams p) {
@@ -156,27 +199,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             int least = have ? see : INT32_MAX;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
-            // the row into its operand, scaled by a power of two
-            float top = 0.f;
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                if (have) w = *reinterpret_cast<const uint4*>(q + 8 * i);
-                const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) { const float2 x = Num<T>::two(v[k]); top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y))); }
-            }
-            const int bits = (int)(__float_as_uint(top) >> 23), ex = bits == 255 ? 3 : max(bits - 127, -100);
-            const float up = __uint_as_float((uint32_t)(130 - ex) << 23), unit = fmaxf(__uint_as_float((uint32_t)(ex + 124) << 23) * p.scale_log2, 1.2e-38f);
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                if (have) w = *reinterpret_cast<const uint4*>(q + 8 * i);
-                uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) { const float2 x = Num<T>::two(v[k]); v[k] = half_pair(x.x * up, x.y * up); }
-                *reinterpret_cast<uint4*>(sm + C::Q_AT + t * C::Q_BYTES + (i >> 3) * (kTileRows * 128) + tr * 128 + (((i & 7) ^ (tr & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
-            }
+            const float unit = query_row<T, D>(q, have, sm + C::Q_AT + t * C::Q_BYTES, tr, p.scale_log2);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_arrive(q_full);
 
@@ -294,13 +317,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             for (int it = 0; it < 2; ++it) {
                 const int r = it * 32 + (dt >> 2), x = dt & 3;                   // row, quarter of its groups
                 uint32_t w[G][2];
-                if constexpr (G == 2 && !V) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(codes + r * L::WORDS + x * 4);
-                    w[0][0] = v.x; w[0][1] = v.y; w[1][0] = v.z; w[1][1] = v.w;
-                } else {
-#pragma unroll
-                    for (int g = 0; g < G; ++g) { const uint2 v = *reinterpret_cast<const uint2*>(codes + r * L::WORDS + g * 8 + x * 2); w[g][0] = v.x; w[g][1] = v.y; }
-                }
+                quarter_words<D, V>(codes, r, x, w);
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
                     __half2 par = pars[r * G + g];
@@ -347,8 +364,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
         // The whole warp walks the loop, so that addresses and descriptors stay in uniform registers; one lane issues.  With a loop of that
         // lane alone the issue of 24 products a page took 2500 cycles, more than everything else.
         constexpr uint32_t kDescS = at::instr_desc_f16(kTileRows, kRows), kDescO = at::instr_desc_f16(kTileRows, D) | (1u << 16);
-        uint32_t lead;
-        asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(lead));
+        const uint32_t lead = elect_one();
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
         const uint64_t qd = tc::umma_desc(base + C::Q_AT), kd = tc::umma_desc(base + C::K_AT), vd = at::umma_desc_mn(base + C::V_AT, (uint32_t)(kRows * 128), 1024u);
         auto issue_s = [&](int t, int j) {                       // into the buffer of the page's parity
@@ -418,6 +434,184 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
     if (warp == 12) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+template <int D>
+struct WeightsCfg {
+    static constexpr int G = D / 64, KEYS = 128, ROWS = 128, K_PART = Tile<D>::V_CODES;       // keys of a block, packed rows of a step; codes and parameters of a page's keys
+    static constexpr int K_BYTES = KEYS * 128 * G, Q_BYTES = ROWS * 128 * G;                 // K: of its high and of its low half
+    static constexpr int K_AT = 0, Q_AT = 2 * K_BYTES, PAR_AT = Q_AT + 2 * Q_BYTES, RAW_AT = PAR_AT + 2 * ROWS * 16, BARS = RAW_AT + 2 * K_PART;
+    static constexpr size_t SMEM = BARS + 96 + 1024;
+};
+constexpr int kWeightThreads = 9 * 32;
+
+// Summed weights where scores were not kept: S^T = K Q^T once more, 128 keys against 128 packed rows at a time, keys as a pair high + low of
+// fp16 so that scores have 32-bit accuracy.  A key is a lane of tensor memory and a thread of warps 0-3, which adds up its weights
+// 2^(s - m) / l over the rows in order: no atomics, no shuffles.  Warps 4-7 bring the rows' operands and (unit, m, 1 / l), warp 8 issues the products.
+// grid (blocks of 128 cached rows, kv heads, batch).  Bound: exponentials and tensor pipe alike (128 x 128 of them in 1024 cycles, two products of K = D).
+template <typename T, int D>
+__global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const Cache c, const AttnParams p) {
+    using C = WeightsCfg<D>;
+    using L = Tile<D>;
+    constexpr int G = C::G;
+    extern __shared__ unsigned char weights_smem[];
+    const uint32_t raw_base = tc::smem_u32(weights_smem), base = (raw_base + 1023u) & ~1023u;
+    unsigned char* sm = weights_smem + (base - raw_base);
+    const uint32_t bars = base + C::BARS, raw_full = bars, q_full = bars + 8, q_empty = bars + 24, s_full = bars + 40, s_empty = bars + 56, drain = bars + 72;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::BARS + 80);
+    volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int tid = threadIdx.x, warp = tid >> 5, h = blockIdx.y, b = blockIdx.z, group = c.q_heads / c.kv_heads, key0 = blockIdx.x * C::KEYS;
+
+    // lengths, pages and keys are nobody's to write since before the first kernel of this call
+    const Entry e = entry_of(c, p, b);
+    if (key0 >= e.len) { pdl_wait(); return; }
+    int page[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) page[i] = key0 + i * kRows < e.len ? page_of(c, b, key0 / kRows + i) : -1;
+    if (tid == 0) {
+        tc::mbar_init(raw_full, 1);
+        tc::mbar_init(drain, 1);
+        for (int i = 0; i < 2; ++i) { tc::mbar_init(q_full + 8 * i, 128); tc::mbar_init(q_empty + 8 * i, 1); tc::mbar_init(s_full + 8 * i, 1); tc::mbar_init(s_empty + 8 * i, 128); }
+        *abort_s = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        const int there = (page[0] >= 0) + (page[1] >= 0);
+        if (there > 0) tc::mbar_expect_tx(raw_full, there * C::K_PART); else mbar_arrive(raw_full);
+        for (int i = 0; i < 2; ++i)
+            if (page[i] >= 0) bulk_copy(base + C::RAW_AT + i * C::K_PART, tile_of<D>(c, page[i], h), C::K_PART, raw_full);
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(tmem_slot)), "r"(256) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    __syncthreads();
+    if (!tc::mbar_wait(raw_full, 0, abort_s)) *abort_s = 1;
+    if (warp < 8 && *abort_s == 0) {
+#pragma unroll
+        for (int it = 0; it < 2; ++it) {
+            const int r = it * 64 + (tid >> 2), x = tid & 3, pr = r % kRows;     // row of the block, of its page; quarter of its groups
+            const uint8_t* raw = sm + C::RAW_AT + it * C::K_PART;
+            const bool have = page[it] >= 0 && key0 + r < e.len;
+            uint32_t w[G][2];
+            quarter_words<D, false>(reinterpret_cast<const uint32_t*>(raw + L::K_CODES), pr, x, w);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const __half2 par = have ? reinterpret_cast<const __half2*>(raw + L::K_PARAMS)[pr * G + g] : __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint4* dst = reinterpret_cast<uint4*>(sm + C::K_AT + g * (C::KEYS * 128) + r * 128 + (((2 * x + i) ^ (r & 7)) << 4));
+                    uint4 high, low;
+                    half_pairs(w[g][i], par, high, low);
+                    dst[0] = high;
+                    dst[C::K_BYTES / 16] = low;
+                }
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    pdl_launch_dependents();                                     // not before this block has its tensor memory
+    pdl_wait();
+
+    const int rows = e.n * group, first_row = max(0, key0 - (e.len - e.n)) * group / C::ROWS * C::ROWS;       // rows before do not see the block
+    const int n = rows > first_row ? (rows - first_row + C::ROWS - 1) / C::ROWS : 0;
+    auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_s)); };
+    if (warp < 4) {
+        const int key = key0 + tid;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        int i = 0;
+        for (; i < n; ++i) {
+            const int st = i & 1, r0 = first_row + i * C::ROWS;
+            if (!wait(s_full + 8 * st, (uint32_t)(i >> 1) & 1u)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const float4* par = reinterpret_cast<const float4*>(sm + C::PAR_AT) + st * C::ROWS;
+            const bool interior = e.len - e.n + r0 / group >= key0 + C::KEYS - 1;          // the step's first row sees every key
+#pragma unroll 1
+            for (int q = 0; q < C::ROWS; q += 32) {
+                uint32_t s[32];
+                tc::tmem_ld32(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(st * C::ROWS + q), s);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) {
+                    const float4 v = par[q + k];
+                    const float w = at::ex2(fmaf(__uint_as_float(s[k]), v.x, v.y));
+                    if (interior || key < __float_as_int(v.w)) sum[k & 3] = fmaf(w, v.z, sum[k & 3]);
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            mbar_arrive(s_empty + 8 * st);
+        }
+        if (i < n) *abort_s = 1;
+        const int pg = page[tid >> 6];
+        if (i == n && key < e.len && pg >= 0) {
+            const size_t at = row_slot(c, pg, h, key % kRows);
+            p.mass_out[at] = p.mass_in[at] + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        }
+    } else if (warp < 8) {
+        const int tr = tid - 128;
+        int i = 0;
+        for (; i < n; ++i) {
+            const int st = i & 1, row = first_row + i * C::ROWS + tr;
+            // the products and the sums of two steps before have read this place
+            if (i >= 2 && !(wait(q_empty + 8 * st, (uint32_t)(i / 2 - 1) & 1u) && wait(s_empty + 8 * st, (uint32_t)(i / 2 - 1) & 1u))) break;
+            const bool have = row < rows;
+            const int qr = have ? row / group : 0, head = h * group + (have ? row % group : 0);
+            const float unit = query_row<T, D>((const T*)p.q + ((size_t)(e.row0 + qr) * c.q_heads + head) * D, have, sm + C::Q_AT + st * C::Q_BYTES, tr, p.scale_log2);
+            float4 v = make_float4(0.f, -INFINITY, 0.f, __int_as_float(0));
+            if (have) {
+                const float2 s = p.stats[stat_row(c, p, b, qr, head)];
+                if (s.x != -INFINITY) v = make_float4(unit, -s.x, 1.0f / s.y, __int_as_float(min(e.len, e.len - e.n + qr + 1)));
+            }
+            reinterpret_cast<float4*>(sm + C::PAR_AT)[st * C::ROWS + tr] = v;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(q_full + 8 * st);
+        }
+        if (i < n) *abort_s = 1;
+    } else {
+        constexpr uint32_t kDesc = at::instr_desc_f16(C::KEYS, C::ROWS);
+        const uint32_t lead = elect_one(), tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint64_t kd = tc::umma_desc(base + C::K_AT), qd = tc::umma_desc(base + C::Q_AT);
+        bool ok = true;
+        for (int i = 0; i < n && ok; ++i) {
+            const int st = i & 1;
+            ok = (i < 2 || wait(s_empty + 8 * st, (uint32_t)(i / 2 - 1) & 1u)) && wait(q_full + 8 * st, (uint32_t)(i >> 1) & 1u);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (lead) {
+                const uint64_t qt = qd + (uint64_t)(st * (C::Q_BYTES >> 4));
+#pragma unroll
+                for (int k = 0; k < 2 * (D / 16); ++k) {
+                    const int kk = k % (D / 16), low = k / (D / 16);
+                    at::umma_d(tm + (uint32_t)(st * C::ROWS), kd + (uint64_t)((low * C::K_BYTES + (kk >> 2) * (C::KEYS * 128)) / 16 + (kk & 3) * 2), qt + (uint64_t)((kk >> 2) * (C::ROWS * 128 >> 4) + (kk & 3) * 2),
+                               kDesc, k != 0 ? 1u : 0u);
+                }
+                tc::umma_commit(s_full + 8 * st);
+                tc::umma_commit(q_empty + 8 * st);
+            }
+            __syncwarp();
+        }
+        if (!ok) {                                               // given up: the products issued end before the block leaves (bounded)
+            *abort_s = 1;
+            volatile int go_on = 0;
+            if (lead) tc::umma_commit(drain);
+            __syncwarp();
+            (void)tc::mbar_wait(drain, 0, &go_on);
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (*abort_s != 0 && tid == 0) {                             // and the copies land
+        volatile int go_on = 0;
+        (void)tc::mbar_wait(raw_full, 0, &go_on);
+        raise(c, kWait);
+    }
+    __syncthreads();
+    if (warp == 8) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256) : "memory");
     }
 }
 
