@@ -48,6 +48,28 @@ __device__ __forceinline__ size_t stat_row(const Cache& c, const AttnParams& p, 
 
 constexpr int kWarps = 4;
 
+// Wait of a whole warp for a phase, bounded; false when it gave up.
+constexpr int kSpins = 1 << 25;
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    for (int i = 0; i < kSpins; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+            "selp.u32 %0, 1, 0, p;\n"
+            "}\n"
+            : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (__all_sync(0xffffffffu, ok)) return true;
+        if ((i & 0xff) == 0xff && __any_sync(0xffffffffu, *abort_flag != 0)) return false;      // another role already gave up
+    }
+    return false;
+}
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
 // How attend_few's work is dealt: the pages of every (sequence, kv head, tile of R packed rows) in units of p.unit, in that order; block w
 // has the units [w step, (w + 1) step).  Lengths are known on the device only, so every block adds them up for itself.
 struct Deal { int before, all; };          // units ahead of sequence b, and altogether
@@ -358,7 +380,7 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
 
         for (int i = 0; i < mine; ++i) {
             const int st = (slot + i) % C::STAGES, first = (p0 + warp + kWarps * i) * kRows;
-            if (!__all_sync(0xffffffffu, tc::mbar_wait(bar0 + 8 * st, (uint32_t)((slot + i) / C::STAGES) & 1u, abort_s))) { *abort_s = 1; break; }
+            if (!warp_wait(bar0 + 8 * st, (uint32_t)((slot + i) / C::STAGES) & 1u, abort_s)) { *abort_s = 1; break; }
             if (there >> st & 1u) {
                 uint8_t* page = ring + (size_t)st * L::BYTES;
                 if (e.len - first < kRows) clear_rows<D>(page, e.len - first, true);

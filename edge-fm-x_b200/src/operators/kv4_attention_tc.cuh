@@ -1,14 +1,15 @@
 // Many query rows against a 4-bit cache on the 5th-generation tensor cores.
 //
 // Block = 256 packed rows (new rows x heads of a group) of one sequence and kv head, as two tiles of 128 that share the keys and values;
-// 13 warps:
+// 14 warps:
 //   warps 0-3, 4-7   softmax of a tile, a thread per row: S from tensor memory, p = 2^(s - m), P back into tensor memory as fp16, where the
 //                    product takes it as its A operand.  O stays in tensor memory; it is scaled only when a row's maximum has grown by
 //                    more than 2^8 since it was last, which a row's first pages see and later ones hardly;
 //   warps 8-11       pages by bulk copies (a ring of three), codes to fp16 values (min + scale * code, rounded once), written in the
 //                    operands' 128-byte-swizzled layout: K-major rows of K, and the same rows of V read MN-major;
-//   warp 12          one lane issues the products: S = Q K^T (M 128, N 64, K = head size), O += P V (M 128, N = head size, K 64).  S has two
-//                    buffers a tile and runs two pages ahead of P V; weights take the place of the scores they came from.
+//   warps 12, 13     one lane of each issues a tile's products: S = Q K^T (M 128, N 64, K = head size), O += P V (M 128, N = head size, K 64).  S has two
+//                    buffers a tile and runs two pages ahead of P V; weights take the place of the scores they came from.  A wait costs
+//                    that warp some 250 cycles even when it is over; one warp for both tiles left the tensor pipe idle half the time.
 // q is scaled by a power of two per row to be exact in fp16.  k, v and p are rounded to fp16 (2^-11), well below the half step of a bf16
 // output (2^-8).  Where that would show (X: fp16 outputs, and row sums that weights are divided by) each is a pair high + low instead:
 // S = Q (Kh + Kl), O += Ph Vh + Pl Vh + Ph Vl.
@@ -25,17 +26,17 @@
 namespace efm {
 namespace kv4 {
 
-constexpr int kTileRows = 128, kManyThreads = 13 * 32;
+constexpr int kTileRows = 128, kManyThreads = 14 * 32;
 
 template <int D, bool X>
 struct ManyCfg {
     static constexpr int G = D / 64;
-    static constexpr int KS = X ? 2 : 3, VS = 2, LEAD = KS - 1, RAW = LEAD + 2;          // K is converted LEAD pages ahead of V; pages in the ring of raw ones
+    static constexpr int KS = X ? 2 : 3, VS = X ? 2 : 3, LEAD = KS - 1, RAW = LEAD + 2;          // K is converted LEAD pages ahead of V; pages in the ring of raw ones
     static constexpr int Q_BYTES = kTileRows * 128 * G, LOW = kRows * 128 * G;           // of one tile; of K or V of a page, and where its low half begins
     static constexpr int KV_BYTES = X ? 2 * LOW : LOW;
     static constexpr int Q_AT = 0, K_AT = 2 * Q_BYTES, V_AT = K_AT + KS * KV_BYTES, RAW_AT = V_AT + VS * KV_BYTES, BARS = RAW_AT + RAW * Tile<D>::BYTES;
     static constexpr int S_COL = 0, O_COL = 256;                                         // S of (tile, page parity): 64 columns each, P in its place; O: 128 a tile
-    static constexpr size_t SMEM = BARS + 304 + 1024;
+    static constexpr size_t SMEM = BARS + 320 + 1024;
 };
 
 // Pairs of fp16 codes of a word, in the order of the channels: as in low_pair / high_pair, without the 8.
@@ -155,9 +156,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
     const uint32_t raw_base = tc::smem_u32(many_smem), base = (raw_base + 1023u) & ~1023u;
     unsigned char* sm = many_smem + (base - raw_base);
     const uint32_t bars = base + C::BARS;
-    const uint32_t q_full = bars, raw_full = bars + 8, raw_empty = bars + 40, k_full = bars + 72, k_empty = bars + 96, v_full = bars + 120, v_empty = bars + 136,
-                   s_full = bars + 152, p_full = bars + 184, o_done = bars + 216, drain = bars + 248;     // s_full, p_full, o_done: [tile][page parity]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::BARS + 256);
+    const uint32_t q_full = bars, raw_full = bars + 8, raw_empty = bars + 40, k_full = bars + 72, k_empty = bars + 96, v_full = bars + 120, v_empty = bars + 144,
+                   s_full = bars + 168, p_full = bars + 200, o_done = bars + 232, drain = bars + 264;     // s_full, p_full, o_done: [tile][page parity]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::BARS + 280);
     volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* there = reinterpret_cast<volatile int*>(tmem_slot + 2);        // [8] page j % 8 is one of the pool's
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y, b = blockIdx.z, group = c.q_heads / c.kv_heads;
@@ -170,12 +171,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
     const int last = min(rows, r0 + 2 * kTileRows) - 1;
     const int n = (max(0, min(e.len, e.len - e.n + last / group + 1)) + kRows - 1) / kRows;      // pages that any of the rows sees
     if (tid == 0) {
-        tc::mbar_init(q_full, 128 * nt);
+        tc::mbar_init(q_full, 4 * nt);
         for (int i = 0; i < C::RAW; ++i) { tc::mbar_init(raw_full + 8 * i, 1); tc::mbar_init(raw_empty + 8 * i, 4); }
-        tc::mbar_init(drain, 1);
-        for (int i = 0; i < C::KS; ++i) { tc::mbar_init(k_full + 8 * i, 4); tc::mbar_init(k_empty + 8 * i, 1); }
-        for (int i = 0; i < C::VS; ++i) { tc::mbar_init(v_full + 8 * i, 4); tc::mbar_init(v_empty + 8 * i, 1); }
-        for (int i = 0; i < 4; ++i) { tc::mbar_init(s_full + 8 * i, 1); tc::mbar_init(p_full + 8 * i, 128); tc::mbar_init(o_done + 8 * i, 1); }
+        for (int i = 0; i < 2; ++i) tc::mbar_init(drain + 8 * i, 1);
+        for (int i = 0; i < C::KS; ++i) { tc::mbar_init(k_full + 8 * i, 4); tc::mbar_init(k_empty + 8 * i, nt); }
+        for (int i = 0; i < C::VS; ++i) { tc::mbar_init(v_full + 8 * i, 4); tc::mbar_init(v_empty + 8 * i, nt); }
+        for (int i = 0; i < 4; ++i) { tc::mbar_init(s_full + 8 * i, 1); tc::mbar_init(p_full + 8 * i, 4); tc::mbar_init(o_done + 8 * i, 1); }
         *abort_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -201,7 +202,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
             const float unit = query_row<T, D>(q, have, sm + C::Q_AT + t * C::Q_BYTES, tr, p.scale_log2);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(q_full);
+            warp_arrive(q_full);
 
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t o_at = tmem + lanes + (uint32_t)(C::O_COL + t * 128);
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             for (; j < n; ++j) {
                 const int buf = t * 2 + (j & 1);
                 const uint32_t s_at = tmem + lanes + (uint32_t)(C::S_COL + buf * 64);
-                if (!__all_sync(0xffffffffu, tc::mbar_wait(s_full + 8 * buf, (uint32_t)(j >> 1) & 1u, abort_s))) { *abort_s = 1; break; }
+                if (!warp_wait(s_full + 8 * buf, (uint32_t)(j >> 1) & 1u, abort_s)) { *abort_s = 1; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 float s[64];
                 tmem_ld64(s_at, s);
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
                 }
                 l += sum[0] + sum[1];
                 if (j > 0 && __any_sync(0xffffffffu, grow)) {    // O once P V of the page before is through
-                    if (!__all_sync(0xffffffffu, tc::mbar_wait(o_done + 8 * (buf ^ 1), (uint32_t)((j - 1) >> 1) & 1u, abort_s))) { *abort_s = 1; break; }
+                    if (!warp_wait(o_done + 8 * (buf ^ 1), (uint32_t)((j - 1) >> 1) & 1u, abort_s)) { *abort_s = 1; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
                     for (int d = 0; d < D; d += 32) {
@@ -257,9 +258,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
                 if constexpr (X) tmem_st32(s_at + 32, pl);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                mbar_arrive(p_full + 8 * buf);
+                warp_arrive(p_full + 8 * buf);
             }
-            const bool done = j == n && (n == 0 || __all_sync(0xffffffffu, tc::mbar_wait(o_done + 8 * (t * 2 + ((n - 1) & 1)), (uint32_t)((n - 1) >> 1) & 1u, abort_s)));
+            const bool done = j == n && (n == 0 || warp_wait(o_done + 8 * (t * 2 + ((n - 1) & 1)), (uint32_t)((n - 1) >> 1) & 1u, abort_s));
             if (!done) *abort_s = 1;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (done) {
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
                 }
             }
         };
-        auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_s)); };
+        auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait(bar, parity, abort_s); };
         auto convert = [&](auto values, int j, uint32_t full) {  // K or V of page j, by all four warps
             constexpr bool V = decltype(values)::value;
             const uint8_t* page = sm + C::RAW_AT + (j % C::RAW) * L::BYTES;
@@ -337,8 +338,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full);
+            warp_arrive(full);
         };
         int asked = 0;
         if (dw == 0) for (; asked < min(n, C::RAW); ++asked) request(asked);
@@ -353,73 +353,69 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             if (j < 0) continue;
             if (j >= C::VS && !wait(v_empty + 8 * (j % C::VS), (uint32_t)(j / C::VS - 1) & 1u)) break;
             convert(std::true_type(), j, v_full + 8 * (j % C::VS));
-            if (lane == 0) mbar_arrive(raw_empty + 8 * (j % C::RAW));
+            warp_arrive(raw_empty + 8 * (j % C::RAW));
             if (dw == 0 && asked < n) {                          // once all four warps have read page j
                 if (!wait(raw_empty + 8 * (j % C::RAW), (uint32_t)(j / C::RAW) & 1u)) break;
                 request(asked++);
             }
         }
         if (i < n + C::LEAD) *abort_s = 1;
-    } else {
-        // The whole warp walks the loop, so that addresses and descriptors stay in uniform registers; one lane issues.  With a loop of that
-        // lane alone the issue of 24 products a page took 2500 cycles, more than everything else.
+    } else if (warp - 12 < nt) {
+        // The whole warp walks the loop, so that addresses and descriptors stay in uniform registers; one lane issues.
         constexpr uint32_t kDescS = at::instr_desc_f16(kTileRows, kRows), kDescO = at::instr_desc_f16(kTileRows, D) | (1u << 16);
+        const int t = warp - 12;
         const uint32_t lead = elect_one();
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-        const uint64_t qd = tc::umma_desc(base + C::Q_AT), kd = tc::umma_desc(base + C::K_AT), vd = at::umma_desc_mn(base + C::V_AT, (uint32_t)(kRows * 128), 1024u);
-        auto issue_s = [&](int t, int j) {                       // into the buffer of the page's parity
+        const uint64_t qt = tc::umma_desc(base + C::Q_AT + t * C::Q_BYTES), kd = tc::umma_desc(base + C::K_AT), vd = at::umma_desc_mn(base + C::V_AT, (uint32_t)(kRows * 128), 1024u);
+        const uint32_t s0 = tm + (uint32_t)(C::S_COL + t * 128), to = tm + (uint32_t)(C::O_COL + t * 128);
+        auto issue_s = [&](int j) {                              // into the buffer of the page's parity
             if (lead) {
-                const int st = j % C::KS, buf = t * 2 + (j & 1);
-                const uint64_t qt = qd + (uint64_t)(t * (C::Q_BYTES >> 4)), kt = kd + (uint64_t)(st * (C::KV_BYTES >> 4));
-                const uint32_t to = tm + (uint32_t)(C::S_COL + buf * 64);
+                const uint64_t kt = kd + (uint64_t)(j % C::KS * (C::KV_BYTES >> 4));
+                const uint32_t s_to = s0 + (uint32_t)((j & 1) * 64);
 #pragma unroll
                 for (int i = 0; i < (X ? 2 : 1) * (D / 16); ++i) {
                     const int k = i % (D / 16), low = i / (D / 16);
-                    at::umma_d(to, qt + (uint64_t)((k >> 2) * (kTileRows * 128 >> 4) + (k & 3) * 2), kt + (uint64_t)((low * C::LOW + (k >> 2) * (kRows * 128)) / 16 + (k & 3) * 2), kDescS, i != 0 ? 1u : 0u);
+                    at::umma_d(s_to, qt + (uint64_t)((k >> 2) * (kTileRows * 128 >> 4) + (k & 3) * 2), kt + (uint64_t)((low * C::LOW + (k >> 2) * (kRows * 128)) / 16 + (k & 3) * 2), kDescS, i != 0 ? 1u : 0u);
                 }
-                tc::umma_commit(s_full + 8 * buf);
-                if (t == nt - 1) tc::umma_commit(k_empty + 8 * st);
+                tc::umma_commit(s_full + 8 * (t * 2 + (j & 1)));
+                tc::umma_commit(k_empty + 8 * (j % C::KS));
             }
             __syncwarp();
         };
-        auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_s)); };
+        auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait(bar, parity, abort_s); };
         bool ok = n > 0 && wait(q_full, 0);
         for (int j = 0; j < min(n, 2) && ok; ++j) {
             ok = wait(k_full + 8 * j, 0);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            for (int t = 0; t < nt; ++t) issue_s(t, j);
+            issue_s(j);
         }
         for (int j = 0; j < n && ok; ++j) {
-            const int st = j & 1;
-            const uint32_t ph = (uint32_t)(j >> 1) & 1u;
             // what the products need besides the weights first: it is there long before them
-            ok = wait(v_full + 8 * st, ph) && (j + 2 >= n || wait(k_full + 8 * ((j + 2) % C::KS), (uint32_t)((j + 2) / C::KS) & 1u));
-            for (int t = 0; t < nt && ok; ++t) {
-                ok = wait(p_full + 8 * (t * 2 + st), ph);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (lead) {
-                    const uint64_t vt = vd + (uint64_t)(st * (C::KV_BYTES >> 4));
-                    const uint32_t to = tm + (uint32_t)(C::O_COL + t * 128), from = tm + (uint32_t)(C::S_COL + (t * 2 + st) * 64);
+            ok = wait(v_full + 8 * (j % C::VS), (uint32_t)(j / C::VS) & 1u) && (j + 2 >= n || wait(k_full + 8 * ((j + 2) % C::KS), (uint32_t)((j + 2) / C::KS) & 1u)) &&
+                 wait(p_full + 8 * (t * 2 + (j & 1)), (uint32_t)(j >> 1) & 1u);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (lead) {
+                const uint64_t vt = vd + (uint64_t)(j % C::VS * (C::KV_BYTES >> 4));
+                const uint32_t from = s0 + (uint32_t)((j & 1) * 64);
 #pragma unroll
-                    for (int i = 0; i < (X ? 3 : 1) * (kRows / 16); ++i) {
-                        const int k = i % (kRows / 16), part = i / (kRows / 16);                   // Ph Vh, Pl Vh, Ph Vl
-                        at::umma_ts(to, from + (uint32_t)((part == 1 ? 32 : 0) + 8 * k), vt + (uint64_t)((part == 2 ? C::LOW : 0) / 16 + k * (2048 >> 4)), kDescO, i != 0 || j > 0 ? 1u : 0u);
-                    }
-                    tc::umma_commit(o_done + 8 * (t * 2 + st));
-                    if (t == nt - 1) tc::umma_commit(v_empty + 8 * st);
+                for (int i = 0; i < (X ? 3 : 1) * (kRows / 16); ++i) {
+                    const int k = i % (kRows / 16), part = i / (kRows / 16);                       // Ph Vh, Pl Vh, Ph Vl
+                    at::umma_ts(to, from + (uint32_t)((part == 1 ? 32 : 0) + 8 * k), vt + (uint64_t)((part == 2 ? C::LOW : 0) / 16 + k * (2048 >> 4)), kDescO, i != 0 || j > 0 ? 1u : 0u);
                 }
-                __syncwarp();
-                if (j + 2 < n) issue_s(t, j + 2);                // behind P V, which reads the weights in that place
+                tc::umma_commit(o_done + 8 * (t * 2 + (j & 1)));
+                tc::umma_commit(v_empty + 8 * (j % C::VS));
             }
+            __syncwarp();
+            if (j + 2 < n) issue_s(j + 2);                       // behind P V, which reads the weights in that place
         }
         if (n > 0 && !ok) {                                      // given up: the products issued end before the block leaves (bounded)
             *abort_s = 1;
             volatile int go_on = 0;
-            if (lead) tc::umma_commit(drain);
+            if (lead) tc::umma_commit(drain + 8 * t);
             __syncwarp();
-            (void)tc::mbar_wait(drain, 0, &go_on);
+            (void)tc::mbar_wait(drain + 8 * t, 0, &go_on);
         }
     }
     __syncwarp();
@@ -472,7 +468,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
     if (tid == 0) {
         tc::mbar_init(raw_full, 1);
         tc::mbar_init(drain, 1);
-        for (int i = 0; i < 2; ++i) { tc::mbar_init(q_full + 8 * i, 128); tc::mbar_init(q_empty + 8 * i, 1); tc::mbar_init(s_full + 8 * i, 1); tc::mbar_init(s_empty + 8 * i, 128); }
+        for (int i = 0; i < 2; ++i) { tc::mbar_init(q_full + 8 * i, 4); tc::mbar_init(q_empty + 8 * i, 1); tc::mbar_init(s_full + 8 * i, 1); tc::mbar_init(s_empty + 8 * i, 4); }
         *abort_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         const int there = (page[0] >= 0) + (page[1] >= 0);
@@ -485,7 +481,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     __syncthreads();
-    if (!tc::mbar_wait(raw_full, 0, abort_s)) *abort_s = 1;
+    if (!warp_wait(raw_full, 0, abort_s)) *abort_s = 1;
     if (warp < 8 && *abort_s == 0) {
 #pragma unroll
         for (int it = 0; it < 2; ++it) {
@@ -518,7 +514,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
 
     const int rows = e.n * group, first_row = max(0, key0 - (e.len - e.n)) * group / C::ROWS * C::ROWS;       // rows before do not see the block
     const int n = rows > first_row ? (rows - first_row + C::ROWS - 1) / C::ROWS : 0;
-    auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_s)); };
+    auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait(bar, parity, abort_s); };
     if (warp < 4) {
         const int key = key0 + tid;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -541,7 +537,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            mbar_arrive(s_empty + 8 * st);
+            warp_arrive(s_empty + 8 * st);
         }
         if (i < n) *abort_s = 1;
         const int pg = page[tid >> 6];
@@ -566,7 +562,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
             }
             reinterpret_cast<float4*>(sm + C::PAR_AT)[st * C::ROWS + tr] = v;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(q_full + 8 * st);
+            warp_arrive(q_full + 8 * st);
         }
         if (i < n) *abort_s = 1;
     } else {
