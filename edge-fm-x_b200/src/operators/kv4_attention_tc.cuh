@@ -1,11 +1,12 @@
 // Many query rows against a 4-bit cache on the 5th-generation tensor cores.
 //
 // Block = 256 packed rows (new rows x heads of a group) of one sequence and kv head, as two tiles of 128 that share the keys and values;
-// 14 warps:
+// 15 warps:
 //   warps 0-3, 4-7   softmax of a tile, a thread per row: S from tensor memory, p = 2^(s - m), P back into tensor memory as fp16, where the
 //                    product takes it as its A operand.  O stays in tensor memory; it is scaled only when a row's maximum has grown by
 //                    more than 2^8 since it was last, which a row's first pages see and later ones hardly;
-//   warps 8-11       pages by bulk copies (a ring of three), codes to fp16 values (min + scale * code, rounded once), written in the
+//   warp 14          asks for pages, a bulk copy each into a ring;
+//   warps 8-11       codes to fp16 values (min + scale * code, rounded once), written in the
 //                    operands' 128-byte-swizzled layout: K-major rows of K, and the same rows of V read MN-major;
 //   warps 12, 13     one lane of each issues a tile's products: S = Q K^T (M 128, N 64, K = head size), O += P V (M 128, N = head size, K 64).  S has two
 //                    buffers a tile and runs two pages ahead of P V; weights take the place of the scores they came from.  A wait costs
@@ -26,7 +27,7 @@
 namespace efm {
 namespace kv4 {
 
-constexpr int kTileRows = 128, kManyThreads = 14 * 32;
+constexpr int kTileRows = 128, kManyThreads = 15 * 32;
 
 template <int D, bool X>
 struct ManyCfg {
@@ -286,26 +287,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             }
         }
     } else if (warp < 12) {
-        const int dw = warp - 8, dt = tid - 8 * 32;
-        int lane_page = -1;
-        auto request = [&](int j) {                              // by warp 8
-            if ((j & 31) == 0) {
-                const bool in = j + lane < n;
-                lane_page = in ? c.page_table[(size_t)b * c.max_pages + j + lane] : -1;
-                if ((unsigned)lane_page >= (unsigned)c.n_pages) { if (in) raise(c, kBadPage); lane_page = -1; }
-            }
-            const int page = __shfl_sync(0xffffffffu, lane_page, j & 31);
-            const uint32_t bar = raw_full + 8 * (j % C::RAW);
-            if (lane == 0) {
-                there[j & 7] = page >= 0;
-                if (page >= 0) {
-                    tc::mbar_expect_tx(bar, L::BYTES);
-                    bulk_copy(base + C::RAW_AT + (j % C::RAW) * L::BYTES, tile_of<D>(c, page, h), L::BYTES, bar);
-                } else {
-                    mbar_arrive(bar);
-                }
-            }
-        };
+        const int dt = tid - 8 * 32;
         auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait(bar, parity, abort_s); };
         auto convert = [&](auto values, int j, uint32_t full) {  // K or V of page j, by all four warps
             constexpr bool V = decltype(values)::value;
@@ -340,8 +322,6 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             warp_arrive(full);
         };
-        int asked = 0;
-        if (dw == 0) for (; asked < min(n, C::RAW); ++asked) request(asked);
         int i = 0;
         for (; i < n + C::LEAD; ++i) {
             if (i < n) {
@@ -354,12 +334,30 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             if (j >= C::VS && !wait(v_empty + 8 * (j % C::VS), (uint32_t)(j / C::VS - 1) & 1u)) break;
             convert(std::true_type(), j, v_full + 8 * (j % C::VS));
             warp_arrive(raw_empty + 8 * (j % C::RAW));
-            if (dw == 0 && asked < n) {                          // once all four warps have read page j
-                if (!wait(raw_empty + 8 * (j % C::RAW), (uint32_t)(j / C::RAW) & 1u)) break;
-                request(asked++);
-            }
         }
         if (i < n + C::LEAD) *abort_s = 1;
+    } else if (warp == 14) {
+        int lane_page = -1;
+        for (int j = 0; j < n; ++j) {
+            if ((j & 31) == 0) {                                 // a lane knows one page of 32
+                const bool in = j + lane < n;
+                lane_page = in ? c.page_table[(size_t)b * c.max_pages + j + lane] : -1;
+                if ((unsigned)lane_page >= (unsigned)c.n_pages) { if (in) raise(c, kBadPage); lane_page = -1; }
+            }
+            const int page = __shfl_sync(0xffffffffu, lane_page, j & 31);
+            const uint32_t bar = raw_full + 8 * (j % C::RAW);
+            if (j >= C::RAW && !warp_wait(raw_empty + 8 * (j % C::RAW), (uint32_t)(j / C::RAW - 1) & 1u, abort_s)) { *abort_s = 1; break; }
+            if (lane == 0) {
+                there[j & 7] = page >= 0;
+                if (page >= 0) {
+                    tc::mbar_expect_tx(bar, L::BYTES);
+                    bulk_copy(base + C::RAW_AT + (j % C::RAW) * L::BYTES, tile_of<D>(c, page, h), L::BYTES, bar);
+                } else {
+                    mbar_arrive(bar);
+                }
+            }
+            __syncwarp();
+        }
     } else if (warp - 12 < nt) {
         // The whole warp walks the loop, so that addresses and descriptors stay in uniform registers; one lane issues.
         constexpr uint32_t kDescS = at::instr_desc_f16(kTileRows, kRows), kDescO = at::instr_desc_f16(kTileRows, D) | (1u << 16);
