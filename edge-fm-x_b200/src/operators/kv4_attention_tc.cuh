@@ -108,30 +108,39 @@ __device__ __forceinline__ uint32_t elect_one() {
     asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(lead));
     return lead;
 }
-// A query row into row r of a K-major operand of 128 rows, as fp16 scaled by a power of two; returns what a score is to be multiplied with.
+// 32 query rows into rows r0 .. r0 + 31 of a K-major operand of 128 rows, as fp16 scaled by a power of two, by a warp: neighbouring lanes
+// have neighbouring channels (a thread per row took 6000 cycles over its strided loads).  mine: where the row of this lane begins, -1:
+// no such row.  Returns what this lane's row's scores are to be multiplied with.
 template <typename T, int D>
-__device__ __forceinline__ float query_row(const T* q, bool have, unsigned char* to, int r, float scale_log2) {
-    float top = 0.f;
+__device__ __forceinline__ float query_rows(const T* q, long long mine, unsigned char* to, int r0, float scale_log2) {
+    constexpr int LANES = D / 8, PER = 32 / LANES;               // lanes of a row, rows at a time
+    const int lane = threadIdx.x & 31, i = lane % LANES;
+    uint4 w[LANES];
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (have) w = *reinterpret_cast<const uint4*>(q + 8 * i);
-        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) { const float2 x = Num<T>::two(v[k]); top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y))); }
+    for (int it = 0; it < LANES; ++it) {
+        const long long at = __shfl_sync(0xffffffffu, mine, it * PER + lane / LANES);
+        w[it] = at >= 0 ? *reinterpret_cast<const uint4*>(q + at + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
     }
-    const int bits = (int)(__float_as_uint(top) >> 23), ex = bits == 255 ? 3 : max(bits - 127, -100);
-    const float up = __uint_as_float((uint32_t)(130 - ex) << 23);
+    float unit = 0.f;
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (have) w = *reinterpret_cast<const uint4*>(q + 8 * i);
-        uint32_t v[4] = {w.x, w.y, w.z, w.w};
+    for (int it = 0; it < LANES; ++it) {
+        uint32_t v[4] = {w[it].x, w[it].y, w[it].z, w[it].w};
+        float2 x[4];
+        float top = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) { const float2 x = Num<T>::two(v[k]); v[k] = half_pair(x.x * up, x.y * up); }
+        for (int k = 0; k < 4; ++k) { x[k] = Num<T>::two(v[k]); top = fmaxf(top, fmaxf(fabsf(x[k].x), fabsf(x[k].y))); }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int bits = (int)(__float_as_uint(top) >> 23), ex = bits == 255 ? 3 : max(bits - 127, -100);
+        const float up = __uint_as_float((uint32_t)(130 - ex) << 23), down = fmaxf(__uint_as_float((uint32_t)(ex + 124) << 23) * scale_log2, 1.2e-38f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = half_pair(x[k].x * up, x[k].y * up);
+        const int r = r0 + it * PER + lane / LANES;
         *reinterpret_cast<uint4*>(to + (i >> 3) * (kTileRows * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+        const float u = __shfl_sync(0xffffffffu, down, (lane % PER) * LANES);
+        if (lane / PER == it) unit = u;
     }
-    return fmaxf(__uint_as_float((uint32_t)(ex + 124) << 23) * scale_log2, 1.2e-38f);
+    return unit;
 }
 // The two words of a key row's quarter x of each group
 template <int D, bool V>
@@ -196,12 +205,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
         if (t < nt) {
             const bool have = row < rows;
             const size_t at = ((size_t)(e.row0 + row / group) * c.q_heads + h * group + row % group) * D;
-            const T* q = (const T*)p.q + at;
             const int see = have ? max(0, min(e.len, e.len - e.n + row / group + 1)) : 0;
             int least = have ? see : INT32_MAX;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
-            const float unit = query_row<T, D>(q, have, sm + C::Q_AT + t * C::Q_BYTES, tr, p.scale_log2);
+            const float unit = query_rows<T, D>((const T*)p.q, have ? (long long)at : -1, sm + C::Q_AT + t * C::Q_BYTES, (warp & 3) * 32, p.scale_log2);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             warp_arrive(q_full);
 
@@ -435,7 +443,7 @@ template <int D>
 struct WeightsCfg {
     static constexpr int G = D / 64, KEYS = 128, ROWS = 128, K_PART = Tile<D>::V_CODES;       // keys of a block, packed rows of a step; codes and parameters of a page's keys
     static constexpr int K_BYTES = KEYS * 128 * G, Q_BYTES = ROWS * 128 * G;                 // K: of its high and of its low half
-    static constexpr int K_AT = 0, Q_AT = 2 * K_BYTES, PAR_AT = Q_AT + 2 * Q_BYTES, RAW_AT = PAR_AT + 2 * ROWS * 16, BARS = RAW_AT + 2 * K_PART;
+    static constexpr int K_AT = 0, Q_AT = 2 * K_BYTES, PAR_AT = Q_AT + 2 * Q_BYTES, RAW_AT = PAR_AT + 2 * 4 * ROWS * 4, BARS = RAW_AT + 2 * K_PART;
     static constexpr size_t SMEM = BARS + 96 + 1024;
 };
 constexpr int kWeightThreads = 9 * 32;
@@ -521,17 +529,24 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
             const int st = i & 1, r0 = first_row + i * C::ROWS;
             if (!wait(s_full + 8 * st, (uint32_t)(i >> 1) & 1u)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const float4* par = reinterpret_cast<const float4*>(sm + C::PAR_AT) + st * C::ROWS;
+            const float* par = reinterpret_cast<const float*>(sm + C::PAR_AT) + st * 4 * C::ROWS;      // [unit | -m | 1 / l | rows seen][row]
             const bool interior = e.len - e.n + r0 / group >= key0 + C::KEYS - 1;          // the step's first row sees every key
 #pragma unroll 1
-            for (int q = 0; q < C::ROWS; q += 32) {
-                uint32_t s[32];
-                tc::tmem_ld32(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(st * C::ROWS + q), s);
+            for (int q = 0; q < C::ROWS; q += 64) {
+                float s[64];
+                tmem_ld64(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(st * C::ROWS + q), s);
+                if (!interior) {
 #pragma unroll
-                for (int k = 0; k < 32; ++k) {
-                    const float4 v = par[q + k];
-                    const float w = at::ex2(fmaf(__uint_as_float(s[k]), v.x, v.y));
-                    if (interior || key < __float_as_int(v.w)) sum[k & 3] = fmaf(w, v.z, sum[k & 3]);
+                    for (int k = 0; k < 64; ++k) if (key >= reinterpret_cast<const int*>(par)[3 * C::ROWS + q + k]) s[k] = -INFINITY;
+                }
+#pragma unroll
+                for (int k = 0; k < 64; k += 4) {
+                    const float4 u = *reinterpret_cast<const float4*>(par + q + k), m = *reinterpret_cast<const float4*>(par + C::ROWS + q + k),
+                                 l = *reinterpret_cast<const float4*>(par + 2 * C::ROWS + q + k);
+                    sum[0] = fmaf(at::ex2(fmaf(s[k], u.x, m.x)), l.x, sum[0]);
+                    sum[1] = fmaf(at::ex2(fmaf(s[k + 1], u.y, m.y)), l.y, sum[1]);
+                    sum[2] = fmaf(at::ex2(fmaf(s[k + 2], u.z, m.z)), l.z, sum[2]);
+                    sum[3] = fmaf(at::ex2(fmaf(s[k + 3], u.w, m.w)), l.w, sum[3]);
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -552,13 +567,14 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
             if (i >= 2 && !(wait(q_empty + 8 * st, (uint32_t)(i / 2 - 1) & 1u) && wait(s_empty + 8 * st, (uint32_t)(i / 2 - 1) & 1u))) break;
             const bool have = row < rows;
             const int qr = have ? row / group : 0, head = h * group + (have ? row % group : 0);
-            const float unit = query_row<T, D>((const T*)p.q + ((size_t)(e.row0 + qr) * c.q_heads + head) * D, have, sm + C::Q_AT + st * C::Q_BYTES, tr, p.scale_log2);
-            float4 v = make_float4(0.f, -INFINITY, 0.f, __int_as_float(0));
-            if (have) {
-                const float2 s = p.stats[stat_row(c, p, b, qr, head)];
-                if (s.x != -INFINITY) v = make_float4(unit, -s.x, 1.0f / s.y, __int_as_float(min(e.len, e.len - e.n + qr + 1)));
-            }
-            reinterpret_cast<float4*>(sm + C::PAR_AT)[st * C::ROWS + tr] = v;
+            const float2 s = have ? p.stats[stat_row(c, p, b, qr, head)] : make_float2(-INFINITY, 0.f);
+            const float unit = query_rows<T, D>((const T*)p.q, have ? ((long long)(e.row0 + qr) * c.q_heads + head) * D : -1, sm + C::Q_AT + st * C::Q_BYTES, tr & ~31, p.scale_log2);
+            const bool sees = s.x != -INFINITY;                  // a row that sees nothing: weights of 0
+            float* par = reinterpret_cast<float*>(sm + C::PAR_AT) + st * 4 * C::ROWS + tr;
+            par[0] = unit;
+            par[C::ROWS] = sees ? -s.x : 0.f;
+            par[2 * C::ROWS] = sees ? 1.0f / s.y : 0.f;
+            reinterpret_cast<int*>(par)[3 * C::ROWS] = sees ? min(e.len, e.len - e.n + qr + 1) : 0;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             warp_arrive(q_full + 8 * st);
         }
