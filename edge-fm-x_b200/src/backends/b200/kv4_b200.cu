@@ -136,8 +136,9 @@ struct AttnPlan {
     int max_new, max_len, nt, blocks, unit, few_rows, many_tiles;      // many_tiles: blocks of 256 packed rows a sequence may have
     bool joined;                                      // pieces of a row may lie in several blocks
     bool scores;                                      // attend_few leaves its scores for the summed weights
-    int64_t units, stats, part_stats, part, score_ld, score;
-    int64_t bytes() const { return 4 * (stats + part_stats + part + score); }
+    int64_t units, stats, part_stats, part, score_ld, score, image, image_units;
+    int row_tiles;                                    // tiles of 128 packed rows a sequence may have as operands; 0: nobody asks for them
+    int64_t bytes() const { return 4 * (stats + part_stats + part + score + image + image_units); }
 };
 constexpr int kSms = 148;                              // of the GPU these kernels are built for
 constexpr int kFewRows = 32;                           // packed rows of a sequence up to which attend_few takes it
@@ -160,7 +161,10 @@ AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
     p.stats = a->mass_out != nullptr ? round_up(2 * (int64_t)c->batch * p.max_new * c->q_heads, 4) : 0;
     p.part_stats = p.joined ? 2 * 2 * (int64_t)p.blocks * R : 0;
     p.part = p.joined ? 2 * (int64_t)p.blocks * R * c->head_dim : 0;
-    p.score_ld = round_up(p.max_len, kRows);
+    p.score_ld = round_up(p.max_len, kRows);                   // every part a multiple of 16 bytes
+    p.row_tiles = p.many_tiles > 0 || (a->mass_out != nullptr && !p.scores) ? (int)((rows + kv4::kTileRows - 1) / kv4::kTileRows) : 0;
+    p.image_units = (int64_t)c->batch * c->kv_heads * p.row_tiles * kv4::kTileRows;
+    p.image = p.image_units * c->head_dim / 2;
     p.score = p.scores ? (int64_t)c->batch * c->kv_heads * R * p.score_ld : 0;
     return p;
 }
@@ -304,6 +308,9 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
         p.part = ws + plan.stats + plan.part_stats;
         p.scores = plan.scores ? p.part + plan.part : nullptr;
         p.score_ld = plan.score_ld;
+        p.row_tiles = plan.row_tiles;
+        p.images = (uint8_t*)(ws + plan.stats + plan.part_stats + plan.part + plan.score);
+        p.units = (float*)p.images + plan.image;
         Launcher L = on_stream(stream);
         by_type(cache, [&](auto t, auto d) {
             using T = decltype(t);
@@ -315,6 +322,7 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
             const dim3 join(merges + masses, cache->kv_heads, cache->batch);
             if (rows > 0 && plan.nt == 1) L.launch(kv4::attend_few_kernel<T, D, 1>, dim3(plan.blocks), block, kv4::FewCfg<D, 1>::SMEM, c, p);
             if (rows > 0 && plan.nt == 2) L.launch(kv4::attend_few_kernel<T, D, 2>, dim3(plan.blocks), block, kv4::FewCfg<D, 2>::SMEM, c, p);
+            if (plan.row_tiles > 0) L.launch(kv4::attend_query_kernel<T, D>, dim3(plan.row_tiles, cache->kv_heads, cache->batch), dim3(kv4::kTileRows), 0, c, p);
             const dim3 many(plan.many_tiles, cache->kv_heads, cache->batch);
             if (plan.many_tiles > 0) {
                 if (cache->dtype == EFM_F16 || p.mass_out != nullptr) L.launch(kv4::attend_many_kernel<T, D, true>, many, dim3(kv4::kManyThreads), kv4::ManyCfg<D, true>::SMEM, c, p);

@@ -26,6 +26,9 @@ struct AttnParams {
     int rows;                 // new rows a sequence has in stats
     float2* part_stats;       // [2 blocks][8 nt] the same of the keys a block had, and
     float* part;              // [2 blocks][8 nt][D] its weighted values: slot 0 is the piece its range begins with, slot 1 the one it ends with
+    uint8_t* images;          // [batch, kv_heads, row_tiles][128 x D fp16] packed rows as operands, and
+    float* units;             // [batch, kv_heads, row_tiles][128] what their scores are multiplied with; where many rows are a sequence's
+    int row_tiles;
     float* scores;            // [batch, kv_heads, 8 nt][score_ld] scores in units of log2; null: not wanted
     int64_t score_ld;
 };

@@ -155,6 +155,23 @@ __device__ __forceinline__ void quarter_words(const uint32_t* codes, int r, int 
     }
 }
 
+__device__ __forceinline__ size_t row_tile(const Cache& c, const AttnParams& p, int b, int h, int tile) { return ((size_t)b * c.kv_heads + h) * p.row_tiles + tile; }
+
+// Packed rows, 128 a tile, as the operands that attend_many and attend_weights copy in one piece (every block of theirs converting rows for
+// itself took 4000 cycles a tile).  grid (tiles, kv heads, batch).
+template <typename T, int D>
+__global__ void __launch_bounds__(kTileRows) attend_query_kernel(const Cache c, const AttnParams p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int h = blockIdx.y, b = blockIdx.z, group = c.q_heads / c.kv_heads, row = blockIdx.x * kTileRows + threadIdx.x;
+    const Entry e = entry_of(c, p, b);
+    const int rows = e.n * group;
+    if ((int)blockIdx.x * kTileRows >= rows) return;
+    const size_t tile = row_tile(c, p, b, h, blockIdx.x);
+    const long long at = row < rows ? ((long long)(e.row0 + row / group) * c.q_heads + h * group + row % group) * D : -1;
+    p.units[tile * kTileRows + threadIdx.x] = query_rows<T, D>((const T*)p.q, at, p.images + tile * (kTileRows * D * 2), threadIdx.x & ~31, p.scale_log2);
+}
+
 // grid (tiles of 256 packed rows, kv heads, batch); late rows see the most keys and come first
 template <typename T, int D, bool X>
 __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cache c, const AttnParams p) {
@@ -181,7 +198,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
     const int last = min(rows, r0 + 2 * kTileRows) - 1;
     const int n = (max(0, min(e.len, e.len - e.n + last / group + 1)) + kRows - 1) / kRows;      // pages that any of the rows sees
     if (tid == 0) {
-        tc::mbar_init(q_full, 4 * nt);
+        tc::mbar_init(q_full, 1);
         for (int i = 0; i < C::RAW; ++i) { tc::mbar_init(raw_full + 8 * i, 1); tc::mbar_init(raw_empty + 8 * i, 4); }
         for (int i = 0; i < 2; ++i) tc::mbar_init(drain + 8 * i, 1);
         for (int i = 0; i < C::KS; ++i) { tc::mbar_init(k_full + 8 * i, 4); tc::mbar_init(k_empty + 8 * i, nt); }
@@ -209,10 +226,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             int least = have ? see : INT32_MAX;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
-            const float unit = query_rows<T, D>((const T*)p.q, have ? (long long)at : -1, sm + C::Q_AT + t * C::Q_BYTES, (warp & 3) * 32, p.scale_log2);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            warp_arrive(q_full);
-
+            const float unit = p.units[row_tile(c, p, b, h, r0 / kTileRows + t) * kTileRows + tr];
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t o_at = tmem + lanes + (uint32_t)(C::O_COL + t * 128);
             float m = -INFINITY, l = 0.f;                        // m: what the row's weights are relative to
@@ -345,6 +359,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
         }
         if (i < n + C::LEAD) *abort_s = 1;
     } else if (warp == 14) {
+        if (lane == 0 && n > 0) {
+            tc::mbar_expect_tx(q_full, nt * C::Q_BYTES);
+            for (int t = 0; t < nt; ++t) bulk_copy(base + C::Q_AT + t * C::Q_BYTES, p.images + row_tile(c, p, b, h, r0 / kTileRows + t) * C::Q_BYTES, C::Q_BYTES, q_full);
+        }
+        __syncwarp();
         int lane_page = -1;
         for (int j = 0; j < n; ++j) {
             if ((j & 31) == 0) {                                 // a lane knows one page of 32
@@ -429,6 +448,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
     __syncthreads();
     if (*abort_s != 0 && tid == 0) {                             // and the copies land
         volatile int go_on = 0;
+        (void)tc::mbar_wait(q_full, 0, &go_on);
         for (int i = 0; i < C::RAW; ++i) { (void)tc::mbar_wait(raw_full + 8 * i, 0, &go_on); (void)tc::mbar_wait(raw_full + 8 * i, 1, &go_on); }
         raise(c, kWait);
     }
@@ -450,7 +470,7 @@ constexpr int kWeightThreads = 9 * 32;
 
 // Summed weights where scores were not kept: S^T = K Q^T once more, 128 keys against 128 packed rows at a time, keys as a pair high + low of
 // fp16 so that scores have 32-bit accuracy.  A key is a lane of tensor memory and a thread of warps 0-3, which adds up its weights
-// 2^(s - m) / l over the rows in order: no atomics, no shuffles.  Warps 4-7 bring the rows' operands and (unit, m, 1 / l), warp 8 issues the products.
+// 2^(s - m) / l over the rows in order: no atomics, no shuffles.  Warps 4-7 bring the rows' operand and (unit, m, 1 / l), warp 8 issues the products.
 // grid (blocks of 128 cached rows, kv heads, batch).  Bound: exponentials and tensor pipe alike (128 x 128 of them in 1024 cycles, two products of K = D).
 template <typename T, int D>
 __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const Cache c, const AttnParams p) {
@@ -474,7 +494,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
     if (tid == 0) {
         tc::mbar_init(raw_full, 1);
         tc::mbar_init(drain, 1);
-        for (int i = 0; i < 2; ++i) { tc::mbar_init(q_full + 8 * i, 4); tc::mbar_init(q_empty + 8 * i, 1); tc::mbar_init(s_full + 8 * i, 1); tc::mbar_init(s_empty + 8 * i, 4); }
+        for (int i = 0; i < 2; ++i) { tc::mbar_init(q_full + 8 * i, 5); tc::mbar_init(q_empty + 8 * i, 1); tc::mbar_init(s_full + 8 * i, 1); tc::mbar_init(s_empty + 8 * i, 4); }
         *abort_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         const int there = (page[0] >= 0) + (page[1] >= 0);
@@ -568,14 +588,18 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
             const bool have = row < rows;
             const int qr = have ? row / group : 0, head = h * group + (have ? row % group : 0);
             const float2 s = have ? p.stats[stat_row(c, p, b, qr, head)] : make_float2(-INFINITY, 0.f);
-            const float unit = query_rows<T, D>((const T*)p.q, have ? ((long long)(e.row0 + qr) * c.q_heads + head) * D : -1, sm + C::Q_AT + st * C::Q_BYTES, tr & ~31, p.scale_log2);
+            const size_t tile = row_tile(c, p, b, h, first_row / C::ROWS + i);
+            if (tr == 0) {                                       // the operand as it is, the rows' parameters by these four warps
+                tc::mbar_expect_tx(q_full + 8 * st, C::Q_BYTES);
+                bulk_copy(base + C::Q_AT + st * C::Q_BYTES, p.images + tile * C::Q_BYTES, C::Q_BYTES, q_full + 8 * st);
+            }
+            const float unit = p.units[tile * kTileRows + tr];
             const bool sees = s.x != -INFINITY;                  // a row that sees nothing: weights of 0
             float* par = reinterpret_cast<float*>(sm + C::PAR_AT) + st * 4 * C::ROWS + tr;
             par[0] = unit;
             par[C::ROWS] = sees ? -s.x : 0.f;
             par[2 * C::ROWS] = sees ? 1.0f / s.y : 0.f;
             reinterpret_cast<int*>(par)[3 * C::ROWS] = sees ? min(e.len, e.len - e.n + qr + 1) : 0;
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             warp_arrive(q_full + 8 * st);
         }
         if (i < n) *abort_s = 1;
@@ -616,6 +640,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
     if (*abort_s != 0 && tid == 0) {                             // and the copies land
         volatile int go_on = 0;
         (void)tc::mbar_wait(raw_full, 0, &go_on);
+        for (int i = 0; i < min(n, 2); ++i) { (void)tc::mbar_wait(q_full + 8 * i, 0, &go_on); (void)tc::mbar_wait(q_full + 8 * i, 1, &go_on); }
         raise(c, kWait);
     }
     __syncthreads();
