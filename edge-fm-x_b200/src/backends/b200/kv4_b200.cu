@@ -61,10 +61,13 @@ template <typename T, int D>
 cudaError_t more_smem() {
     cudaError_t e = cudaFuncSetAttribute(kv4::attend_few_kernel<T, D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::FewCfg<D, 1>::SMEM);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_few_kernel<T, D, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::FewCfg<D, 2>::SMEM);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_many_kernel<T, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::ManyCfg<D, true>::SMEM);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_weights_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::WeightsCfg<D>::SMEM);
-    if constexpr (std::is_same<T, __nv_bfloat16>::value)
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_many_kernel<T, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::ManyCfg<D, false>::SMEM);
+    if constexpr (std::is_same<T, __half>::value) {
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_many_kernel<T, D, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::ManyCfg<D, 2>::SMEM);
+    } else {
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_many_kernel<T, D, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::ManyCfg<D, 0>::SMEM);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_many_kernel<T, D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::ManyCfg<D, 1>::SMEM);
+    }
     return e;
 }
 
@@ -325,8 +328,10 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
             if (plan.row_tiles > 0) L.launch(kv4::attend_query_kernel<T, D>, dim3(plan.row_tiles, cache->kv_heads, cache->batch), dim3(kv4::kTileRows), 0, c, p);
             const dim3 many(plan.many_tiles, cache->kv_heads, cache->batch);
             if (plan.many_tiles > 0) {
-                if (cache->dtype == EFM_F16 || p.mass_out != nullptr) L.launch(kv4::attend_many_kernel<T, D, true>, many, dim3(kv4::kManyThreads), kv4::ManyCfg<D, true>::SMEM, c, p);
-                else if constexpr (std::is_same<T, __nv_bfloat16>::value) L.launch(kv4::attend_many_kernel<T, D, false>, many, dim3(kv4::kManyThreads), kv4::ManyCfg<D, false>::SMEM, c, p);
+                const dim3 threads(kv4::kManyThreads);
+                if constexpr (std::is_same<T, __half>::value) L.launch(kv4::attend_many_kernel<T, D, 2>, many, threads, kv4::ManyCfg<D, 2>::SMEM, c, p);
+                else if (p.mass_out != nullptr) L.launch(kv4::attend_many_kernel<T, D, 1>, many, threads, kv4::ManyCfg<D, 1>::SMEM, c, p);
+                else L.launch(kv4::attend_many_kernel<T, D, 0>, many, threads, kv4::ManyCfg<D, 0>::SMEM, c, p);
             }
             L.pdl = rows > 0;                          // what follows reads lengths ahead of its wait: not as a call's first launch
             if (join.x > 0 && plan.nt == 1) L.launch(kv4::attend_merge_kernel<T, D, 8>, join, block, 0, c, p, masses);

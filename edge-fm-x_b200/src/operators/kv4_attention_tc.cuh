@@ -12,8 +12,8 @@
 //                    buffers a tile and runs two pages ahead of P V; weights take the place of the scores they came from.  A wait costs
 //                    that warp some 250 cycles even when it is over; one warp for both tiles left the tensor pipe idle half the time.
 // q is scaled by a power of two per row to be exact in fp16.  k, v and p are rounded to fp16 (2^-11), well below the half step of a bf16
-// output (2^-8).  Where that would show (X: fp16 outputs, and row sums that weights are divided by) each is a pair high + low instead:
-// S = Q (Kh + Kl), O += Ph Vh + Pl Vh + Ph Vl.
+// output (2^-8).  Where that would show they are pairs high + low: k where row sums are wanted that summed weights are divided by (X 1:
+// S = Q (Kh + Kl)), and all of them for fp16 outputs (X 2: O += Ph Vh + Pl Vh + Ph Vl as well).
 // A barrier is waited for by parity, which tells a phase from its neighbours only: every barrier here is either waited for in each of its
 // phases by whoever its next phase needs, or (o_done) has a copy per page parity, whose next phase needs the waiting thread's weights of
 // two pages later.
@@ -29,13 +29,13 @@ namespace kv4 {
 
 constexpr int kTileRows = 128, kManyThreads = 15 * 32;
 
-template <int D, bool X>
+template <int D, int X>
 struct ManyCfg {
     static constexpr int G = D / 64;
-    static constexpr int KS = X ? 2 : 3, VS = X ? 2 : 3, LEAD = KS - 1, RAW = LEAD + 2;          // K is converted LEAD pages ahead of V; pages in the ring of raw ones
+    static constexpr int KS = X >= 1 ? 2 : 3, VS = X == 2 ? 2 : 3, LEAD = KS - 1, RAW = LEAD + 2;          // K is converted LEAD pages ahead of V; pages in the ring of raw ones
     static constexpr int Q_BYTES = kTileRows * 128 * G, LOW = kRows * 128 * G;           // of one tile; of K or V of a page, and where its low half begins
-    static constexpr int KV_BYTES = X ? 2 * LOW : LOW;
-    static constexpr int Q_AT = 0, K_AT = 2 * Q_BYTES, V_AT = K_AT + KS * KV_BYTES, RAW_AT = V_AT + VS * KV_BYTES, BARS = RAW_AT + RAW * Tile<D>::BYTES;
+    static constexpr int KB = X >= 1 ? 2 * LOW : LOW, VB = X == 2 ? 2 * LOW : LOW;       // bytes of a stage
+    static constexpr int Q_AT = 0, K_AT = 2 * Q_BYTES, V_AT = K_AT + KS * KB, RAW_AT = V_AT + VS * VB, BARS = RAW_AT + RAW * Tile<D>::BYTES;
     static constexpr int S_COL = 0, O_COL = 256;                                         // S of (tile, page parity): 64 columns each, P in its place; O: 128 a tile
     static constexpr size_t SMEM = BARS + 320 + 1024;
 };
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(kTileRows) attend_query_kernel(const Cache c, 
 }
 
 // grid (tiles of 256 packed rows, kv heads, batch); late rows see the most keys and come first
-template <typename T, int D, bool X>
+template <typename T, int D, int X>
 __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cache c, const AttnParams p) {
     using C = ManyCfg<D, X>;
     using L = Tile<D>;
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
                 float alpha = 1.0f;
                 if (grow) { alpha = at::ex2(m - mn); l *= alpha; m = mn; }
                 const float off = m == -INFINITY ? kLift : kLift - m;
-                uint32_t pk[32], pl[X ? 32 : 1];
+                uint32_t pk[32], pl[X == 2 ? 32 : 1];
                 float sum[2] = {0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < 64; i += 2) {
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
                     sum[0] += a;
                     sum[1] += bb;
                     pk[i >> 1] = half_pair(a, bb);
-                    if constexpr (X) {
+                    if constexpr (X == 2) {
                         const float2 r = Num<__half>::two(pk[i >> 1]);
                         pl[i >> 1] = half_pair(a - r.x, bb - r.y);
                     }
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
                     }
                 }
                 tmem_st32(s_at, pk);
-                if constexpr (X) tmem_st32(s_at + 32, pl);
+                if constexpr (X == 2) tmem_st32(s_at + 32, pl);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 warp_arrive(p_full + 8 * buf);
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             constexpr bool V = decltype(values)::value;
             const uint8_t* page = sm + C::RAW_AT + (j % C::RAW) * L::BYTES;
             const int valid = there[j & 7] ? min(kRows, e.len - j * kRows) : 0;
-            unsigned char* to = sm + (V ? C::V_AT + (j % C::VS) * C::KV_BYTES : C::K_AT + (j % C::KS) * C::KV_BYTES);
+            unsigned char* to = sm + (V ? C::V_AT + (j % C::VS) * C::VB : C::K_AT + (j % C::KS) * C::KB);
             const uint32_t* codes = reinterpret_cast<const uint32_t*>(page + (V ? L::V_CODES : L::K_CODES));
             const __half2* pars = reinterpret_cast<const __half2*>(page + (V ? L::V_PARAMS : L::K_PARAMS));
 #pragma unroll
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         uint4* dst = reinterpret_cast<uint4*>(to + g * (kRows * 128) + r * 128 + (((2 * x + i) ^ (r & 7)) << 4));
-                        if constexpr (X) {
+                        if constexpr (V ? X == 2 : X >= 1) {
                             uint4 high, low;
                             half_pairs(w[g][i], par, high, low);
                             *dst = high;
@@ -395,10 +395,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
         const uint32_t s0 = tm + (uint32_t)(C::S_COL + t * 128), to = tm + (uint32_t)(C::O_COL + t * 128);
         auto issue_s = [&](int j) {                              // into the buffer of the page's parity
             if (lead) {
-                const uint64_t kt = kd + (uint64_t)(j % C::KS * (C::KV_BYTES >> 4));
+                const uint64_t kt = kd + (uint64_t)(j % C::KS * (C::KB >> 4));
                 const uint32_t s_to = s0 + (uint32_t)((j & 1) * 64);
 #pragma unroll
-                for (int i = 0; i < (X ? 2 : 1) * (D / 16); ++i) {
+                for (int i = 0; i < (X >= 1 ? 2 : 1) * (D / 16); ++i) {
                     const int k = i % (D / 16), low = i / (D / 16);
                     at::umma_d(s_to, qt + (uint64_t)((k >> 2) * (kTileRows * 128 >> 4) + (k & 3) * 2), kt + (uint64_t)((low * C::LOW + (k >> 2) * (kRows * 128)) / 16 + (k & 3) * 2), kDescS, i != 0 ? 1u : 0u);
                 }
@@ -422,10 +422,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (lead) {
-                const uint64_t vt = vd + (uint64_t)(j % C::VS * (C::KV_BYTES >> 4));
+                const uint64_t vt = vd + (uint64_t)(j % C::VS * (C::VB >> 4));
                 const uint32_t from = s0 + (uint32_t)((j & 1) * 64);
 #pragma unroll
-                for (int i = 0; i < (X ? 3 : 1) * (kRows / 16); ++i) {
+                for (int i = 0; i < (X == 2 ? 3 : 1) * (kRows / 16); ++i) {
                     const int k = i % (kRows / 16), part = i / (kRows / 16);                       // Ph Vh, Pl Vh, Ph Vl
                     at::umma_ts(to, from + (uint32_t)((part == 1 ? 32 : 0) + 8 * k), vt + (uint64_t)((part == 2 ? C::LOW : 0) / 16 + k * (2048 >> 4)), kDescO, i != 0 || j > 0 ? 1u : 0u);
                 }
