@@ -270,12 +270,13 @@ efm_status efm_b200_op_kv4_append(const efm_kv4_cache* cache, const efm_kv4_appe
         p.inv_freq = a->inv_freq; p.positions = a->positions; p.token_index = a->token_index;
         p.q_out = a->q_out; p.k_held = a->k_held; p.v_held = a->v_held;
         p.index = a->index; p.mass = a->mass;
-        const int heads = cache->q_heads + 2 * cache->kv_heads, warps = kv4::kAppendThreads / 32;
-        // few rows: a head per warp, so that the row's heads are on as many SMs as there are; many rows: a block per row, one table of angles
-        const int per_block = a->max_rows * ((heads + warps - 1) / warps) <= 2 * info.sms ? warps : heads;
+        const int per = 256 / cache->head_dim, kv = (cache->kv_heads + per - 1) / per, tasks = (a->q != nullptr ? (cache->q_heads + per - 1) / per : 0) + 2 * kv, warps = kv4::kAppendThreads / 32;
+        // few rows: a task (the heads a warp has at a time) per warp, so that a row's heads are on as many SMs as there are; many rows: a
+        // block per row, one table of angles
+        const int per_block = a->max_rows * ((tasks + warps - 1) / warps) <= 2 * info.sms ? warps : tasks;
         Launcher L = on_stream(stream);
         by_type(cache, [&](auto t, auto d) {
-            L.launch(kv4::append_kernel<decltype(t), decltype(d)::value>, dim3(std::max(a->max_rows, 1), (heads + per_block - 1) / per_block), dim3(kv4::kAppendThreads), 0,
+            L.launch(kv4::append_kernel<decltype(t), decltype(d)::value>, dim3(std::max(a->max_rows, 1), (tasks + per_block - 1) / per_block), dim3(kv4::kAppendThreads), 0,
                      device_cache(cache), p, per_block);
         });
         return launched(call, L);

@@ -97,14 +97,23 @@ __device__ __forceinline__ float turn(float a, float c, float b, float s, bool p
     return plus ? __fadd_rn(x, y) : __fsub_rn(x, y);
 }
 
-// grid (rows, parts of the row's heads); a warp has one head at a time, a lane D / 32 neighbouring channels of it.
+// rint(a / s) for 0 <= a <= 15.01 s: by the reciprocal unless that lies within its error of a border (products and quotient are off by
+// 2^-22 each: 8e-6 at 16), where the division decides.  Divisions for every code were half of the kernel's instructions.
+__device__ __forceinline__ float code_of(float a, float s, float inv) {
+    const float r = a * inv, n = rintf(r);
+    if (fabsf(fabsf(r - n) - 0.5f) < 1e-5f) return rintf(__fdiv_rn(a, s));
+    return n;
+}
+
+// grid (rows, parts of the row's heads); a lane has eight neighbouring channels of a head (one word of codes), a warp 32 / (D / 8) heads
+// of one kind at a time.
 template <typename T, int D>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const Cache c, const AppendParams p, int heads_per_block) {
-    constexpr int E = D / 32;
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const Cache c, const AppendParams p, int tasks_per_block) {
+    constexpr int LANES = D / 8, HEADS = 32 / LANES;         // lanes of a head, heads of a warp
     using L = Tile<D>;
     __shared__ float2 rot[D / 2];
     __shared__ int owner;
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LANES, c0 = sub * 8;
     const int cap = c.max_pages * kRows;
     pdl_launch_dependents();
     pdl_wait();
@@ -119,8 +128,9 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const Cache c, c
             if (n > cap - have) raise(c, kFull);
         }
     }
-    if (p.rot_dims > 0 && row < p.max_rows)
-        for (int i = tid; i < p.rot_dims / 2; i += kAppendThreads) {
+    const int half = p.rot_dims / 2;
+    if (half > 0 && row < p.max_rows)
+        for (int i = kAppendThreads - 1 - tid; i < half; i += kAppendThreads) {      // by the warps that do not look for the owner
             const int axis = p.axes == 1 || i < p.section0 ? 0 : i < p.section0 + p.section1 ? 1 : 2;
             double s, co;
             sincos((double)p.positions[(size_t)axis * p.max_rows + row] * p.inv_freq[i], &s, &co);
@@ -131,107 +141,99 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const Cache c, c
     const int b = owner;
     const int64_t behind = held(c, p.lens_in, b, cap) + ((int64_t)row - p.cu_rows[b]);
     const int place = behind < cap ? (int)behind : cap, page = place < cap ? page_of(c, b, place / kRows) : -1, r = place % kRows;
-    const int heads = c.q_heads + 2 * c.kv_heads, last = min(heads, ((int)blockIdx.y + 1) * heads_per_block);
-    for (int h = blockIdx.y * heads_per_block + warp; h < last; h += kAppendThreads / 32) {
-        const int kind = h < c.q_heads ? 0 : h < c.q_heads + c.kv_heads ? 1 : 2;      // q, k, v
-        const int hh = kind == 0 ? h : kind == 1 ? h - c.q_heads : h - c.q_heads - c.kv_heads;
-        if (kind == 0 && p.q == nullptr) continue;
-        const T* src = kind == 0 ? (const T*)p.q + row * p.q_stride : kind == 1 ? (const T*)p.k + row * p.k_stride : (const T*)p.v + row * p.v_stride;
-        src += (size_t)hh * D + lane * E;
-        float x[E];
-        if constexpr (E == 4) {
-            const uint2 w = *reinterpret_cast<const uint2*>(src);
-            const float2 lo = Num<T>::two(w.x), hi = Num<T>::two(w.y);
-            x[0] = lo.x; x[1] = lo.y; x[2] = hi.x; x[3] = hi.y;
-        } else {
-            const float2 lo = Num<T>::two(*reinterpret_cast<const uint32_t*>(src));
-            x[0] = lo.x; x[1] = lo.y;
+    const bool turns = c0 < p.rot_dims, second = c0 >= half;
+    const int partner = (lane & ~(LANES - 1)) + ((second ? sub - half / 8 : sub + half / 8) & (LANES - 1));
+    const int tq = p.q != nullptr ? (c.q_heads + HEADS - 1) / HEADS : 0, tk = (c.kv_heads + HEADS - 1) / HEADS;
+    const int last = min(tq + 2 * tk, ((int)blockIdx.y + 1) * tasks_per_block);
+    for (int task = blockIdx.y * tasks_per_block + warp; task < last; task += kAppendThreads / 32) {
+        const int kind = task < tq ? 0 : task < tq + tk ? 1 : 2;                      // q, k, v
+        const int h = (kind == 0 ? task : kind == 1 ? task - tq : task - tq - tk) * HEADS + lane / LANES, n_heads = kind == 0 ? c.q_heads : c.kv_heads;
+        const bool have = h < n_heads;
+        const T* src = (kind == 0 ? (const T*)p.q + row * p.q_stride : kind == 1 ? (const T*)p.k + row * p.k_stride : (const T*)p.v + row * p.v_stride) + (size_t)h * D + c0;
+        float x[8];
+        {
+            const uint4 w = have ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
+            const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { const float2 f = Num<T>::two(v[k]); x[2 * k] = f.x; x[2 * k + 1] = f.y; }
         }
         if (kind < 2 && p.norm) {
             double sq = 0.0;
 #pragma unroll
-            for (int e = 0; e < E; ++e) sq += (double)x[e] * (double)x[e];
+            for (int e = 0; e < 8; ++e) sq += (double)x[e] * (double)x[e];
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+            for (int o = LANES / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
             const float f = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn((float)(sq / D), p.eps)));
             const T* w = (const T*)(kind == 0 ? p.q_norm : p.k_norm);
+            uint4 ww = make_uint4(0u, 0u, 0u, 0u);
+            if (w != nullptr) ww = *reinterpret_cast<const uint4*>(w + c0);
+            const uint32_t v[4] = {ww.x, ww.y, ww.z, ww.w};
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                x[e] = __fmul_rn(x[e], f);
-                if (w != nullptr) x[e] = __fmul_rn(x[e], (float)w[lane * E + e]);
+            for (int k = 0; k < 4; ++k) {
+                const float2 g = Num<T>::two(v[k]);
+                x[2 * k] = __fmul_rn(x[2 * k], f);
+                x[2 * k + 1] = __fmul_rn(x[2 * k + 1], f);
+                if (w != nullptr) { x[2 * k] = __fmul_rn(x[2 * k], g.x); x[2 * k + 1] = __fmul_rn(x[2 * k + 1], g.y); }
             }
         }
-        if (kind < 2 && p.rot_dims > 0) {
-            const int c0 = lane * E, half = p.rot_dims / 2;
+        if (kind < 2 && half > 0) {
             if (p.neighbours) {
-                if (c0 < p.rot_dims) {
+                if (turns) {
 #pragma unroll
-                    for (int e = 0; e < E; e += 2) {
+                    for (int e = 0; e < 8; e += 2) {
                         const float2 cs = rot[(c0 + e) / 2];
-                        const float a = x[e], bb = x[e + 1];
-                        x[e] = turn(a, cs.x, bb, cs.y, false);
-                        x[e + 1] = turn(bb, cs.x, a, cs.y, true);
+                        const float u = x[e], w = x[e + 1];
+                        x[e] = turn(u, cs.x, w, cs.y, false);
+                        x[e + 1] = turn(w, cs.x, u, cs.y, true);
                     }
                 }
             } else {
-                const bool second = c0 >= half;
-                const int from = second ? lane - half / E : lane + half / E;
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float o = __shfl_sync(0xffffffffu, x[e], from & 31);
-                    if (c0 < p.rot_dims) {
+                for (int e = 0; e < 8; ++e) {
+                    const float o = __shfl_sync(0xffffffffu, x[e], partner);
+                    if (turns) {
                         const float2 cs = rot[(second ? c0 - half : c0) + e];
                         x[e] = turn(x[e], cs.x, o, cs.y, second);
                     }
                 }
             }
         }
-        auto put = [&](void* out, int n_heads) {
-            T* dst = (T*)out + ((size_t)row * n_heads + hh) * D + lane * E;
-            if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(Num<T>::pack(x[0], x[1]), Num<T>::pack(x[2], x[3]));
-            else *reinterpret_cast<uint32_t*>(dst) = Num<T>::pack(x[0], x[1]);
+        auto put = [&](void* out) {
+            if (have)
+                *reinterpret_cast<uint4*>((T*)out + ((size_t)row * n_heads + h) * D + c0) =
+                    make_uint4(Num<T>::pack(x[0], x[1]), Num<T>::pack(x[2], x[3]), Num<T>::pack(x[4], x[5]), Num<T>::pack(x[6], x[7]));
         };
-        if (kind == 0) { put(p.q_out, c.q_heads); continue; }
+        if (kind == 0) { put(p.q_out); continue; }
         float lo = INFINITY, hi = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
+        for (int e = 0; e < 8; ++e) {
             x[e] = x[e] != x[e] ? 0.0f : fminf(fmaxf(x[e], -65504.0f), 65504.0f);
             lo = fminf(lo, x[e]);
             hi = fmaxf(hi, x[e]);
         }
 #pragma unroll
-        for (int o = kGroup / E / 2; o > 0; o >>= 1) {
+        for (int o = kGroup / 16; o > 0; o >>= 1) {
             lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
             hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         }
         const __half sh = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f)), mh = __float2half_rn(lo);
-        const float s = __half2float(sh), m = __half2float(mh);
+        const float s = __half2float(sh), m = __half2float(mh), inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
         uint32_t word = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const float code = s > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[e], m), s)), 0.0f), 15.0f) : 0.0f;
+        for (int e = 0; e < 8; ++e) {
+            const float code = s > 0.0f ? fminf(fmaxf(code_of(__fsub_rn(x[e], m), s, inv), 0.0f), 15.0f) : 0.0f;
             x[e] = __fadd_rn(m, __fmul_rn(s, code));
-            const int i = (lane * E + e) & 7;
-            word |= (uint32_t)(int)code << (4 * ((i >> 1) + 4 * (i & 1)));
+            word |= (uint32_t)(int)code << (4 * nibble(e));
         }
-        word |= __shfl_xor_sync(0xffffffffu, word, 1);
-        if constexpr (E == 2) word |= __shfl_xor_sync(0xffffffffu, word, 2);
         void* want = kind == 1 ? p.k_held : p.v_held;
-        if (want != nullptr) put(want, c.kv_heads);
-        if (page < 0) continue;
-        uint8_t* tile = tile_of<D>(c, page, hh);
-        const int w = lane * E / 8;
-        if (lane * E % 8 == 0) {
-            uint32_t* codes = reinterpret_cast<uint32_t*>(tile + (kind == 1 ? L::K_CODES : L::V_CODES)) + r * L::WORDS;
-            codes[kind == 1 ? key_word<D>(w) : w] = word;
-        }
-        if (lane * E % kGroup == 0) {
-            __half2* par = reinterpret_cast<__half2*>(tile + (kind == 1 ? L::K_PARAMS : L::V_PARAMS)) + r * L::G;
-            par[lane * E / kGroup] = __halves2half2(sh, mh);
-        }
-        if (kind == 1 && lane == 0) {
-            if (p.index != nullptr) p.index[row_slot(c, page, hh, r)] = p.token_index != nullptr ? p.token_index[row] : place;
-            if (p.mass != nullptr) p.mass[row_slot(c, page, hh, r)] = 0.0f;
+        if (want != nullptr) put(want);
+        if (page < 0 || !have) continue;
+        uint8_t* tile = tile_of<D>(c, page, h);
+        reinterpret_cast<uint32_t*>(tile + (kind == 1 ? L::K_CODES : L::V_CODES))[r * L::WORDS + (kind == 1 ? key_word<D>(sub) : sub)] = word;
+        if (sub % 8 == 0) reinterpret_cast<__half2*>(tile + (kind == 1 ? L::K_PARAMS : L::V_PARAMS))[r * L::G + sub / 8] = __halves2half2(sh, mh);
+        if (kind == 1 && sub == 0) {
+            if (p.index != nullptr) p.index[row_slot(c, page, h, r)] = p.token_index != nullptr ? p.token_index[row] : place;
+            if (p.mass != nullptr) p.mass[row_slot(c, page, h, r)] = 0.0f;
         }
     }
 }
