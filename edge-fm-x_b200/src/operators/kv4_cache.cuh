@@ -89,7 +89,7 @@ struct AppendParams {
     float* mass;
 };
 
-constexpr int kAppendThreads = 256;
+constexpr int kAppendThreads = 128;
 
 // Channels turned: (a, b) -> (a cos - b sin, b cos + a sin), three roundings each.
 __device__ __forceinline__ float turn(float a, float c, float b, float s, bool plus) {
@@ -97,12 +97,27 @@ __device__ __forceinline__ float turn(float a, float c, float b, float s, bool p
     return plus ? __fadd_rn(x, y) : __fsub_rn(x, y);
 }
 
-// rint(a / s) for 0 <= a <= 15.01 s: by the reciprocal unless that lies within its error of a border (products and quotient are off by
-// 2^-22 each: 8e-6 at 16), where the division decides.  Divisions for every code were half of the kernel's instructions.
-__device__ __forceinline__ float code_of(float a, float s, float inv) {
-    const float r = a * inv, n = rintf(r);
-    if (fabsf(fabsf(r - n) - 0.5f) < 1e-5f) return rintf(__fdiv_rn(a, s));
-    return n;
+// Codes of eight channels, rint((x - m) / s) in 0 .. 15, and the word they make.  By the reciprocal unless a quotient lies within its error
+// of a border (product and reciprocal are off by 2^-22 together: 4e-6 at 16), where the divisions decide: IEEE divisions for all of them
+// were half of the kernel's instructions.  Rounding by adding 1.5 * 2^23 leaves the code in the sum's low bits.
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float m, float s, float (&code)[8]) {
+    constexpr float kMagic = 12582912.0f;
+    const float inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
+    float near = 1.0f, r[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        r[e] = fminf(fmaxf(__fmul_rn(__fsub_rn(x[e], m), inv), 0.0f), 15.25f);
+        const float t = __fadd_rn(r[e], kMagic);
+        code[e] = __fsub_rn(t, kMagic);
+        near = fminf(near, fabsf(fabsf(__fsub_rn(r[e], code[e])) - 0.5f));
+    }
+    if (near < 1e-5f && s > 0.0f)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) code[e] = rintf(fminf(fmaxf(__fdiv_rn(__fsub_rn(x[e], m), s), 0.0f), 15.25f));
+    uint32_t word = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) word |= (__float_as_uint(__fadd_rn(code[e], kMagic)) & 15u) << (4 * nibble(e));
+    return word;
 }
 
 // grid (rows, parts of the row's heads); a lane has eight neighbouring channels of a head (one word of codes), a warp 32 / (D / 8) heads
@@ -112,20 +127,39 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const Cache c, c
     constexpr int LANES = D / 8, HEADS = 32 / LANES;         // lanes of a head, heads of a warp
     using L = Tile<D>;
     __shared__ float2 rot[D / 2];
-    __shared__ int owner;
+    __shared__ int place_s, page_s;                          // cache row and page of the row; place -1: nobody's row
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LANES, c0 = sub * 8;
     const int cap = c.max_pages * kRows;
+    const int tq = p.q != nullptr ? (c.q_heads + HEADS - 1) / HEADS : 0, tk = (c.kv_heads + HEADS - 1) / HEADS;
+    const int last = min(tq + 2 * tk, ((int)blockIdx.y + 1) * tasks_per_block);
+    auto kind_of = [&](int task) { return task < tq ? 0 : task < tq + tk ? 1 : 2; };      // q, k, v
+    auto head_of = [&](int task) { return (task < tq ? task : task < tq + tk ? task - tq : task - tq - tk) * HEADS + lane / LANES; };
+    auto fetch = [&](int task) {
+        const int kind = kind_of(task), h = head_of(task);
+        if (task >= last || h >= (kind == 0 ? c.q_heads : c.kv_heads)) return make_uint4(0u, 0u, 0u, 0u);
+        const T* src = kind == 0 ? (const T*)p.q + row * p.q_stride : kind == 1 ? (const T*)p.k + row * p.k_stride : (const T*)p.v + row * p.v_stride;
+        return *reinterpret_cast<const uint4*>(src + (size_t)h * D + c0);
+    };
+    if (tid == 0) place_s = -1;
+    __syncthreads();
     pdl_launch_dependents();
     pdl_wait();
-    if (tid == 0) owner = -1;
-    __syncthreads();
+    int task = blockIdx.y * tasks_per_block + warp;
+    uint4 next = row < p.max_rows ? fetch(task) : make_uint4(0u, 0u, 0u, 0u);             // on its way while the row's place is looked up
     for (int b = tid; b < c.batch; b += kAppendThreads) {
         const int lo = p.cu_rows[b], hi = p.cu_rows[b + 1];
-        if (row >= lo && row < hi && row < p.max_rows) owner = b;
-        if (row == 0 && blockIdx.y == 0) {
-            const int n = max(0, min(hi, p.max_rows) - max(min(lo, p.max_rows), 0)), have = held(c, p.lens_in, b, cap);
+        const bool mine = row >= lo && row < hi && row < p.max_rows, tells = row == 0 && blockIdx.y == 0;
+        if (!mine && !tells) continue;
+        const int have = held(c, p.lens_in, b, cap);
+        if (tells) {
+            const int n = max(0, min(hi, p.max_rows) - max(min(lo, p.max_rows), 0));
             p.lens_out[b] = min(cap - have, n) + have;
             if (n > cap - have) raise(c, kFull);
+        }
+        if (mine) {
+            const int64_t behind = have + ((int64_t)row - lo);
+            place_s = behind < cap ? (int)behind : cap;
+            page_s = behind < cap ? page_of(c, b, (int)behind / kRows) : -1;
         }
     }
     const int half = p.rot_dims / 2;
@@ -137,26 +171,20 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const Cache c, c
             rot[i] = make_float2((float)co, (float)s);
         }
     __syncthreads();
-    if (owner < 0) return;
-    const int b = owner;
-    const int64_t behind = held(c, p.lens_in, b, cap) + ((int64_t)row - p.cu_rows[b]);
-    const int place = behind < cap ? (int)behind : cap, page = place < cap ? page_of(c, b, place / kRows) : -1, r = place % kRows;
+    if (place_s < 0) return;
+    const int place = place_s, page = page_s, r = place % kRows;
     const bool turns = c0 < p.rot_dims, second = c0 >= half;
     const int partner = (lane & ~(LANES - 1)) + ((second ? sub - half / 8 : sub + half / 8) & (LANES - 1));
-    const int tq = p.q != nullptr ? (c.q_heads + HEADS - 1) / HEADS : 0, tk = (c.kv_heads + HEADS - 1) / HEADS;
-    const int last = min(tq + 2 * tk, ((int)blockIdx.y + 1) * tasks_per_block);
-    for (int task = blockIdx.y * tasks_per_block + warp; task < last; task += kAppendThreads / 32) {
-        const int kind = task < tq ? 0 : task < tq + tk ? 1 : 2;                      // q, k, v
-        const int h = (kind == 0 ? task : kind == 1 ? task - tq : task - tq - tk) * HEADS + lane / LANES, n_heads = kind == 0 ? c.q_heads : c.kv_heads;
+    for (; task < last; task += kAppendThreads / 32) {
+        const int kind = kind_of(task), h = head_of(task), n_heads = kind == 0 ? c.q_heads : c.kv_heads;
         const bool have = h < n_heads;
-        const T* src = (kind == 0 ? (const T*)p.q + row * p.q_stride : kind == 1 ? (const T*)p.k + row * p.k_stride : (const T*)p.v + row * p.v_stride) + (size_t)h * D + c0;
         float x[8];
         {
-            const uint4 w = have ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
-            const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+            const uint32_t v[4] = {next.x, next.y, next.z, next.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) { const float2 f = Num<T>::two(v[k]); x[2 * k] = f.x; x[2 * k + 1] = f.y; }
         }
+        next = fetch(task + kAppendThreads / 32);
         if (kind < 2 && p.norm) {
             double sq = 0.0;
 #pragma unroll
@@ -217,16 +245,15 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const Cache c, c
             hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         }
         const __half sh = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f)), mh = __float2half_rn(lo);
-        const float s = __half2float(sh), m = __half2float(mh), inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
-        uint32_t word = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float code = s > 0.0f ? fminf(fmaxf(code_of(__fsub_rn(x[e], m), s, inv), 0.0f), 15.0f) : 0.0f;
-            x[e] = __fadd_rn(m, __fmul_rn(s, code));
-            word |= (uint32_t)(int)code << (4 * nibble(e));
-        }
+        const float s = __half2float(sh), m = __half2float(mh);
+        float code[8];
+        const uint32_t word = codes_of(x, m, s, code);
         void* want = kind == 1 ? p.k_held : p.v_held;
-        if (want != nullptr) put(want);
+        if (want != nullptr) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __fadd_rn(m, __fmul_rn(s, code[e]));
+            put(want);
+        }
         if (page < 0 || !have) continue;
         uint8_t* tile = tile_of<D>(c, page, h);
         reinterpret_cast<uint32_t*>(tile + (kind == 1 ? L::K_CODES : L::V_CODES))[r * L::WORDS + (kind == 1 ? key_word<D>(sub) : sub)] = word;
