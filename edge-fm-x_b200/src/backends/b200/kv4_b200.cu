@@ -23,7 +23,7 @@ efm_status check_cache(const char* call, const efm_kv4_cache* c) {
     if (c->dtype != EFM_BF16 && c->dtype != EFM_F16) return fail(nullptr, EFM_ERR_UNSUPPORTED, std::string(call) + ": dtype bf16 or fp16");
     if (c->head_dim != 64 && c->head_dim != 128) return fail(nullptr, EFM_ERR_UNSUPPORTED, std::string(call) + ": head_dim 64 or 128");
     if (c->kv_heads < 1 || c->q_heads < 1 || c->q_heads > 1024 || c->q_heads % c->kv_heads != 0) return bad(call, "q_heads a multiple of kv_heads, at most 1024");
-    if (c->n_pages < 1 || c->batch < 1 || c->batch > 65535 || c->max_pages < 1 || c->max_pages >= (1 << 24)) return bad(call, "n_pages, batch or max_pages out of range");
+    if (c->n_pages < 1 || c->n_pages > (1 << 24) || c->batch < 1 || c->batch > 65535 || c->max_pages < 1 || c->max_pages >= (1 << 24)) return bad(call, "n_pages, batch or max_pages out of range");
     return EFM_OK;
 }
 efm_status check_buffers(const char* call, const efm_kv4_cache* c) {
@@ -367,13 +367,15 @@ efm_status efm_b200_op_kv4_evict(const efm_kv4_cache* cache, const efm_kv4_evict
         p.n_moves = (int32_t*)a->workspace;
         p.moves = (int2*)((char*)a->workspace + evict_counts(cache));
         p.most_moves = (int)most_moves(cache, a);
+        p.head_dim = cache->head_dim;
+        p.inline_moves = p.most_moves <= kv4::kInlineMoves;
         p.keys_cap = (int)std::min<int64_t>(capacity(cache), (info.smem - kEvictSmemReserve) / 4);
         Launcher L = on_stream(stream);
         const kv4::Cache c = device_cache(cache);
         L.launch(kv4::evict_select_kernel, dim3(cache->kv_heads, cache->batch), dim3(kv4::kEvictThreads), (size_t)p.keys_cap * 4, c, p);
-        if (p.most_moves > 0) {
+        if (!p.inline_moves) {
             const int per = kv4::kMoveThreads / 16, all = (p.most_moves + per - 1) / per;
-            const int parts = (int)std::min<int64_t>(all, std::max<int64_t>(1, (int64_t)16 * info.sms / ((int64_t)cache->batch * cache->kv_heads)));
+            const int parts = (int)std::min<int64_t>(all, std::max<int64_t>(1, (int64_t)8 * info.sms / ((int64_t)cache->batch * cache->kv_heads)));
             if (cache->head_dim == 64) L.launch(kv4::evict_move_kernel<64>, dim3(parts, cache->kv_heads, cache->batch), dim3(kv4::kMoveThreads), 0, c, p);
             else L.launch(kv4::evict_move_kernel<128>, dim3(parts, cache->kv_heads, cache->batch), dim3(kv4::kMoveThreads), 0, c, p);
         }

@@ -46,7 +46,7 @@ typedef struct efm_kv4_cache {
     int32_t dtype;                /* of q, k, v and the outputs: EFM_BF16 or EFM_F16 */
     int32_t q_heads, kv_heads;    /* q_heads a multiple of kv_heads, <= 1024 */
     int32_t head_dim;             /* 64 or 128 */
-    int32_t n_pages;              /* pages in pool */
+    int32_t n_pages;              /* pages in pool, <= 2^24 */
     int32_t batch;                /* sequences of the call, >= 1, <= 65535 */
     int32_t max_pages;            /* columns of page_table, >= 1, < 2^24 */
     void* pool;                   /* [n_pages, kv_heads, efm_b200_kv4_tile_bytes] */

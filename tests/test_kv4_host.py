@@ -102,7 +102,7 @@ def read(**over):
 
 INVALID, UNSUPPORTED = 1, 5
 CACHE_FAULTS = [(dict(struct_size=8), INVALID), (dict(dtype=cabi.EFM_F32), UNSUPPORTED), (dict(head_dim=96), UNSUPPORTED), (dict(q_heads=7), INVALID),
-                (dict(kv_heads=0), INVALID), (dict(q_heads=0), INVALID), (dict(q_heads=2048), INVALID), (dict(n_pages=0), INVALID), (dict(batch=0), INVALID),
+                (dict(kv_heads=0), INVALID), (dict(q_heads=0), INVALID), (dict(q_heads=2048), INVALID), (dict(n_pages=0), INVALID), (dict(n_pages=(1 << 24) + 1), INVALID), (dict(batch=0), INVALID),
                 (dict(batch=65536), INVALID), (dict(max_pages=0), INVALID), (dict(max_pages=1 << 24), INVALID), (dict(pool=None), INVALID),
                 (dict(pool=FAKE + 8), INVALID), (dict(page_table=None), INVALID), (dict(status=FAKE + 1), INVALID)]
 FAULTS = [
