@@ -79,7 +79,7 @@ __device__ __forceinline__ void move_rows(const Cache& c, const EvictParams& p, 
 // for itself.
 __global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const Cache c, const EvictParams p) {
     extern __shared__ uint32_t keys[];
-    __shared__ int hist[kBins * kCopies], counts[2][kKeep * kEvictWarps], digit_sums[2][kEvictWarps], found[2], newest_s;
+    __shared__ int hist[kBins * kCopies], counts[2][kKeep * kEvictWarps + 1], digit_sums[2][kEvictWarps], found[2], newest_s;
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) newest_s = INT32_MIN;
     for (int i = tid; i < kBins * kCopies; i += kEvictThreads) hist[i] = 0;
@@ -190,11 +190,22 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const Ca
     // round by (row of the thread, warp), within a warp by lane.
     int2* moves = p.moves + (size_t)(b * c.kv_heads + h) * p.most_moves;
     int ties = 0, holes = 0, extra = 0;                          // of the rounds before
-    auto offset = [&](const int* cnt, int i, int& total) {       // sum of the round's counts ahead of (i, this warp); all of them
-        int ahead = 0, all = 0;
-        for (int k = lane; k < kKeep * kEvictWarps; k += 32) { const int v = cnt[k]; all += v; if (k < i * kEvictWarps + warp) ahead += v; }
-        total = __reduce_add_sync(0xffffffffu, all);
-        return __reduce_add_sync(0xffffffffu, ahead);
+    auto number = [&](int* cnt) {                                // counts in the rows' order become sums of those ahead, the last entry the total
+        __syncthreads();
+        if (warp == 0) {
+            constexpr int PER = kKeep * kEvictWarps / 32;
+            int v[PER], sum = 0;
+#pragma unroll
+            for (int k = 0; k < PER; ++k) { v[k] = cnt[lane * PER + k]; sum += v[k]; }
+            int before = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += y; }
+            if (lane == 31) cnt[kKeep * kEvictWarps] = before;
+            before -= sum;
+#pragma unroll
+            for (int k = 0; k < PER; ++k) { cnt[lane * PER + k] = before; before += v[k]; }
+        }
+        __syncthreads();
     };
     const uint32_t below = (1u << lane) - 1u;
     for (int base = 0; base < n; base += kKeep * kEvictThreads) {
@@ -215,36 +226,30 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const Ca
             if (lane == 0) counts[0][i * kEvictWarps + warp] = __popc(m);
             if (in && key[i] > border) kept |= 1u << i;
         }
-        __syncthreads();
-        int total = 0;
+        number(counts[0]);
 #pragma unroll
         for (int i = 0; i < kKeep; ++i) {
             const int row = base + i * kEvictThreads + tid;
             const bool in = row < n, tie = in && key[i] == border;
             const uint32_t m = __ballot_sync(0xffffffffu, tie);
-            if (m != 0 || i == 0) {                              // by the whole warp
-                const int rank = ties + offset(counts[0], i, total) + __popc(m & below);
-                if (tie && rank < want) kept |= 1u << i;
-            }
+            if (tie && ties + counts[0][i * kEvictWarps + warp] + __popc(m & below) < want) kept |= 1u << i;
             const bool k = kept >> i & 1u;
             const uint32_t mh = __ballot_sync(0xffffffffu, in && !k && row < p.budget), me = __ballot_sync(0xffffffffu, in && k && row >= p.budget);
             if (lane == 0) counts[1][i * kEvictWarps + warp] = __popc(mh) | __popc(me) << 16;
         }
-        ties += total;
-        __syncthreads();
-        int both = 0;
+        ties += counts[0][kKeep * kEvictWarps];
+        number(counts[1]);
 #pragma unroll
         for (int i = 0; i < kKeep; ++i) {
             const int row = base + i * kEvictThreads + tid;
             const bool in = row < n, k = kept >> i & 1u, hole = in && !k && row < p.budget, ext = in && k && row >= p.budget;
             const uint32_t mh = __ballot_sync(0xffffffffu, hole), me = __ballot_sync(0xffffffffu, ext);
-            if ((mh | me) == 0 && i != 0) continue;
-            const int off = offset(counts[1], i, both);
+            const int off = counts[1][i * kEvictWarps + warp];
             if (hole) moves[holes + (off & 0xffff) + __popc(mh & below)].y = at[i];
             if (ext) moves[extra + (off >> 16) + __popc(me & below)].x = at[i];
         }
-        holes += both & 0xffff;
-        extra += both >> 16;
+        holes += counts[1][kKeep * kEvictWarps] & 0xffff;
+        extra += counts[1][kKeep * kEvictWarps] >> 16;
     }
     if (!p.inline_moves) {
         if (tid == 0) p.n_moves[b * c.kv_heads + h] = holes;     // as many as extra
