@@ -139,11 +139,12 @@ struct AttnPlan {
     int max_new, max_len, nt, blocks, unit, few_rows, many_tiles;      // many_tiles: blocks of 256 packed rows a sequence may have
     bool joined;                                      // pieces of a row may lie in several blocks
     bool scores;                                      // attend_few leaves its scores for the summed weights
-    int64_t units, stats, part_stats, part, score_ld, score, image, image_units;
+    int64_t units, stats, part_stats, part, score_ld, score, image, image_units, starts;
     int row_tiles;                                    // tiles of 128 packed rows a sequence may have as operands; 0: nobody asks for them
-    int64_t bytes() const { return 4 * (stats + part_stats + part + score + image + image_units); }
+    int64_t bytes() const { return 4 * (stats + part_stats + part + score + image + image_units + starts); }
 };
 constexpr int kSms = 148;                              // of the GPU these kernels are built for
+constexpr int kWholePages = 4;
 constexpr int kFewRows = 32;                           // packed rows of a sequence up to which attend_few takes it
 
 AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
@@ -155,15 +156,17 @@ AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
     p.few_rows = kFewRows;
     p.many_tiles = rows > p.few_rows ? (int)((rows + 2 * kv4::kTileRows - 1) / (2 * kv4::kTileRows)) : 0;
     const int64_t R = 8 * p.nt, tiles = (std::min<int64_t>(rows, p.few_rows) + R - 1) / R, pages = std::max(1, (p.max_len + kRows - 1) / kRows);
-    // a page for each warp, or short caches whole: nothing is left to join then
-    p.unit = pages <= 2 * kv4::kWarps ? 2 * kv4::kWarps : kv4::kWarps;
+    // a page at a time, or caches of up to four pages whole: nothing is left to join then, which saves the smallest calls a launch
+    p.unit = pages <= kWholePages ? kWholePages : 1;
     p.units = (pages + p.unit - 1) / p.unit * tiles * c->kv_heads * c->batch;
-    p.blocks = (int)std::max<int64_t>(1, std::min<int64_t>(kSms * (p.nt == 1 ? 3 : 2), p.units));
-    p.joined = pages > p.unit && p.blocks > 1;
+    p.blocks = (int)std::max<int64_t>(1, std::min<int64_t>(kSms * (p.nt == 1 ? 3 : 2), (p.units + kv4::kWarps - 1) / kv4::kWarps));
+    p.joined = pages > p.unit;
     p.scores = a->mass_out != nullptr && rows <= R;
     p.stats = a->mass_out != nullptr ? round_up(2 * (int64_t)c->batch * p.max_new * c->q_heads, 4) : 0;
-    p.part_stats = p.joined ? 2 * 2 * (int64_t)p.blocks * R : 0;
-    p.part = p.joined ? 2 * (int64_t)p.blocks * R * c->head_dim : 0;
+    const int64_t pieces = p.joined ? 2 * (int64_t)p.blocks * kv4::kWarps * R : 0;      // two a warp: the one it begins in and the one it ends in
+    p.part_stats = 2 * pieces;
+    p.part = pieces * c->head_dim;
+    p.starts = round_up(c->batch + 1, 4);
     p.score_ld = round_up(p.max_len, kRows);                   // every part a multiple of 16 bytes
     p.row_tiles = p.many_tiles > 0 || (a->mass_out != nullptr && !p.scores) ? (int)((rows + kv4::kTileRows - 1) / kv4::kTileRows) : 0;
     p.image_units = (int64_t)c->batch * c->kv_heads * p.row_tiles * kv4::kTileRows;
@@ -305,7 +308,7 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
         p.cu_rows = a->cu_rows; p.lens = a->lens; p.q = a->q; p.out = a->out;
         p.scale_log2 = a->scale * 1.4426950408889634f;
         p.mass_in = a->mass_in; p.mass_out = a->mass_out;
-        p.few_rows = plan.few_rows; p.blocks = plan.blocks; p.unit = plan.unit; p.rows = plan.max_new;
+        p.few_rows = plan.few_rows; p.warps = plan.blocks * kv4::kWarps; p.unit = plan.unit; p.rows = plan.max_new;
         float* ws = (float*)a->workspace;
         p.stats = plan.stats > 0 ? (float2*)ws : nullptr;
         p.part_stats = (float2*)(ws + plan.stats);
@@ -315,6 +318,7 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
         p.row_tiles = plan.row_tiles;
         p.images = (uint8_t*)(ws + plan.stats + plan.part_stats + plan.part + plan.score);
         p.units = (float*)p.images + plan.image;
+        p.starts = (int32_t*)(p.units + plan.image_units);
         Launcher L = on_stream(stream);
         by_type(cache, [&](auto t, auto d) {
             using T = decltype(t);
@@ -322,7 +326,9 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
             const dim3 block(kv4::kWarps * 32);
             const kv4::Cache c = device_cache(cache);
             const int64_t rows = (int64_t)plan.max_new * (cache->q_heads / cache->kv_heads);
-            const int merges = plan.joined ? (int)std::min<int64_t>(64, std::min<int64_t>(rows, plan.few_rows)) : 0, masses = plan.scores ? (plan.max_len + kv4::kMassTokens - 1) / kv4::kMassTokens : 0;
+            // as many merging blocks as find room at once
+            const int64_t jobs = std::min<int64_t>(rows, plan.few_rows) * (D / 32), room = std::max<int64_t>(1, 8 * kSms / ((int64_t)cache->batch * cache->kv_heads));
+            const int merges = plan.joined ? (int)std::min(jobs, room) : 0, masses = plan.scores ? (plan.max_len + kv4::kMassTokens - 1) / kv4::kMassTokens : 0;
             const dim3 join(merges + masses, cache->kv_heads, cache->batch);
             if (rows > 0 && plan.nt == 1) L.launch(kv4::attend_few_kernel<T, D, 1>, dim3(plan.blocks), block, kv4::FewCfg<D, 1>::SMEM, c, p);
             if (rows > 0 && plan.nt == 2) L.launch(kv4::attend_few_kernel<T, D, 2>, dim3(plan.blocks), block, kv4::FewCfg<D, 2>::SMEM, c, p);

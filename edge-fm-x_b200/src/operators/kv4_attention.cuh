@@ -21,11 +21,12 @@ struct AttnParams {
     const float* mass_in;
     float* mass_out;
     int few_rows;             // sequences with at most this many packed rows (new rows x heads of a group) are attend_few's
-    int blocks, unit;         // attend_few's blocks; pages of a unit of work
-    float2* stats;            // [batch, rows, q_heads] (maximum, sum) of a row's weights, where one block had all its keys; null: not wanted
+    int warps, unit;          // attend_few's warps; pages of a unit of work
+    float2* stats;            // [batch, rows, q_heads] (maximum, sum) of a row's weights, where one warp had all its keys; null: not wanted
     int rows;                 // new rows a sequence has in stats
-    float2* part_stats;       // [2 blocks][8 nt] the same of the keys a block had, and
-    float* part;              // [2 blocks][8 nt][D] its weighted values: slot 0 is the piece its range begins with, slot 1 the one it ends with
+    float2* part_stats;       // [8 nt][2 warps] the same of the keys a warp had, and
+    float* part;              // [2 warps][8 nt][D] its weighted values: slot 0 is the piece its range begins with, slot 1 the one it ends with
+    int32_t* starts;          // [batch + 1] units ahead of every sequence, and all of them
     uint8_t* images;          // [batch, kv_heads, row_tiles][128 x D fp16] packed rows as operands, and
     float* units;             // [batch, kv_heads, row_tiles][128] what their scores are multiplied with; where many rows are a sequence's
     int row_tiles;
@@ -73,7 +74,7 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar) {
     if ((threadIdx.x & 31) == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// How attend_few's work is dealt: the pages of every (sequence, kv head, tile of R packed rows) in units of p.unit, in that order; block w
+// How attend_few's work is dealt: the pages of every (sequence, kv head, tile of R packed rows) in units of p.unit, in that order; warp w
 // has the units [w step, (w + 1) step).  Lengths are known on the device only, so every block adds them up for itself.
 struct Deal { int before, all; };          // units ahead of sequence b, and altogether
 struct Share { int units, tiles, each; };      // of a sequence; row tiles; units of a tile and head
@@ -87,7 +88,7 @@ __device__ __forceinline__ Share share_of(const Cache& c, const AttnParams& p, i
     s.units = s.tiles * s.each * c.kv_heads;
     return s;
 }
-__device__ __forceinline__ int step_of(const AttnParams& p, int all) { return max(1, (all + p.blocks - 1) / p.blocks); }
+__device__ __forceinline__ int step_of(const AttnParams& p, int all) { return max(1, (all + p.warps - 1) / p.warps); }
 
 // ---- fragments -------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -95,16 +96,16 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
 }
 // d = a b + (c0, c1, c0, c1)
 __device__ __forceinline__ void mma16816_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 __device__ __forceinline__ float ex2f(float x) {
@@ -138,17 +139,25 @@ struct QueryTile {
     uint32_t f[G][4][2];
     float sum[G][2], eight[G][2], unit[2];      // of the lane's two columns 2 j, 2 j + 1: sums of the scaled q, 8 times those, what a score is multiplied with
 
+    struct Raw { uint4 w[G][2]; };
     template <typename T>
-    __device__ __forceinline__ void load(const T* row, bool have, float scale_log2) {       // row: of column lane / 4
-        const int lane = threadIdx.x & 31, j = lane & 3;
+    static __device__ __forceinline__ Raw fetch(const T* row, bool have) {                  // row: of column lane / 4
+        Raw r;
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) r.w[g][h] = have ? *reinterpret_cast<const uint4*>(row + g * 64 + (threadIdx.x & 3) * 16 + h * 8) : make_uint4(0u, 0u, 0u, 0u);
+        return r;
+    }
+    template <typename T>
+    __device__ __forceinline__ void take(const Raw& raw, float scale_log2) {
+        const int j = threadIdx.x & 3;
         float x[G][16], top = 0.f;
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                if (have) w = *reinterpret_cast<const uint4*>(row + g * 64 + j * 16 + h * 8);
-                const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+                const uint32_t v[4] = {raw.w[g][h].x, raw.w[g][h].y, raw.w[g][h].z, raw.w[g][h].w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float2 t = Num<T>::two(v[i]);
@@ -259,25 +268,24 @@ struct FewCfg {
     static constexpr int STAGES = D == 128 ? 2 : 4;
     static constexpr int BLOCKS = NT == 1 ? 3 : 2;                               // per SM
     static constexpr size_t RING = (size_t)kWarps * STAGES * Tile<D>::BYTES;
-    static constexpr int LD = D + 4;                                             // floats of a row in the merge of the warps
-    static constexpr size_t MERGE = (size_t)kWarps * 8 * NT * LD * 4;
-    static constexpr size_t BARS = RING > MERGE ? RING : MERGE;                  // the merge takes the place of the rings, which are idle then
-    static constexpr size_t SMEM = BARS + kWarps * STAGES * 8 + kWarps * 8 * NT * 8 + 16;
+    static constexpr size_t SMEM = RING + kWarps * STAGES * 8 + 16;
 };
 
-// Few query rows.  A warp takes every fourth page of its block's units, each page (one kv head's tile) one bulk copy into the warp's own
-// ring.  The MMA's 16 rows are tokens (channels in P V) and its 8 columns query rows -- the heads of a group, times the new rows -- so
-// that a single token of up to 8 heads per kv head fills it: m16n8k16 the other way round would leave half of it empty.
+// Few query rows.  A warp works for itself on the pages of its units, each page (one kv head's tile) one bulk copy into a ring of its own;
+// where a row's keys are dealt over several warps it leaves its sums, and attend_merge joins them.  Blocks whose warps shared a row and
+// joined it in shared memory spent a third of their time on barriers and waiting for queries behind their own copies.
+// The MMA's 16 rows are tokens (channels in P V) and its 8 columns query rows -- the heads of a group, times the new rows -- so that a
+// single token of up to 8 heads per kv head fills it: m16n8k16 the other way round would leave half of it empty.
+// Bound: instruction issue, 1500 a page of 64 x 128 (half of them on the integer pipe, which takes the codes apart), then bytes.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few_kernel(const Cache c, const AttnParams p) {
     using L = Tile<D>;
     using C = FewCfg<D, NT>;
     constexpr int G = L::G, R = 8 * NT;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ int sums[kWarps], before_s, first_s;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
-    float2* ml_s = reinterpret_cast<float2*>(bars + kWarps * C::STAGES);         // [warps][R]
-    volatile int* abort_s = reinterpret_cast<volatile int*>(ml_s + kWarps * R);
+    __shared__ int sums[kWarps], before_s[kWarps], first_s[kWarps];
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::RING);
+    volatile int* abort_s = reinterpret_cast<volatile int*>(bars + kWarps * C::STAGES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3, group = c.q_heads / c.kv_heads;
     unsigned char* ring = smem + (size_t)warp * C::STAGES * L::BYTES;
     const uint32_t bar0 = tc::smem_u32(bars + warp * C::STAGES);
@@ -285,10 +293,10 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
         for (int i = 0; i < C::STAGES; ++i) tc::mbar_init(bar0 + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (threadIdx.x == 0) { *abort_s = 0; first_s = -1; }
+    if (threadIdx.x == 0) *abort_s = 0;
     pdl_wait();
     pdl_launch_dependents();
-    // this block's range of the units, and the sequence it begins in
+    // the warps' ranges of the units, and the sequences they begin in
     const int per = (c.batch + kWarps * 32 - 1) / (kWarps * 32), b_lo = min(c.batch, (int)threadIdx.x * per), b_hi = min(c.batch, b_lo + per);
     int own = 0;
     for (int b = b_lo; b < b_hi; ++b) own += share_of<R>(c, p, b, group).units;
@@ -302,60 +310,90 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
     __syncthreads();
     int all = 0;
     for (int w = 0; w < kWarps; ++w) { if (w < warp) upto += sums[w]; all += sums[w]; }
-    const int step = step_of(p, all), u0 = min((int64_t)all, (int64_t)blockIdx.x * step), u1 = min(all - u0, step) + u0;
-    if (u0 >= all) return;
-    if (upto - own <= u0 && u0 < upto) {
-        int at = upto - own, b = b_lo;
-        for (int n; at + (n = share_of<R>(c, p, b, group).units) <= u0; ++b) at += n;
-        first_s = b;
-        before_s = at;
+    if (blockIdx.x == 0) {                                                       // for attend_merge
+        if (threadIdx.x == 0) p.starts[c.batch] = all;
+        int at = upto - own;
+        for (int b = b_lo; b < b_hi; ++b) { p.starts[b] = at; at += share_of<R>(c, p, b, group).units; }
+    }
+    const int step = step_of(p, all);
+    auto begins = [&](int w) { return (int)min((int64_t)all, (int64_t)w * step); };
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        const int u = begins(blockIdx.x * kWarps + w);
+        if (upto - own <= u && u < upto) {
+            int at = upto - own, b = b_lo;
+            for (int n; at + (n = share_of<R>(c, p, b, group).units) <= u; ++b) at += n;
+            first_s[w] = b;
+            before_s[w] = at;
+        }
     }
     __syncthreads();
-    int b = first_s, slot = 0;                                                   // slot: of the copies and their barriers
-    int start = before_s;                                                 // unit that sequence b begins with
+    const int me = blockIdx.x * kWarps + warp, u1 = begins(me + 1);
+    int u = begins(me), slot = 0;                                                // slot: of the copies and their barriers
+    if (u >= u1) return;
+    int b = first_s[warp], start = before_s[warp];                               // start: unit that sequence b begins with
 
-    for (int at = u0; at < u1;) {
-        const Share sh = share_of<R>(c, p, b, group);
-        if (at >= start + sh.units) { start += sh.units; ++b; continue; }
-        const Entry e = entry_of(c, p, b);
-        const int rows = e.n * group, pages = (e.len + kRows - 1) / kRows;
-        const int piece = (at - start) / sh.each, h = piece / sh.tiles, tile = piece % sh.tiles, first_unit = (at - start) % sh.each;
-        const int last_unit = min(sh.each, first_unit + (u1 - at)), p0 = first_unit * p.unit;
-        const bool from_start = first_unit == 0, to_end = last_unit == sh.each;
-        at += last_unit - first_unit;
-        const int mine = max(0, min(last_unit * p.unit, pages) - p0 - warp + kWarps - 1) / kWarps;      // of the pages from p0 on
-        int lane_page = -1;
-        uint32_t there = 0;                                                      // bit per stage: its page is one of the pool's
-        auto request = [&](int i) {
-            if ((i & 31) == 0) {
-                const int col = p0 + warp + kWarps * (i + lane);
-                const bool in = i + lane < mine;
-                lane_page = in ? c.page_table[(size_t)b * c.max_pages + col] : -1;
-                if ((unsigned)lane_page >= (unsigned)c.n_pages) { if (in) raise(c, kBadPage); lane_page = -1; }
+    // one piece after the other: pages of a (sequence, kv head, tile of rows)
+    struct Piece { Entry e; int b, h, tile, p0, mine; bool from_start, to_end; };
+    auto next_piece = [&]() {
+        Share sh;
+        while (u >= start + (sh = share_of<R>(c, p, b, group)).units) { start += sh.units; ++b; }
+        Piece x;
+        x.b = b;
+        x.e = entry_of(c, p, b);
+        const int i = (u - start) / sh.each, first = (u - start) - i * sh.each, last = min(sh.each, first + (u1 - u));
+        x.h = i / sh.tiles;
+        x.tile = i - x.h * sh.tiles;
+        x.p0 = first * p.unit;
+        x.mine = max(0, min(last * p.unit, (x.e.len + kRows - 1) / kRows) - x.p0);
+        x.from_start = first == 0;
+        x.to_end = last == sh.each;
+        u += last - first;
+        return x;
+    };
+    auto row_at = [&](const Piece& x, int row) { return ((size_t)(x.e.row0 + row / group) * c.q_heads + x.h * group + row % group) * D; };
+    int lane_page = -1;
+    uint32_t there = 0;                                                          // bit per stage: its page is one of the pool's
+    auto request = [&](const Piece& x, int i) {
+        if ((i & 31) == 0) {                                                     // a lane knows one page of 32
+            const bool in = i + lane < x.mine;
+            lane_page = in ? c.page_table[(size_t)x.b * c.max_pages + x.p0 + i + lane] : -1;
+            if ((unsigned)lane_page >= (unsigned)c.n_pages) { if (in) raise(c, kBadPage); lane_page = -1; }
+        }
+        const int page = __shfl_sync(0xffffffffu, lane_page, i & 31), st = (slot + i) % C::STAGES;
+        there = page >= 0 ? there | 1u << st : there & ~(1u << st);
+        if (lane == 0) {
+            if (page >= 0) {
+                tc::mbar_expect_tx(bar0 + 8 * st, L::BYTES);
+                bulk_copy(tc::smem_u32(ring) + st * L::BYTES, tile_of<D>(c, page, x.h), L::BYTES, bar0 + 8 * st);
+            } else {
+                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar0 + 8 * st) : "memory");
             }
-            const int page = __shfl_sync(0xffffffffu, lane_page, i & 31), st = (slot + i) % C::STAGES;
-            there = page >= 0 ? there | 1u << st : there & ~(1u << st);
-            if (lane == 0) {
-                if (page >= 0) {
-                    tc::mbar_expect_tx(bar0 + 8 * st, L::BYTES);
-                    bulk_copy(tc::smem_u32(ring) + st * L::BYTES, tile_of<D>(c, page, h), L::BYTES, bar0 + 8 * st);
-                } else {
-                    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar0 + 8 * st) : "memory");
-                }
-            }
-        };
-        for (int i = 0; i < min(mine, C::STAGES); ++i) request(i);
-
-        QueryTile<D> q[NT];
-        int see[NT][2], least = INT32_MAX;                                       // cached rows that the lane's columns see
+        }
+    };
+    typename QueryTile<D>::Raw raw[NT];
+    auto ask = [&](const Piece& x) {                                             // queries ahead of the pages, which they would queue behind
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const int row = tile * R + t * 8 + r;
-            q[t].load((const T*)p.q + ((size_t)(e.row0 + row / group) * c.q_heads + h * group + row % group) * D, row < rows, p.scale_log2);
+            const int row = x.tile * R + t * 8 + r;
+            const bool have = row < x.e.n * group;
+            raw[t] = QueryTile<D>::fetch((const T*)p.q + (have ? row_at(x, row) : 0), have);
+        }
+        for (int i = 0; i < min(x.mine, C::STAGES); ++i) request(x, i);
+    };
+    Piece x = next_piece();
+    ask(x);
+    for (bool more = true; more;) {
+        QueryTile<D> q[NT];
+        int see[NT][2], least = INT32_MAX;                                       // cached rows that the lane's columns see
+        const int rows = x.e.n * group;                                          // packed: new row x head of the group
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            q[t].template take<T>(raw[t], p.scale_log2);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const int cr = tile * R + t * 8 + 2 * j + k;
-                see[t][k] = cr < rows ? max(0, min(e.len, e.len - e.n + cr / group + 1)) : 0;
+                const int cr = x.tile * R + t * 8 + 2 * j + k;
+                see[t][k] = cr < rows ? max(0, min(x.e.len, x.e.len - x.e.n + cr / group + 1)) : 0;
                 if (cr < rows) least = min(least, see[t][k]);
             }
         }
@@ -374,19 +412,27 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
+            for (int y = 0; y < 4; ++y)
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) o[g][x][t][k] = 0.f;
+                    for (int k = 0; k < 4; ++k) o[g][y][t][k] = 0.f;
         int ev = -40;                                                            // exponent of the largest value scale seen
 
-        for (int i = 0; i < mine; ++i) {
-            const int st = (slot + i) % C::STAGES, first = (p0 + warp + kWarps * i) * kRows;
-            if (!warp_wait(bar0 + 8 * st, (uint32_t)((slot + i) / C::STAGES) & 1u, abort_s)) { *abort_s = 1; break; }
+        for (int i = 0; i < x.mine; ++i) {
+            const int st = (slot + i) % C::STAGES, first = (x.p0 + i) * kRows;
+            if (!warp_wait(bar0 + 8 * st, (uint32_t)((slot + i) / C::STAGES) & 1u, abort_s)) {      // given up: copies in flight land first (bounded)
+                *abort_s = 1;
+                if (lane == 0) {
+                    volatile int go_on = 0;
+                    for (int k = 0; k < C::STAGES; ++k) { (void)tc::mbar_wait(bar0 + 8 * k, 0, &go_on); (void)tc::mbar_wait(bar0 + 8 * k, 1, &go_on); }
+                    raise(c, kWait);
+                }
+                return;
+            }
             if (there >> st & 1u) {
                 uint8_t* page = ring + (size_t)st * L::BYTES;
-                if (e.len - first < kRows) clear_rows<D>(page, e.len - first, true);
+                if (x.e.len - first < kRows) clear_rows<D>(page, x.e.len - first, true);
                 float s[4][NT][4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) score_tile<D, NT>(page, u, q, s[u]);
@@ -400,7 +446,7 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
                                 if (first + u * 16 + token_of(r) + 8 * (k >> 1) >= see[t][k & 1]) s[u][t][k] = -INFINITY;
                 }
                 if (p.scores != nullptr) {
-                    float* to = p.scores + ((size_t)b * c.kv_heads + h) * R * p.score_ld + first + token_of(r);
+                    float* to = p.scores + ((size_t)x.b * c.kv_heads + x.h) * R * p.score_ld + first + token_of(r);
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -469,7 +515,7 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
                             for (int g = 0; g < G; ++g) {
                                 pc[g][t][k] *= alpha;
 #pragma unroll
-                                for (int x = 0; x < 4; ++x) { o[g][x][t][k] *= f; o[g][x][t][2 + k] *= f; }
+                                for (int y = 0; y < 4; ++y) { o[g][y][t][k] *= f; o[g][y][t][2 + k] *= f; }
                             }
                         }
                     ev = en;
@@ -510,9 +556,9 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
                         const uint32_t w0 = codes[g * 8], w1 = codes[4 * L::WORDS + g * 8], w2 = codes[8 * L::WORDS + g * 8], w3 = codes[12 * L::WORDS + g * 8];
 #pragma unroll
                         for (int hl = 0; hl < 2; ++hl) {
-                            const uint32_t x = __byte_perm(w0, w1, hl ? 0x7632 : 0x5410), y = __byte_perm(w2, w3, hl ? 0x7632 : 0x5410);
-                            const uint32_t a0[4] = {low_pair(x), high_pair(x), low_pair(y), high_pair(y)};
-                            const uint32_t a1[4] = {low_pair(x >> 8), high_pair(x >> 8), low_pair(y >> 8), high_pair(y >> 8)};
+                            const uint32_t ta = __byte_perm(w0, w1, hl ? 0x7632 : 0x5410), tb = __byte_perm(w2, w3, hl ? 0x7632 : 0x5410);
+                            const uint32_t a0[4] = {low_pair(ta), high_pair(ta), low_pair(tb), high_pair(tb)};
+                            const uint32_t a1[4] = {low_pair(ta >> 8), high_pair(ta >> 8), low_pair(tb >> 8), high_pair(tb >> 8)};
 #pragma unroll
                             for (int t = 0; t < NT; ++t) {
                                 mma16816(o[g][2 * hl][t], a0, b0[g][t], b1[g][t]);
@@ -523,13 +569,16 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
                 }
             }
             __syncwarp();                                                        // every lane has read the page
-            if (i + C::STAGES < mine) request(i + C::STAGES);
+            if (i + C::STAGES < x.mine) request(x, i + C::STAGES);
         }
-        if (*abort_s != 0 && lane == 0)                                          // given up: let the copies in flight land (bounded)
-            for (int i = 0; i < C::STAGES; ++i) { volatile int go_on = 0; (void)tc::mbar_wait(bar0 + 8 * i, 0, &go_on); (void)tc::mbar_wait(bar0 + 8 * i, 1, &go_on); }
-        slot += mine;
+        slot += x.mine;
+        const Piece done = x;
+        more = u < u1;
+        if (more) {                                                              // the next piece is on its way while this one is written
+            x = next_piece();
+            ask(x);
+        }
 
-        // the warps' results: maxima first, then values relative to the block's
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1)
 #pragma unroll
@@ -540,119 +589,87 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
 #pragma unroll
                     for (int g = 0; g < G; ++g) pc[g][t][k] += __shfl_xor_sync(0xffffffffu, pc[g][t][k], off);
                 }
-        if (r == 0)
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) ml_s[warp * R + t * 8 + 2 * j + k] = make_float2(m[t][k], l[t][k]);
-        __syncthreads();
-        if (*abort_s != 0) { if (threadIdx.x == 0) raise(c, kWait); return; }
-        float* merge = reinterpret_cast<float*>(smem);
         const float back = __uint_as_float((uint32_t)(127 + ev - 14) << 23);
+        const bool alone = done.from_start && done.to_end;
+        const int piece = 2 * me + (done.from_start ? 1 : 0);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const int rr = t * 8 + 2 * j + k;
-                float top = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml_s[w * R + rr].x);
-                const float f = m[t][k] == -INFINITY ? 0.f : ex2f(m[t][k] - top);
-                float* dst = merge + ((size_t)warp * R + rr) * C::LD + 8 * r;
+                const int rr = t * 8 + 2 * j + k, row = done.tile * R + rr;
+                if (row >= rows) continue;
+                const float inv = alone ? (l[t][k] > 0.f ? 1.0f / l[t][k] : l[t][k] != l[t][k] ? l[t][k] : 0.f) : 1.0f;
+                const size_t at = row_at(done, row);
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
                     float v[8];                                                  // channels of word r of the group, see the nibbles' order
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const int ch = (x & 1) * 4 + (x >> 1);
-                        v[ch] = fmaf(o[g][x][t][k], back, pc[g][t][k]) * f;
-                        v[ch + 2] = fmaf(o[g][x][t][2 + k], back, pc[g][t][k]) * f;
+                    for (int y = 0; y < 4; ++y) {
+                        const int ch = (y & 1) * 4 + (y >> 1);
+                        v[ch] = fmaf(o[g][y][t][k], back, pc[g][t][k]) * inv;
+                        v[ch + 2] = fmaf(o[g][y][t][2 + k], back, pc[g][t][k]) * inv;
                     }
-                    *reinterpret_cast<float4*>(dst + g * 64) = make_float4(v[0], v[1], v[2], v[3]);
-                    *reinterpret_cast<float4*>(dst + g * 64 + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                    if (alone) {
+                        *reinterpret_cast<uint4*>((T*)p.out + at + g * 64 + 8 * r) = make_uint4(Num<T>::pack(v[0], v[1]), Num<T>::pack(v[2], v[3]), Num<T>::pack(v[4], v[5]), Num<T>::pack(v[6], v[7]));
+                    } else {
+                        float4* dst = reinterpret_cast<float4*>(p.part + ((size_t)piece * R + rr) * D + g * 64 + 8 * r);
+                        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+                        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+                    }
+                }
+                if (r == 0) {
+                    if (!alone) p.part_stats[(size_t)rr * 2 * p.warps + piece] = make_float2(m[t][k], l[t][k]);
+                    else if (p.stats != nullptr) p.stats[stat_row(c, p, done.b, row / group, done.h * group + row % group)] = make_float2(m[t][k], l[t][k]);
                 }
             }
-        __syncthreads();
-        const bool alone = from_start && to_end;
-        const size_t piece_row = ((size_t)2 * blockIdx.x + (from_start ? 1 : 0)) * R;
-        for (int i = threadIdx.x; i < R * (D / 4); i += kWarps * 32) {
-            const int rr = i / (D / 4), d = i % (D / 4) * 4, row = tile * R + rr;
-            if (row >= rows) continue;
-            float top = -INFINITY, sum = 0.f;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml_s[w * R + rr].x);
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float2 ml = ml_s[w * R + rr];
-                if (ml.x != -INFINITY) sum = fmaf(ml.y, ex2f(ml.x - top), sum);
-                const float4 x = *reinterpret_cast<const float4*>(merge + ((size_t)w * R + rr) * C::LD + d);
-                v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-            }
-            const int head = h * group + row % group;
-            if (alone) {
-                const float inv = sum > 0.f ? 1.0f / sum : 0.f;
-                T* dst = (T*)p.out + ((size_t)(e.row0 + row / group) * c.q_heads + head) * D + d;
-                *reinterpret_cast<uint2*>(dst) = make_uint2(Num<T>::pack(v.x * inv, v.y * inv), Num<T>::pack(v.z * inv, v.w * inv));
-                if (p.stats != nullptr && d == 0) p.stats[stat_row(c, p, b, row / group, head)] = make_float2(top, sum);
-            } else {
-                *reinterpret_cast<float4*>(p.part + (piece_row + rr) * D + d) = v;
-                if (d == 0) p.part_stats[piece_row + rr] = make_float2(top, sum);
-            }
-        }
-        if (at < u1) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");         // the merge is over ahead of copies into the rings
-            __syncthreads();
-        }
     }
 }
 
-// Where the keys of a tile of packed rows were dealt: to one block, which finished the rows itself, or to blocks [w0, w1].
+// Where the keys of a tile of packed rows were dealt: to one warp, which finished the rows itself, or to warps [w0, w1].
 struct Pieces { int w0, w1; };
 __device__ __forceinline__ Pieces pieces_of(const AttnParams& p, const Share& s, const Deal& d, int h, int tile) {
     const int step = step_of(p, d.all), at = d.before + (h * s.tiles + tile) * s.each;
     return Pieces{at / step, (at + s.each - 1) / step};
 }
-__device__ __forceinline__ size_t piece_row(int w, const Pieces& x, int R, int rr) { return ((size_t)2 * w + (w == x.w0 ? 1 : 0)) * R + rr; }
+__device__ __forceinline__ int piece_of(int w, const Pieces& x) { return 2 * w + (w == x.w0 ? 1 : 0); }
 
 // Maximum and sum of packed row rr of a tile over its pieces, by a warp.
-__device__ __forceinline__ float2 merged_stats(const AttnParams& p, const Pieces& x, int R, int rr) {
+__device__ __forceinline__ float2 merged_stats(const AttnParams& p, const Pieces& x, int rr) {
     const int lane = threadIdx.x & 31;
     float top = -INFINITY, sum = 0.f;
-    for (int w = x.w0 + lane; w <= x.w1; w += 32) {
-        const float2 s = p.part_stats[piece_row(w, x, R, rr)];
-        const float mx = fmaxf(top, s.x);
-        if (mx != -INFINITY) sum = (top == -INFINITY ? 0.f : sum * ex2f(top - mx)) + (s.x == -INFINITY ? 0.f : s.y * ex2f(s.x - mx));
+    for (int base = x.w0; base <= x.w1; base += 256) {           // 256 pieces on their way at a time
+        float2 s[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int w = base + k * 32 + lane;
+            s[k] = w <= x.w1 ? p.part_stats[(size_t)rr * 2 * p.warps + piece_of(w, x)] : make_float2(-INFINITY, 0.f);
+        }
+        float mx = top;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mx = fmaxf(mx, s[k].x);
+        if (mx == -INFINITY) continue;
+        sum = top == -INFINITY ? 0.f : sum * ex2f(top - mx);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) if (s[k].x != -INFINITY) sum = fmaf(s[k].y, ex2f(s[k].x - mx), sum);
         top = mx;
     }
     const float all = warp_max(top);
     return make_float2(all, warp_sum(top == -INFINITY ? 0.f : sum * ex2f(top - all)));
 }
 
+constexpr int kFactors = 512;         // pieces whose factors are at hand at a time
 constexpr int kMassTokens = 512;      // cached rows of a block that sums weights from scores
 
 // What needs the whole row.  grid (mass blocks + merging blocks, kv heads, batch): merging blocks join the pieces of rows that attend_few
-// dealt over several blocks, a row at a time; mass blocks sum the weights of 512 cached rows from the scores it left.
+// dealt over several warps, 32 channels of a row at a time; mass blocks sum the weights of 512 cached rows from the scores it left.
 template <typename T, int D, int R>
 __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c, const AttnParams p, int mass_blocks) {
-    __shared__ int sums[2][kWarps];
     __shared__ float2 st_s[R];
     __shared__ float4 v_s[kWarps * 32];
+    __shared__ float f_s[kFactors];
     const int h = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = c.q_heads / c.kv_heads;
     pdl_launch_dependents();
-    // lengths are not attend_few's to write: where the units lie is known before the wait
-    int before = 0, all = 0;
-    for (int i = threadIdx.x; i < c.batch; i += kWarps * 32) {
-        const int n = share_of<R>(c, p, i, group).units;
-        all += n;
-        if (i < b) before += n;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) { all += __shfl_xor_sync(0xffffffffu, all, o); before += __shfl_xor_sync(0xffffffffu, before, o); }
-    if (lane == 0) { sums[0][warp] = before; sums[1][warp] = all; }
-    __syncthreads();
-    Deal deal{0, 0};
-    for (int w = 0; w < kWarps; ++w) { deal.before += sums[0][w]; deal.all += sums[1][w]; }
+    // lengths are not attend_few's to write
     const Entry e = entry_of(c, p, b);
     const Share sh = share_of<R>(c, p, b, group);
     const int rows = sh.tiles > 0 ? e.n * group : 0;
@@ -660,9 +677,9 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
         const int t0 = blockIdx.x * kMassTokens;
         pdl_wait();
         if (t0 >= e.len) return;
-        const Pieces x = rows > 0 ? pieces_of(p, sh, deal, h, 0) : Pieces{0, 0};
+        const Pieces x = rows > 0 ? pieces_of(p, sh, Deal{p.starts[b], p.starts[c.batch]}, h, 0) : Pieces{0, 0};
         for (int row = warp; row < rows; row += kWarps) {
-            const float2 s = x.w0 == x.w1 ? p.stats[stat_row(c, p, b, row / group, h * group + row % group)] : merged_stats(p, x, R, row);
+            const float2 s = x.w0 == x.w1 ? p.stats[stat_row(c, p, b, row / group, h * group + row % group)] : merged_stats(p, x, row);
             if (lane == 0) st_s[row] = s.x == -INFINITY ? make_float2(0.f, 0.f) : make_float2(s.x, 1.0f / s.y);
         }
         __syncthreads();
@@ -671,11 +688,18 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
         const float* from = p.scores + ((size_t)b * c.kv_heads + h) * R * p.score_ld + t0 + threadIdx.x;
 #pragma unroll
         for (int k = 0; k < PER; ++k) w[k] = 0.f;
-        for (int row = 0; row < rows; ++row) {
-            const float2 s = st_s[row];
+        for (int row = 0; row < rows; row += 4) {                // four rows' scores on their way at a time
+            float s[4][PER];
 #pragma unroll
-            for (int k = 0; k < PER; ++k)
-                if (t0 + (int)threadIdx.x + k * kWarps * 32 < e.len) w[k] = fmaf(ex2f(from[row * p.score_ld + k * kWarps * 32] - s.x), s.y, w[k]);
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int k = 0; k < PER; ++k) s[i][k] = row + i < rows && t0 + (int)threadIdx.x + k * kWarps * 32 < e.len ? from[(row + i) * p.score_ld + k * kWarps * 32] : -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 st = st_s[min(row + i, rows - 1)];
+#pragma unroll
+                for (int k = 0; k < PER; ++k) w[k] = fmaf(ex2f(s[i][k] - st.x), st.y, w[k]);
+            }
         }
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
@@ -688,28 +712,83 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
         return;
     }
     pdl_wait();
-    for (int row = (int)blockIdx.x - mass_blocks; row < rows; row += (int)gridDim.x - mass_blocks) {
+    if (rows == 0) return;
+    const Deal deal{p.starts[b], p.starts[c.batch]};
+    const int first = (int)blockIdx.x - mass_blocks, blocks = (int)gridDim.x - mass_blocks;
+    constexpr int SLICES = D / 32, Q = 8, LANES = kWarps * 32 / Q;               // threads side by side, each with four channels of every LANES-th piece
+    // few pieces, or more rows than there are blocks for: a row a warp, no barriers
+    if (sh.each <= (blocks < rows * SLICES ? 64 : 12) * step_of(p, deal.all)) {
+        for (int row = first * kWarps + warp; row < rows; row += blocks * kWarps) {
+            const Pieces x = pieces_of(p, sh, deal, h, row / R);
+            if (x.w0 == x.w1) continue;
+            const int i = row / group, head = h * group + row % group, rr = row % R;
+            const float2 st = merged_stats(p, x, rr);
+            const float inv = st.y > 0.f ? 1.0f / st.y : st.y != st.y ? st.y : 0.f;
+            constexpr int E = D / 32;
+            float v[E];
+#pragma unroll
+            for (int k = 0; k < E; ++k) v[k] = 0.f;
+            for (int w0 = x.w0; w0 <= x.w1; w0 += 6) {
+                float2 y[6][E / 2];
+                float f[6];
+#pragma unroll
+                for (int s = 0; s < 6; ++s) {
+                    const bool in = w0 + s <= x.w1;
+                    const int piece = piece_of(w0 + s, x);
+                    f[s] = in ? p.part_stats[(size_t)rr * 2 * p.warps + piece].x : -INFINITY;
+#pragma unroll
+                    for (int k = 0; k < E / 2; ++k) y[s][k] = in ? *reinterpret_cast<const float2*>(p.part + ((size_t)piece * R + rr) * D + lane * E + 2 * k) : make_float2(0.f, 0.f);
+                }
+#pragma unroll
+                for (int s = 0; s < 6; ++s) {
+                    const float a = f[s] == -INFINITY ? 0.f : ex2f(f[s] - st.x);
+#pragma unroll
+                    for (int k = 0; k < E / 2; ++k) { v[2 * k] = fmaf(y[s][k].x, a, v[2 * k]); v[2 * k + 1] = fmaf(y[s][k].y, a, v[2 * k + 1]); }
+                }
+            }
+            T* dst = (T*)p.out + ((size_t)(e.row0 + i) * c.q_heads + head) * D + lane * E;
+#pragma unroll
+            for (int k = 0; k < E; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = Num<T>::pack(v[k] * inv, v[k + 1] * inv);
+            if (lane == 0 && p.stats != nullptr && mass_blocks == 0) p.stats[stat_row(c, p, b, i, head)] = st;
+        }
+        return;
+    }
+    for (int job = first; job < rows * SLICES; job += blocks) {
+        const int row = job / SLICES, d = job % SLICES * 32 + threadIdx.x % Q * 4;
         const Pieces x = pieces_of(p, sh, deal, h, row / R);
         if (x.w0 == x.w1) continue;
         const int i = row / group, head = h * group + row % group, rr = row % R;
-        const float2 st = merged_stats(p, x, R, rr);
-        constexpr int Q = D / 4, LANES = kWarps * 32 / Q;        // threads side by side, each with four channels of every LANES-th piece
-        const int d = threadIdx.x % Q * 4;
+        // every piece's factor once, in rounds of what fits
+        const float2 st = merged_stats(p, x, rr);
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int w = x.w0 + threadIdx.x / Q; w <= x.w1; w += LANES) {
-            const size_t at = piece_row(w, x, R, rr);
-            const float m = p.part_stats[at].x, f = m == -INFINITY ? 0.f : ex2f(m - st.x);
-            const float4 y = *reinterpret_cast<const float4*>(p.part + at * D + d);
-            v.x = fmaf(y.x, f, v.x); v.y = fmaf(y.y, f, v.y); v.z = fmaf(y.z, f, v.z); v.w = fmaf(y.w, f, v.w);
+        for (int base = x.w0; base <= x.w1; base += kFactors) {
+            const int n = min(kFactors, x.w1 + 1 - base);
+            __syncthreads();
+            for (int k = threadIdx.x; k < n; k += kWarps * 32) {
+                const float m = p.part_stats[(size_t)rr * 2 * p.warps + piece_of(base + k, x)].x;
+                f_s[k] = m == -INFINITY ? 0.f : ex2f(m - st.x);
+            }
+            __syncthreads();
+            for (int k0 = threadIdx.x / Q; k0 < n; k0 += 8 * LANES) {            // eight loads on their way at a time
+                float4 y[8];
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int k = k0 + i * LANES;
+                    f[i] = k < n ? f_s[k] : 0.f;
+                    y[i] = k < n ? *reinterpret_cast<const float4*>(p.part + ((size_t)piece_of(base + k, x) * R + rr) * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { v.x = fmaf(y[i].x, f[i], v.x); v.y = fmaf(y[i].y, f[i], v.y); v.z = fmaf(y[i].z, f[i], v.z); v.w = fmaf(y[i].w, f[i], v.w); }
+            }
         }
         v_s[threadIdx.x] = v;
         __syncthreads();
         if ((int)threadIdx.x < Q) {
             for (int k = 1; k < LANES; ++k) { const float4 y = v_s[k * Q + threadIdx.x]; v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w; }
-            const float inv = st.y > 0.f ? 1.0f / st.y : 0.f;
+            const float inv = st.y > 0.f ? 1.0f / st.y : st.y != st.y ? st.y : 0.f;
             *reinterpret_cast<uint2*>((T*)p.out + ((size_t)(e.row0 + i) * c.q_heads + head) * D + d) = make_uint2(Num<T>::pack(v.x * inv, v.y * inv), Num<T>::pack(v.z * inv, v.w * inv));
-            if (threadIdx.x == 0 && p.stats != nullptr && mass_blocks == 0) p.stats[stat_row(c, p, b, i, head)] = st;
+            if (threadIdx.x == 0 && d == 0 && p.stats != nullptr && mass_blocks == 0) p.stats[stat_row(c, p, b, i, head)] = st;
         }
         __syncthreads();
     }
