@@ -136,7 +136,7 @@ efm_status check_attention(const char* call, const efm_kv4_cache* c, const efm_k
 
 // What a call needs: tiles of 8 nt packed query rows, and the parts of its workspace, in floats.
 struct AttnPlan {
-    int max_new, max_len, nt, blocks, unit, few_rows, many_tiles;      // many_tiles: blocks of 256 packed rows a sequence may have
+    int max_new, max_len, nt, blocks, unit_shift, few_rows, many_tiles;      // many_tiles: blocks of 256 packed rows a sequence may have
     bool joined;                                      // pieces of a row may lie in several blocks
     bool scores;                                      // attend_few leaves its scores for the summed weights
     int64_t units, stats, part_stats, part, score_ld, score, image, image_units, starts;
@@ -144,7 +144,7 @@ struct AttnPlan {
     int64_t bytes() const { return 4 * (stats + part_stats + part + score + image + image_units + starts); }
 };
 constexpr int kSms = 148;                              // of the GPU these kernels are built for
-constexpr int kWholePages = 4;
+constexpr int kWholeShift = 2;
 constexpr int kFewRows = 32;                           // packed rows of a sequence up to which attend_few takes it
 
 AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
@@ -157,10 +157,10 @@ AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
     p.many_tiles = rows > p.few_rows ? (int)((rows + 2 * kv4::kTileRows - 1) / (2 * kv4::kTileRows)) : 0;
     const int64_t R = 8 * p.nt, tiles = (std::min<int64_t>(rows, p.few_rows) + R - 1) / R, pages = std::max(1, (p.max_len + kRows - 1) / kRows);
     // a page at a time, or caches of up to four pages whole: nothing is left to join then, which saves the smallest calls a launch
-    p.unit = pages <= kWholePages ? kWholePages : 1;
-    p.units = (pages + p.unit - 1) / p.unit * tiles * c->kv_heads * c->batch;
+    p.unit_shift = pages <= 1 << kWholeShift ? kWholeShift : 0;
+    p.units = (pages + (1 << p.unit_shift) - 1 >> p.unit_shift) * tiles * c->kv_heads * c->batch;
     p.blocks = (int)std::max<int64_t>(1, std::min<int64_t>(kSms * (p.nt == 1 ? 3 : 2), (p.units + kv4::kWarps - 1) / kv4::kWarps));
-    p.joined = pages > p.unit;
+    p.joined = pages > 1 << p.unit_shift;
     p.scores = a->mass_out != nullptr && rows <= R;
     p.stats = a->mass_out != nullptr ? round_up(2 * (int64_t)c->batch * p.max_new * c->q_heads, 4) : 0;
     const int64_t pieces = p.joined ? 2 * (int64_t)p.blocks * kv4::kWarps * R : 0;      // two a warp: the one it begins in and the one it ends in
@@ -308,7 +308,7 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
         p.cu_rows = a->cu_rows; p.lens = a->lens; p.q = a->q; p.out = a->out;
         p.scale_log2 = a->scale * 1.4426950408889634f;
         p.mass_in = a->mass_in; p.mass_out = a->mass_out;
-        p.few_rows = plan.few_rows; p.warps = plan.blocks * kv4::kWarps; p.unit = plan.unit; p.rows = plan.max_new;
+        p.few_rows = plan.few_rows; p.warps = plan.blocks * kv4::kWarps; p.unit_shift = plan.unit_shift; p.group_inv = (65536 + cache->q_heads / cache->kv_heads - 1) / (cache->q_heads / cache->kv_heads); p.rows = plan.max_new;
         float* ws = (float*)a->workspace;
         p.stats = plan.stats > 0 ? (float2*)ws : nullptr;
         p.part_stats = (float2*)(ws + plan.stats);

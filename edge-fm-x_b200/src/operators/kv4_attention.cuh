@@ -21,7 +21,8 @@ struct AttnParams {
     const float* mass_in;
     float* mass_out;
     int few_rows;             // sequences with at most this many packed rows (new rows x heads of a group) are attend_few's
-    int warps, unit;          // attend_few's warps; pages of a unit of work
+    int warps, unit_shift;    // attend_few's warps; pages of a unit of work: 1 << unit_shift
+    uint32_t group_inv;       // ceil(2^16 / heads of a group): packed rows below 2^8 are divided by it
     float2* stats;            // [batch, rows, q_heads] (maximum, sum) of a row's weights, where one warp had all its keys; null: not wanted
     int rows;                 // new rows a sequence has in stats
     float2* part_stats;       // [8 nt][2 warps] the same of the keys a warp had, and
@@ -79,11 +80,10 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar) {
 struct Deal { int before, all; };          // units ahead of sequence b, and altogether
 struct Share { int units, tiles, each; };      // of a sequence; row tiles; units of a tile and head
 template <int R>
-__device__ __forceinline__ Share share_of(const Cache& c, const AttnParams& p, int b, int group) {
-    const Entry e = entry_of(c, p, b);
+__device__ __forceinline__ Share share_of(const Cache& c, const AttnParams& p, const Entry& e, int group) {
     const int rows = e.n * group;
     Share s;
-    s.each = max(1, ((e.len + kRows - 1) / kRows + p.unit - 1) / p.unit);        // a row that sees nothing is somebody's to clear
+    s.each = max(1, ((e.len + kRows - 1) / kRows + (1 << p.unit_shift) - 1) >> p.unit_shift);      // a row that sees nothing is somebody's to clear
     s.tiles = rows <= p.few_rows ? (rows + R - 1) / R : 0;
     s.units = s.tiles * s.each * c.kv_heads;
     return s;
@@ -284,6 +284,7 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
     constexpr int G = L::G, R = 8 * NT;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int sums[kWarps], before_s[kWarps], first_s[kWarps];
+    __shared__ Entry entry_s[kWarps];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::RING);
     volatile int* abort_s = reinterpret_cast<volatile int*>(bars + kWarps * C::STAGES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3, group = c.q_heads / c.kv_heads;
@@ -297,61 +298,74 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
     pdl_wait();
     pdl_launch_dependents();
     // the warps' ranges of the units, and the sequences they begin in
-    const int per = (c.batch + kWarps * 32 - 1) / (kWarps * 32), b_lo = min(c.batch, (int)threadIdx.x * per), b_hi = min(c.batch, b_lo + per);
-    int own = 0;
-    for (int b = b_lo; b < b_hi; ++b) own += share_of<R>(c, p, b, group).units;
-    int upto = own;
+    const int me = blockIdx.x * kWarps + warp;
+    int all = 0, b = 0, start = 0;                                               // b: sequence, start: unit that it begins with
+    Entry e0;
+    if (c.batch == 1) {
+        e0 = entry_of(c, p, 0);
+        all = share_of<R>(c, p, e0, group).units;
+        if (blockIdx.x == 0 && threadIdx.x == 0) { p.starts[0] = 0; p.starts[1] = all; }      // for attend_merge
+        __syncthreads();                                                         // barriers and the abort word are set up
+    } else {
+        const int per = (c.batch + kWarps * 32 - 1) / (kWarps * 32), b_lo = min(c.batch, (int)threadIdx.x * per), b_hi = min(c.batch, b_lo + per);
+        int own = 0;
+        for (int i = b_lo; i < b_hi; ++i) own += share_of<R>(c, p, e0 = entry_of(c, p, i), group).units;
+        int upto = own;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
-    }
-    if (lane == 31) sums[warp] = upto;
-    __syncthreads();
-    int all = 0;
-    for (int w = 0; w < kWarps; ++w) { if (w < warp) upto += sums[w]; all += sums[w]; }
-    if (blockIdx.x == 0) {                                                       // for attend_merge
-        if (threadIdx.x == 0) p.starts[c.batch] = all;
-        int at = upto - own;
-        for (int b = b_lo; b < b_hi; ++b) { p.starts[b] = at; at += share_of<R>(c, p, b, group).units; }
-    }
-    const int step = step_of(p, all);
-    auto begins = [&](int w) { return (int)min((int64_t)all, (int64_t)w * step); };
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        const int u = begins(blockIdx.x * kWarps + w);
-        if (upto - own <= u && u < upto) {
-            int at = upto - own, b = b_lo;
-            for (int n; at + (n = share_of<R>(c, p, b, group).units) <= u; ++b) at += n;
-            first_s[w] = b;
-            before_s[w] = at;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
         }
+        if (lane == 31) sums[warp] = upto;
+        __syncthreads();
+        for (int w = 0; w < kWarps; ++w) { if (w < warp) upto += sums[w]; all += sums[w]; }
+        const int step = step_of(p, all);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const int u = (int)min((int64_t)all, ((int64_t)blockIdx.x * kWarps + w) * step);
+            if (upto - own <= u && u < upto) {
+                int at = upto - own, i = b_lo;
+                if (per > 1)
+                    for (int n; at + (n = share_of<R>(c, p, e0 = entry_of(c, p, i), group).units) <= u; ++i) at += n;
+                first_s[w] = i;
+                before_s[w] = at;
+                entry_s[w] = e0;
+            }
+        }
+        if (blockIdx.x == 0) {
+            if (threadIdx.x == 0) p.starts[c.batch] = all;
+            int at = upto - own;
+            for (int i = b_lo; i < b_hi; ++i) { p.starts[i] = at; at += share_of<R>(c, p, entry_of(c, p, i), group).units; }
+        }
+        __syncthreads();
+        b = first_s[warp];
+        start = before_s[warp];
+        e0 = entry_s[warp];
     }
-    __syncthreads();
-    const int me = blockIdx.x * kWarps + warp, u1 = begins(me + 1);
-    int u = begins(me), slot = 0;                                                // slot: of the copies and their barriers
+    const int step = step_of(p, all), u1 = (int)min((int64_t)all, ((int64_t)me + 1) * step);
+    int u = (int)min((int64_t)all, (int64_t)me * step), slot = 0;                // slot: of the copies and their barriers
     if (u >= u1) return;
-    int b = first_s[warp], start = before_s[warp];                               // start: unit that sequence b begins with
+    auto by_group = [&](int row) { return (int)((uint32_t)row * p.group_inv >> 16); };       // row / group
 
     // one piece after the other: pages of a (sequence, kv head, tile of rows)
     struct Piece { Entry e; int b, h, tile, p0, mine; bool from_start, to_end; };
     auto next_piece = [&]() {
-        Share sh;
-        while (u >= start + (sh = share_of<R>(c, p, b, group)).units) { start += sh.units; ++b; }
+        Share sh = share_of<R>(c, p, e0, group);
+        while (u >= start + sh.units) { start += sh.units; sh = share_of<R>(c, p, e0 = entry_of(c, p, ++b), group); }
         Piece x;
         x.b = b;
-        x.e = entry_of(c, p, b);
-        const int i = (u - start) / sh.each, first = (u - start) - i * sh.each, last = min(sh.each, first + (u1 - u));
-        x.h = i / sh.tiles;
+        x.e = e0;
+        const int in = u - start, i = in / sh.each, first = in - i * sh.each, last = min(sh.each, first + (u1 - u));
+        x.h = sh.tiles == 1 ? i : i / sh.tiles;
         x.tile = i - x.h * sh.tiles;
-        x.p0 = first * p.unit;
-        x.mine = max(0, min(last * p.unit, (x.e.len + kRows - 1) / kRows) - x.p0);
+        x.p0 = first << p.unit_shift;
+        x.mine = max(0, min(last << p.unit_shift, (x.e.len + kRows - 1) / kRows) - x.p0);
         x.from_start = first == 0;
         x.to_end = last == sh.each;
         u += last - first;
         return x;
     };
-    auto row_at = [&](const Piece& x, int row) { return ((size_t)(x.e.row0 + row / group) * c.q_heads + x.h * group + row % group) * D; };
+    auto row_at = [&](const Piece& x, int row) { return ((size_t)(x.e.row0 + by_group(row)) * c.q_heads + x.h * group + row - by_group(row) * group) * D; };
     int lane_page = -1;
     uint32_t there = 0;                                                          // bit per stage: its page is one of the pool's
     auto request = [&](const Piece& x, int i) {
@@ -393,7 +407,7 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const int cr = x.tile * R + t * 8 + 2 * j + k;
-                see[t][k] = cr < rows ? max(0, min(x.e.len, x.e.len - x.e.n + cr / group + 1)) : 0;
+                see[t][k] = cr < rows ? max(0, min(x.e.len, x.e.len - x.e.n + by_group(cr) + 1)) : 0;
                 if (cr < rows) least = min(least, see[t][k]);
             }
         }
@@ -619,7 +633,7 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
                 }
                 if (r == 0) {
                     if (!alone) p.part_stats[(size_t)rr * 2 * p.warps + piece] = make_float2(m[t][k], l[t][k]);
-                    else if (p.stats != nullptr) p.stats[stat_row(c, p, done.b, row / group, done.h * group + row % group)] = make_float2(m[t][k], l[t][k]);
+                    else if (p.stats != nullptr) p.stats[stat_row(c, p, done.b, by_group(row), done.h * group + row - by_group(row) * group)] = make_float2(m[t][k], l[t][k]);
                 }
             }
     }
@@ -671,7 +685,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
     pdl_launch_dependents();
     // lengths are not attend_few's to write
     const Entry e = entry_of(c, p, b);
-    const Share sh = share_of<R>(c, p, b, group);
+    const Share sh = share_of<R>(c, p, e, group);
     const int rows = sh.tiles > 0 ? e.n * group : 0;
     if ((int)blockIdx.x < mass_blocks) {
         const int t0 = blockIdx.x * kMassTokens;
