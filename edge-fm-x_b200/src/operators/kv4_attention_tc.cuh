@@ -463,14 +463,15 @@ template <int D>
 struct WeightsCfg {
     static constexpr int G = D / 64, KEYS = 128, ROWS = 128, K_PART = Tile<D>::V_CODES;       // keys of a block, packed rows of a step; codes and parameters of a page's keys
     static constexpr int K_BYTES = KEYS * 128 * G, Q_BYTES = ROWS * 128 * G;                 // K: of its high and of its low half
-    static constexpr int K_AT = 0, Q_AT = 2 * K_BYTES, PAR_AT = Q_AT + 2 * Q_BYTES, RAW_AT = PAR_AT + 2 * 4 * ROWS * 4, BARS = RAW_AT + 2 * K_PART;
+    static constexpr int K_AT = 0, Q_AT = 2 * K_BYTES, PAR_AT = Q_AT + 2 * Q_BYTES, SUM_AT = PAR_AT + 2 * 4 * ROWS * 4, RAW_AT = SUM_AT + KEYS * 4, BARS = RAW_AT + 2 * K_PART;
     static constexpr size_t SMEM = BARS + 96 + 1024;
 };
-constexpr int kWeightThreads = 9 * 32;
+constexpr int kWeightThreads = 13 * 32;
 
 // Summed weights where scores were not kept: S^T = K Q^T once more, 128 keys against 128 packed rows at a time, keys as a pair high + low of
-// fp16 so that scores have 32-bit accuracy.  A key is a lane of tensor memory and a thread of warps 0-3, which adds up its weights
-// 2^(s - m) / l over the rows in order: no atomics, no shuffles.  Warps 4-7 bring the rows' operand and (unit, m, 1 / l), warp 8 issues the products.
+// fp16 so that scores have 32-bit accuracy.  A key is a lane of tensor memory and two threads of warps 0-7, each of which adds up its weights
+// 2^(s - m) / l over half the rows of a step, in order: no atomics, no shuffles.  Warps 8-11 bring the rows' operand and (unit, m, 1 / l),
+// warp 12 issues the products.
 // grid (blocks of 128 cached rows, kv heads, batch).  Bound: exponentials and tensor pipe alike (128 x 128 of them in 1024 cycles, two products of K = D).
 template <typename T, int D>
 __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const Cache c, const AttnParams p) {
@@ -494,7 +495,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
     if (tid == 0) {
         tc::mbar_init(raw_full, 1);
         tc::mbar_init(drain, 1);
-        for (int i = 0; i < 2; ++i) { tc::mbar_init(q_full + 8 * i, 5); tc::mbar_init(q_empty + 8 * i, 1); tc::mbar_init(s_full + 8 * i, 1); tc::mbar_init(s_empty + 8 * i, 4); }
+        for (int i = 0; i < 2; ++i) { tc::mbar_init(q_full + 8 * i, 5); tc::mbar_init(q_empty + 8 * i, 1); tc::mbar_init(s_full + 8 * i, 1); tc::mbar_init(s_empty + 8 * i, 8); }
         *abort_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         const int there = (page[0] >= 0) + (page[1] >= 0);
@@ -502,7 +503,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
         for (int i = 0; i < 2; ++i)
             if (page[i] >= 0) bulk_copy(base + C::RAW_AT + i * C::K_PART, tile_of<D>(c, page[i], h), C::K_PART, raw_full);
     }
-    if (warp == 8) {
+    if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(tmem_slot)), "r"(256) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -541,8 +542,8 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
     const int rows = e.n * group, first_row = max(0, key0 - (e.len - e.n)) * group / C::ROWS * C::ROWS;       // rows before do not see the block
     const int n = rows > first_row ? (rows - first_row + C::ROWS - 1) / C::ROWS : 0;
     auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait(bar, parity, abort_s); };
-    if (warp < 4) {
-        const int key = key0 + tid;
+    if (warp < 8) {
+        const int key = key0 + (tid & 127), half = warp >> 2;         // which half of a step's rows
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
         int i = 0;
         for (; i < n; ++i) {
@@ -551,10 +552,10 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const float* par = reinterpret_cast<const float*>(sm + C::PAR_AT) + st * 4 * C::ROWS;      // [unit | -m | 1 / l | rows seen][row]
             const bool interior = e.len - e.n + r0 / group >= key0 + C::KEYS - 1;          // the step's first row sees every key
-#pragma unroll 1
-            for (int q = 0; q < C::ROWS; q += 64) {
+            {
+                const int q = half * 64;
                 float s[64];
-                tmem_ld64(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(st * C::ROWS + q), s);
+                tmem_ld64(tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(st * C::ROWS + q), s);
                 if (!interior) {
 #pragma unroll
                     for (int k = 0; k < 64; ++k) if (key >= reinterpret_cast<const int*>(par)[3 * C::ROWS + q + k]) s[k] = -INFINITY;
@@ -573,13 +574,17 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
             warp_arrive(s_empty + 8 * st);
         }
         if (i < n) *abort_s = 1;
-        const int pg = page[tid >> 6];
-        if (i == n && key < e.len && pg >= 0) {
+        float* other = reinterpret_cast<float*>(sm + C::SUM_AT);
+        const float mine = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (half == 1) other[tid & 127] = mine;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const int pg = page[(tid & 127) >> 6];
+        if (half == 0 && i == n && key < e.len && pg >= 0) {
             const size_t at = row_slot(c, pg, h, key % kRows);
-            p.mass_out[at] = p.mass_in[at] + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+            p.mass_out[at] = p.mass_in[at] + (mine + other[tid]);
         }
-    } else if (warp < 8) {
-        const int tr = tid - 128;
+    } else if (warp < 12) {
+        const int tr = tid - 256;
         int i = 0;
         for (; i < n; ++i) {
             const int st = i & 1, row = first_row + i * C::ROWS + tr;
@@ -644,7 +649,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
         raise(c, kWait);
     }
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 12) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256) : "memory");
     }
