@@ -161,8 +161,8 @@ __device__ __forceinline__ size_t row_tile(const Cache& c, const AttnParams& p, 
 // itself took 4000 cycles a tile).  grid (tiles, kv heads, batch).
 template <typename T, int D>
 __global__ void __launch_bounds__(kTileRows) attend_query_kernel(const Cache c, const AttnParams p) {
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     const int h = blockIdx.y, b = blockIdx.z, group = c.q_heads / c.kv_heads, row = blockIdx.x * kTileRows + threadIdx.x;
     const Entry e = entry_of(c, p, b);
     const int rows = e.n * group;

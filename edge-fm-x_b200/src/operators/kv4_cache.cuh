@@ -142,8 +142,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const Cache c, c
     };
     if (tid == 0) place_s = -1;
     __syncthreads();
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     int task = blockIdx.y * tasks_per_block + warp;
     uint4 next = row < p.max_rows ? fetch(task) : make_uint4(0u, 0u, 0u, 0u);             // on its way while the row's place is looked up
     for (int b = tid; b < c.batch; b += kAppendThreads) {
@@ -283,8 +283,8 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const Cache c, const
     using L = Tile<D>;
     constexpr int PER = kRows * L::WORDS / kReadThreads;
     const int b = blockIdx.y, h = blockIdx.x % c.kv_heads, k = first / kRows + blockIdx.x / c.kv_heads;
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     const int n = min(held(c, lens, b, c.max_pages * kRows), first + rows);
     if (k * kRows >= n) return;
     const int page = page_of(c, b, k);

@@ -83,8 +83,8 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const Ca
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) newest_s = INT32_MIN;
     for (int i = tid; i < kBins * kCopies; i += kEvictThreads) hist[i] = 0;
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     const int n = held(c, p.lens_in, b, c.max_pages * kRows);
     const bool over = n > p.limit, apart = p.index_out != p.index_in || p.mass_out != p.mass_in;
     if (h == 0 && tid == 0) p.lens_out[b] = over ? p.budget : n;
@@ -264,8 +264,8 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const Ca
 template <int D>
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const Cache c, const EvictParams p) {
     const int h = blockIdx.y, b = blockIdx.z;
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     const int2* moves = p.moves + (size_t)(b * c.kv_heads + h) * p.most_moves;
     move_rows<D, 4>(c, p, h, moves, blockIdx.x * (kMoveThreads / 16) + threadIdx.x / 16, gridDim.x * (kMoveThreads / 16), p.n_moves[b * c.kv_heads + h], threadIdx.x & 15);
 }
