@@ -145,7 +145,15 @@ struct AttnPlan {
 };
 constexpr int kSms = 148;                              // of the GPU these kernels are built for
 constexpr int kWholeShift = 2;
-constexpr int kFewRows = 32;                           // packed rows of a sequence up to which attend_few takes it
+// Packed rows of a sequence up to which attend_few takes it, in tiles of 16.  A page costs attend_few 3.7 ns a tile once the tiles fill the
+// GPU; it costs attend_many 1.3 us (bf16; fp16, with its products in three parts, 2.2 us) for every round of 256-row blocks over the SMs,
+// however few rows are in them.  Equal at some 350 tiles (fp16: 590) of all sequences and kv heads while the blocks are one round, and at
+// 2.3 (fp16: 3.9) tiles of each beyond.  Measured (28 query heads, 4 kv heads of 128, attend_few / attend_many): 128 rows on 4000 tokens,
+// 224 tiles, 55 / 83 us; 256 rows, 448 tiles, 107 / 86 us; 64 heads on one kv head, a row on 30000 tokens, 4 tiles, 23 / 392 us.
+int few_rows_of(const efm_kv4_cache* c) {
+    const int64_t each = (int64_t)c->batch * c->kv_heads, bf16 = c->dtype == EFM_BF16;
+    return (int)(16 * std::max<int64_t>(bf16 ? 2 : 3, (bf16 ? 3 : 5) * kSms / 2 / each));
+}
 
 AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
     AttnPlan p{};
@@ -153,7 +161,7 @@ AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
     p.max_len = a->max_len > 0 ? a->max_len : (int)capacity(c);
     const int64_t rows = (int64_t)p.max_new * (c->q_heads / c->kv_heads);
     p.nt = rows <= 8 ? 1 : 2;
-    p.few_rows = kFewRows;
+    p.few_rows = few_rows_of(c);
     p.many_tiles = rows > p.few_rows ? (int)((rows + 2 * kv4::kTileRows - 1) / (2 * kv4::kTileRows)) : 0;
     const int64_t R = 8 * p.nt, tiles = (std::min<int64_t>(rows, p.few_rows) + R - 1) / R, pages = std::max(1, (p.max_len + kRows - 1) / kRows);
     // a page at a time, or caches of up to four pages whole: nothing is left to join then, which saves the smallest calls a launch
@@ -276,7 +284,7 @@ efm_status efm_b200_op_kv4_append(const efm_kv4_cache* cache, const efm_kv4_appe
         const int per = 256 / cache->head_dim, kv = (cache->kv_heads + per - 1) / per, tasks = (a->q != nullptr ? (cache->q_heads + per - 1) / per : 0) + 2 * kv, warps = kv4::kAppendThreads / 32;
         // few rows: a task (the heads a warp has at a time) per warp, so that a row's heads are on as many SMs as there are; many rows: a
         // block per row, one table of angles
-        const int per_block = a->max_rows * ((tasks + warps - 1) / warps) <= 2 * info.sms ? warps : tasks;
+        const int per_block = (int64_t)a->max_rows * ((tasks + warps - 1) / warps) <= 2 * info.sms ? warps : tasks;
         Launcher L = on_stream(stream);
         by_type(cache, [&](auto t, auto d) {
             L.launch(kv4::append_kernel<decltype(t), decltype(d)::value>, dim3(std::max(a->max_rows, 1), (tasks + per_block - 1) / per_block), dim3(kv4::kAppendThreads), 0,
@@ -303,12 +311,13 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
         OnDevice on;
         DeviceInfo info;
         if ((st = on.enter(call, cache->pool)) != EFM_OK || (st = device_info(call, on.device, info)) != EFM_OK) return st;
+        const uint32_t group = cache->q_heads / cache->kv_heads;
         kv4::AttnParams p{};
         p.max_rows = a->max_rows; p.max_new = plan.max_new; p.max_len = plan.max_len;
         p.cu_rows = a->cu_rows; p.lens = a->lens; p.q = a->q; p.out = a->out;
         p.scale_log2 = a->scale * 1.4426950408889634f;
         p.mass_in = a->mass_in; p.mass_out = a->mass_out;
-        p.few_rows = plan.few_rows; p.warps = plan.blocks * kv4::kWarps; p.unit_shift = plan.unit_shift; p.group_inv = (65536 + cache->q_heads / cache->kv_heads - 1) / (cache->q_heads / cache->kv_heads); p.rows = plan.max_new;
+        p.few_rows = plan.few_rows; p.warps = plan.blocks * kv4::kWarps; p.unit_shift = plan.unit_shift; p.group_inv = group == 1 ? 0u : (uint32_t)(((1ull << 32) + group - 1) / group); p.rows = plan.max_new;
         float* ws = (float*)a->workspace;
         p.stats = plan.stats > 0 ? (float2*)ws : nullptr;
         p.part_stats = (float2*)(ws + plan.stats);

@@ -22,7 +22,7 @@ struct AttnParams {
     float* mass_out;
     int few_rows;             // sequences with at most this many packed rows (new rows x heads of a group) are attend_few's
     int warps, unit_shift;    // attend_few's warps; pages of a unit of work: 1 << unit_shift
-    uint32_t group_inv;       // ceil(2^16 / heads of a group): packed rows below 2^8 are divided by it
+    uint32_t group_inv;       // ceil(2^32 / heads of a group), 0 for one: what packed rows are divided by
     float2* stats;            // [batch, rows, q_heads] (maximum, sum) of a row's weights, where one warp had all its keys; null: not wanted
     int rows;                 // new rows a sequence has in stats
     float2* part_stats;       // [8 nt][2 warps] the same of the keys a warp had, and
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
     const int step = step_of(p, all), u1 = (int)min((int64_t)all, ((int64_t)me + 1) * step);
     int u = (int)min((int64_t)all, (int64_t)me * step), slot = 0;                // slot: of the copies and their barriers
     if (u >= u1) return;
-    auto by_group = [&](int row) { return (int)((uint32_t)row * p.group_inv >> 16); };       // row / group
+    auto by_group = [&](int row) { return p.group_inv != 0u ? (int)__umulhi((uint32_t)row, p.group_inv) : row; };      // row / group, exact below 2^22
 
     // one piece after the other: pages of a (sequence, kv head, tile of rows)
     struct Piece { Entry e; int b, h, tile, p0, mine; bool from_start, to_end; };
@@ -682,7 +682,6 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
     __shared__ float4 v_s[kWarps * 32];
     __shared__ float f_s[kFactors];
     const int h = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = c.q_heads / c.kv_heads;
-    pdl_launch_dependents();
     // lengths are not attend_few's to write
     const Entry e = entry_of(c, p, b);
     const Share sh = share_of<R>(c, p, e, group);
@@ -690,6 +689,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
     if ((int)blockIdx.x < mass_blocks) {
         const int t0 = blockIdx.x * kMassTokens;
         pdl_wait();
+        pdl_launch_dependents();
         if (t0 >= e.len) return;
         const Pieces x = rows > 0 ? pieces_of(p, sh, Deal{p.starts[b], p.starts[c.batch]}, h, 0) : Pieces{0, 0};
         for (int row = warp; row < rows; row += kWarps) {
@@ -726,6 +726,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
         return;
     }
     pdl_wait();
+    pdl_launch_dependents();
     if (rows == 0) return;
     const Deal deal{p.starts[b], p.starts[c.batch]};
     const int first = (int)blockIdx.x - mass_blocks, blocks = (int)gridDim.x - mass_blocks;
