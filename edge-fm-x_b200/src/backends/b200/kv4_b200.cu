@@ -136,23 +136,27 @@ efm_status check_attention(const char* call, const efm_kv4_cache* c, const efm_k
 
 // What a call needs: tiles of 8 nt packed query rows, and the parts of its workspace, in floats.
 struct AttnPlan {
-    int max_new, max_len, nt, blocks, unit_shift, few_rows, many_tiles;      // many_tiles: blocks of 256 packed rows a sequence may have
+    int max_new, max_len, nt, blocks, unit_shift, few_rows;
+    int many_tiles, many_blocks;                      // blocks of 256 packed rows a sequence may have; blocks that deal with them
+    int64_t many_units, many_starts, many_stats, many_part;
     bool joined;                                      // pieces of a row may lie in several blocks
     bool scores;                                      // attend_few leaves its scores for the summed weights
     int64_t units, stats, part_stats, part, score_ld, score, image, image_units, starts;
     int row_tiles;                                    // tiles of 128 packed rows a sequence may have as operands; 0: nobody asks for them
-    int64_t bytes() const { return 4 * (stats + part_stats + part + score + image + image_units + starts); }
+    int64_t bytes() const { return 4 * (stats + part_stats + part + score + image + image_units + starts + many_starts + many_stats + many_part); }
 };
 constexpr int kSms = 148;                              // of the GPU these kernels are built for
 constexpr int kWholeShift = 2;
-// Packed rows of a sequence up to which attend_few takes it, in tiles of 16.  A page costs attend_few 3.7 ns a tile once the tiles fill the
-// GPU; it costs attend_many 1.3 us (bf16; fp16, with its products in three parts, 2.2 us) for every round of 256-row blocks over the SMs,
-// however few rows are in them.  Equal at some 350 tiles (fp16: 590) of all sequences and kv heads while the blocks are one round, and at
-// 2.3 (fp16: 3.9) tiles of each beyond.  Measured (28 query heads, 4 kv heads of 128, attend_few / attend_many): 128 rows on 4000 tokens,
-// 224 tiles, 55 / 83 us; 256 rows, 448 tiles, 107 / 86 us; 64 heads on one kv head, a row on 30000 tokens, 4 tiles, 23 / 392 us.
+// Packed rows of a sequence up to which attend_few takes it, in tiles of 16.  A page costs attend_few 3.7 ns a tile of 128 channels (half
+// of it with 64) once the tiles fill the GPU; attend_many has three launches more and some 8.6 ns a block of 256 rows, however few rows are
+// in it (fp16, with its products in three parts: 14).  Equal at some 90 tiles of all sequences and kv heads (fp16: 190), and where those are
+// many, at 2 (fp16: 3) of each.  Measured (attend_few / attend_many, us): 28 query heads on 4 kv heads of 128, 4000 tokens, 32 rows (56 tiles)
+// 26 / 33, 64 rows (112) 39 / 33; 8 sequences of 2000 tokens with 32 on 4, 6 rows (96) 27 / 31, 12 rows (192) 36 / 33, fp16 16 rows (256) 40 / 41;
+// 64 such, 4 rows (2 tiles each) 72 / 82, 6 rows (3 each) 100 / 84, fp16 8 rows (4 each) 128 / 135; 64 channels, 14 on 2, 256 rows (224) 25 / 28.
 int few_rows_of(const efm_kv4_cache* c) {
-    const int64_t each = (int64_t)c->batch * c->kv_heads, bf16 = c->dtype == EFM_BF16;
-    return (int)(16 * std::max<int64_t>(bf16 ? 2 : 3, (bf16 ? 3 : 5) * kSms / 2 / each));
+    const bool bf16 = c->dtype == EFM_BF16;
+    const int64_t each = (int64_t)c->batch * c->kv_heads, all = (bf16 ? 90 : 190) * (128 / c->head_dim);
+    return (int)(16 * std::max<int64_t>(bf16 ? 2 : 3, all / each));
 }
 
 AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
@@ -162,7 +166,7 @@ AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
     const int64_t rows = (int64_t)p.max_new * (c->q_heads / c->kv_heads);
     p.nt = rows <= 8 ? 1 : 2;
     p.few_rows = few_rows_of(c);
-    p.many_tiles = rows > p.few_rows ? (int)((rows + 2 * kv4::kTileRows - 1) / (2 * kv4::kTileRows)) : 0;
+    p.many_tiles = rows > p.few_rows ? (int)((rows + kv4::kManyRows - 1) / kv4::kManyRows) : 0;
     const int64_t R = 8 * p.nt, tiles = (std::min<int64_t>(rows, p.few_rows) + R - 1) / R, pages = std::max(1, (p.max_len + kRows - 1) / kRows);
     // a page at a time, or caches of up to four pages whole: nothing is left to join then, which saves the smallest calls a launch
     p.unit_shift = pages <= 1 << kWholeShift ? kWholeShift : 0;
@@ -179,6 +183,14 @@ AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
     p.row_tiles = p.many_tiles > 0 || (a->mass_out != nullptr && !p.scores) ? (int)((rows + kv4::kTileRows - 1) / kv4::kTileRows) : 0;
     p.image_units = (int64_t)c->batch * c->kv_heads * p.row_tiles * kv4::kTileRows;
     p.image = p.image_units * c->head_dim / 2;
+    if (p.many_tiles > 0) {                           // no more blocks of rows than one a sequence and those that all rows fill
+        const int64_t tiles_all = std::min<int64_t>((int64_t)c->batch * p.many_tiles, c->batch + (int64_t)a->max_rows * (c->q_heads / c->kv_heads) / kv4::kManyRows);
+        p.many_units = tiles_all * c->kv_heads * pages;
+        p.many_blocks = (int)std::min<int64_t>(kSms, (p.many_units + kv4::kManyStep - 1) / kv4::kManyStep);
+        p.many_starts = round_up((int64_t)c->batch * p.many_tiles + 1, 4);
+        p.many_stats = 2 * 2 * (int64_t)p.many_blocks * kv4::kManyRows;
+        p.many_part = 2 * (int64_t)p.many_blocks * kv4::kManyRows * c->head_dim;
+    }
     p.score = p.scores ? (int64_t)c->batch * c->kv_heads * R * p.score_ld : 0;
     return p;
 }
@@ -307,7 +319,7 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
         const AttnPlan plan = plan_attention(cache, a);
         if (plan.bytes() > 0 && (a->workspace == nullptr || a->workspace_bytes < plan.bytes() || !aligned(a->workspace, 16)))
             return bad(call, "workspace: 16-byte aligned, as large as efm_b200_kv4_attention_workspace says");
-        if (plan.units > (1 << 30)) return fail(nullptr, EFM_ERR_UNSUPPORTED, std::string(call) + ": more than 2^30 pages x kv heads x row tiles");
+        if (plan.units > (1 << 30) || plan.many_units > (1 << 30) || plan.many_starts > (1 << 30)) return fail(nullptr, EFM_ERR_UNSUPPORTED, std::string(call) + ": more than 2^30 pages x kv heads x row tiles");
         OnDevice on;
         DeviceInfo info;
         if ((st = on.enter(call, cache->pool)) != EFM_OK || (st = device_info(call, on.device, info)) != EFM_OK) return st;
@@ -328,6 +340,10 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
         p.images = (uint8_t*)(ws + plan.stats + plan.part_stats + plan.part + plan.score);
         p.units = (float*)p.images + plan.image;
         p.starts = (int32_t*)(p.units + plan.image_units);
+        p.many_tiles = plan.many_tiles; p.many_blocks = plan.many_blocks;
+        p.many_starts = p.starts + plan.starts;
+        p.many_stats = (float2*)(p.many_starts + plan.many_starts);
+        p.many_part = (float*)p.many_stats + plan.many_stats;
         Launcher L = on_stream(stream);
         by_type(cache, [&](auto t, auto d) {
             using T = decltype(t);
@@ -341,13 +357,14 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
             const dim3 join(merges + masses, cache->kv_heads, cache->batch);
             if (rows > 0 && plan.nt == 1) L.launch(kv4::attend_few_kernel<T, D, 1>, dim3(plan.blocks), block, kv4::FewCfg<D, 1>::SMEM, c, p);
             if (rows > 0 && plan.nt == 2) L.launch(kv4::attend_few_kernel<T, D, 2>, dim3(plan.blocks), block, kv4::FewCfg<D, 2>::SMEM, c, p);
-            if (plan.row_tiles > 0) L.launch(kv4::attend_query_kernel<T, D>, dim3(plan.row_tiles, cache->kv_heads, cache->batch), dim3(kv4::kTileRows), 0, c, p);
-            const dim3 many(plan.many_tiles, cache->kv_heads, cache->batch);
+            if (plan.row_tiles > 0) L.launch(kv4::attend_query_kernel<T, D>, dim3(plan.row_tiles + 1, cache->kv_heads, cache->batch), dim3(kv4::kTileRows), 0, c, p);
             if (plan.many_tiles > 0) {
+                const dim3 many(plan.many_blocks);
                 const dim3 threads(kv4::kManyThreads);
                 if constexpr (std::is_same<T, __half>::value) L.launch(kv4::attend_many_kernel<T, D, 2>, many, threads, kv4::ManyCfg<D, 2>::SMEM, c, p);
                 else if (p.mass_out != nullptr) L.launch(kv4::attend_many_kernel<T, D, 1>, many, threads, kv4::ManyCfg<D, 1>::SMEM, c, p);
                 else L.launch(kv4::attend_many_kernel<T, D, 0>, many, threads, kv4::ManyCfg<D, 0>::SMEM, c, p);
+                if (plan.many_blocks > 1) L.launch(kv4::attend_join_kernel<T, D>, dim3(plan.many_blocks - 1, D / 16), dim3(kv4::kManyRows), 0, c, p);
             }
             L.pdl = rows > 0;                          // what follows reads lengths ahead of its wait: not as a call's first launch
             if (join.x > 0 && plan.nt == 1) L.launch(kv4::attend_merge_kernel<T, D, 8>, join, block, 0, c, p, masses);

@@ -31,6 +31,10 @@ struct AttnParams {
     uint8_t* images;          // [batch, kv_heads, row_tiles][128 x D fp16] packed rows as operands, and
     float* units;             // [batch, kv_heads, row_tiles][128] what their scores are multiplied with; where many rows are a sequence's
     int row_tiles;
+    int many_tiles, many_blocks;      // blocks of 256 packed rows a sequence may have; blocks of attend_many
+    int32_t* many_starts;     // [batch x many_tiles + 1] its units ahead, and all of them
+    float2* many_stats;       // [2 many_blocks][256] and
+    float* many_part;         // [2 many_blocks][D / 4][256][4] what part_stats and part are, of its pieces
     float* scores;            // [batch, kv_heads, 8 nt][score_ld] scores in units of log2; null: not wanted
     int64_t score_ld;
 };

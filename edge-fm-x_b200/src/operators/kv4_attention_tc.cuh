@@ -28,6 +28,7 @@ namespace efm {
 namespace kv4 {
 
 constexpr int kTileRows = 128, kManyThreads = 15 * 32;
+constexpr float kLift = 7.0f;              // weights of many rows are relative to their maximum less this power of two
 
 template <int D, int X>
 struct ManyCfg {
@@ -37,7 +38,7 @@ struct ManyCfg {
     static constexpr int KB = X >= 1 ? 2 * LOW : LOW, VB = X == 2 ? 2 * LOW : LOW;       // bytes of a stage
     static constexpr int Q_AT = 0, K_AT = 2 * Q_BYTES, V_AT = K_AT + KS * KB, RAW_AT = V_AT + VS * VB, BARS = RAW_AT + RAW * Tile<D>::BYTES;
     static constexpr int S_COL = 0, O_COL = 256;                                         // S of (tile, page parity): 64 columns each, P in its place; O: 128 a tile
-    static constexpr size_t SMEM = BARS + 320 + 1024;
+    static constexpr size_t SMEM = BARS + 336 + 1024;
 };
 
 // Pairs of fp16 codes of a word, in the order of the channels: as in low_pair / high_pair, without the 8.
@@ -103,6 +104,29 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&r)[64]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// Two 32-bit numbers a register pair, one instruction for both.
+__device__ __forceinline__ uint64_t pair_of_floats(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float low_of(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float high_of(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ uint32_t elect_one() {
     uint32_t lead;
     asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(lead));
@@ -157,12 +181,107 @@ __device__ __forceinline__ void quarter_words(const uint32_t* codes, int r, int 
 
 __device__ __forceinline__ size_t row_tile(const Cache& c, const AttnParams& p, int b, int h, int tile) { return ((size_t)b * c.kv_heads + h) * p.row_tiles + tile; }
 
+// How attend_many's work is dealt: its units are the pages of every (sequence, block of 256 packed rows, kv head), in that order, block w of
+// the grid has the units [w step, (w + 1) step).  Rows that begin or end inside such a range are joined by attend_join.
+constexpr int kManyRows = 2 * kTileRows;
+constexpr int64_t kMostUnits = 1 << 30;
+constexpr int kManyStep = 4;               // at least that many pages a block: fewer cost more to join than they save
+// Pages of a block of rows of a sequence, 0: nobody's, or attend_few's; rows that see nothing are somebody's to clear.
+__device__ __forceinline__ int many_pages(const AttnParams& p, const Entry& e, int group, int tile) {
+    const int rows = e.n * group;
+    if (rows <= p.few_rows || tile * kManyRows >= rows) return 0;
+    const int last = min(rows, (tile + 1) * kManyRows) - 1;
+    return max(1, (min(e.len, e.len - e.n + last / group + 1) + kRows - 1) / kRows);
+}
+__device__ __forceinline__ int many_step(const AttnParams& p, int all) { return max(kManyStep, (all + p.many_blocks - 1) / p.many_blocks); }
+// many_starts[b * many_tiles + tile]: units ahead, by one block of kTileRows threads
+__device__ __forceinline__ void lay_out_units(const Cache& c, const AttnParams& p) {
+    __shared__ int64_t sums[kTileRows / 32];
+    const int group = c.q_heads / c.kv_heads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t pairs = (int64_t)c.batch * p.many_tiles, per = (pairs + kTileRows - 1) / kTileRows, lo = min(pairs, (int64_t)threadIdx.x * per), hi = min(pairs, lo + per);
+    int64_t own = 0;
+    auto walk = [&](auto&& visit) {
+        int b = (int)(lo / p.many_tiles), tile = (int)(lo % p.many_tiles);
+        Entry e{};
+        if (lo < hi) e = entry_of(c, p, b);
+        for (int64_t i = lo; i < hi; ++i) {
+            visit(i, many_pages(p, e, group, tile) * c.kv_heads);
+            if (++tile == p.many_tiles) {
+                tile = 0;
+                if (++b < c.batch) e = entry_of(c, p, b);
+            }
+        }
+    };
+    walk([&](int64_t, int n) { own += n; });
+    int64_t upto = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    int64_t all = 0;
+    for (int w = 0; w < kTileRows / 32; ++w) { if (w < warp) upto += sums[w]; all += sums[w]; }
+    int64_t at = upto - own;                                     // row counts that lie may add up to more than the caller's sizes allow: cut off there
+    walk([&](int64_t i, int n) { p.many_starts[i] = (int)min(at, kMostUnits); at += n; });
+    if (threadIdx.x == 0) p.many_starts[pairs] = (int)min(all, kMostUnits);
+}
+// Of a (sequence, block of rows) whose units begin at or before `from`, the one that has unit u, by a warp: 32 at a time.
+__device__ __forceinline__ int pair_of(const int32_t* starts, int pairs, int from, int u) {
+    const int lane = threadIdx.x & 31;
+    int lo = from, hi = pairs;                                   // starts[lo] <= u < starts[hi]
+    uint32_t later = __ballot_sync(0xffffffffu, starts[min(hi, lo + 1 + lane)] > u);         // mostly one of the next
+    if (later != 0u) return lo + __ffs(later) - 1;
+    for (lo += 32; hi - lo > 1;) {
+        const int s = (hi - lo + 31) / 32;
+        later = __ballot_sync(0xffffffffu, starts[min(hi, lo + (lane + 1) * s)] > u);
+        const int k = __ffs(later) - 1;                          // lane 31 looks at hi
+        hi = min(hi, lo + (k + 1) * s);
+        lo += k * s;
+    }
+    return lo;
+}
+// Pages [p0, p0 + n) of a (sequence, block of rows, kv head), as a warp walks a block's range of units.
+struct ManyPiece { Entry e; int b, h, r0, tiles, p0, n; bool from_start, to_end; };
+struct ManyWalk {
+    int u, u1, pair, base, pairs;
+    __device__ __forceinline__ ManyWalk(const Cache& c, const AttnParams& p, int block) : pair(0), base(0), pairs(c.batch * p.many_tiles) {
+        const int all = p.many_starts[pairs], step = many_step(p, all);
+        u = (int)min((int64_t)all, (int64_t)block * step);
+        u1 = min(all, u + step);
+    }
+    __device__ __forceinline__ bool more() const { return u < u1; }
+    __device__ __forceinline__ ManyPiece next(const Cache& c, const AttnParams& p) {
+        ManyPiece x;
+        pair = pair_of(p.many_starts, pairs, pair, u);
+        base = p.many_starts[pair];
+        x.b = pair / p.many_tiles;
+        const int tile = pair - x.b * p.many_tiles, group = c.q_heads / c.kv_heads;
+        x.e = entry_of(c, p, x.b);
+        const int each = many_pages(p, x.e, group, tile), in = u - base;
+        x.h = in / each;
+        x.p0 = in - x.h * each;
+        x.n = __shfl_sync(0xffffffffu, min(each - x.p0, u1 - u), 0);
+        x.r0 = tile * kManyRows;
+        x.tiles = x.e.n * group - x.r0 > kTileRows ? 2 : 1;
+        x.from_start = x.p0 == 0;
+        x.to_end = x.p0 + x.n == each;
+        u += x.n;
+        return x;
+    }
+};
+
 // Packed rows, 128 a tile, as the operands that attend_many and attend_weights copy in one piece (every block of theirs converting rows for
-// itself took 4000 cycles a tile).  grid (tiles, kv heads, batch).
+// itself took 4000 cycles a tile).  grid (tiles + 1, kv heads, batch): one block adds up attend_many's units of work instead.
 template <typename T, int D>
 __global__ void __launch_bounds__(kTileRows) attend_query_kernel(const Cache c, const AttnParams p) {
     pdl_wait();
     pdl_launch_dependents();
+    if ((int)blockIdx.x == p.row_tiles) {
+        if (blockIdx.y == 0 && blockIdx.z == 0 && p.many_tiles > 0) lay_out_units(c, p);
+        return;
+    }
     const int h = blockIdx.y, b = blockIdx.z, group = c.q_heads / c.kv_heads, row = blockIdx.x * kTileRows + threadIdx.x;
     const Entry e = entry_of(c, p, b);
     const int rows = e.n * group;
@@ -172,37 +291,33 @@ __global__ void __launch_bounds__(kTileRows) attend_query_kernel(const Cache c, 
     p.units[tile * kTileRows + threadIdx.x] = query_rows<T, D>((const T*)p.q, at, p.images + tile * (kTileRows * D * 2), threadIdx.x & ~31, p.scale_log2);
 }
 
-// grid (tiles of 256 packed rows, kv heads, batch); late rows see the most keys and come first
+// grid: one block an SM, each with its share of the units (above)
 template <typename T, int D, int X>
 __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cache c, const AttnParams p) {
     using C = ManyCfg<D, X>;
     using L = Tile<D>;
     constexpr int G = C::G;
-    constexpr float kGrow = 8.0f, kLift = 7.0f;                  // p is up to 2^(8 + 7): fp16 keeps weights down to 2^-21 of the largest whole
+    constexpr float kGrow = 8.0f;                                // p is up to 2^(8 + kLift): fp16 keeps weights down to 2^-21 of the largest whole
     extern __shared__ unsigned char many_smem[];
     const uint32_t raw_base = tc::smem_u32(many_smem), base = (raw_base + 1023u) & ~1023u;
     unsigned char* sm = many_smem + (base - raw_base);
     const uint32_t bars = base + C::BARS;
-    const uint32_t q_full = bars, raw_full = bars + 8, raw_empty = bars + 40, k_full = bars + 72, k_empty = bars + 96, v_full = bars + 120, v_empty = bars + 144,
-                   s_full = bars + 168, p_full = bars + 200, o_done = bars + 232, drain = bars + 264;     // s_full, p_full, o_done: [tile][page parity]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::BARS + 280);
+    const uint32_t q_full = bars, raw_full = bars + 16, raw_empty = bars + 48, k_full = bars + 80, k_empty = bars + 104, v_full = bars + 128, v_empty = bars + 152,
+                   s_full = bars + 176, p_full = bars + 208, o_done = bars + 240, drain = bars + 272;     // q_full: [tile]; s_full, p_full, o_done: [tile][parity of its pages]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::BARS + 288);
     volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    volatile int* there = reinterpret_cast<volatile int*>(tmem_slot + 2);        // [8] page j % 8 is one of the pool's
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y, b = blockIdx.z, group = c.q_heads / c.kv_heads;
+    volatile int* valid_s = reinterpret_cast<volatile int*>(tmem_slot + 2);      // [8] rows held of the block's page number j % 8; 0: not one of the pool's
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = c.q_heads / c.kv_heads;
 
     pdl_wait();
-    const Entry e = entry_of(c, p, b);
-    const int rows = e.n * group, r0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * 2 * kTileRows;
-    if (rows <= p.few_rows || r0 >= rows) return;
-    const int nt = rows - r0 > kTileRows ? 2 : 1;                                // tiles in use
-    const int last = min(rows, r0 + 2 * kTileRows) - 1;
-    const int n = (max(0, min(e.len, e.len - e.n + last / group + 1)) + kRows - 1) / kRows;      // pages that any of the rows sees
+    ManyWalk walk(c, p, blockIdx.x);
+    const int pages = walk.u1 - walk.u;                          // of all pieces
+    if (pages <= 0) return;
     if (tid == 0) {
-        tc::mbar_init(q_full, 1);
         for (int i = 0; i < C::RAW; ++i) { tc::mbar_init(raw_full + 8 * i, 1); tc::mbar_init(raw_empty + 8 * i, 4); }
-        for (int i = 0; i < 2; ++i) tc::mbar_init(drain + 8 * i, 1);
-        for (int i = 0; i < C::KS; ++i) { tc::mbar_init(k_full + 8 * i, 4); tc::mbar_init(k_empty + 8 * i, nt); }
-        for (int i = 0; i < C::VS; ++i) { tc::mbar_init(v_full + 8 * i, 4); tc::mbar_init(v_empty + 8 * i, nt); }
+        for (int i = 0; i < 2; ++i) { tc::mbar_init(q_full + 8 * i, 1); tc::mbar_init(drain + 8 * i, 1); }
+        for (int i = 0; i < C::KS; ++i) { tc::mbar_init(k_full + 8 * i, 4); tc::mbar_init(k_empty + 8 * i, 2); }
+        for (int i = 0; i < C::VS; ++i) { tc::mbar_init(v_full + 8 * i, 4); tc::mbar_init(v_empty + 8 * i, 2); }
         for (int i = 0; i < 4; ++i) { tc::mbar_init(s_full + 8 * i, 1); tc::mbar_init(p_full + 8 * i, 4); tc::mbar_init(o_done + 8 * i, 1); }
         *abort_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -218,63 +333,67 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
     pdl_launch_dependents();                                     // not before this block has its tensor memory
 
     if (warp < 8) {
-        const int t = warp >> 2, tr = (warp & 3) * 32 + lane, row = r0 + t * kTileRows + tr;
-        if (t < nt) {
-            const bool have = row < rows;
-            const size_t at = ((size_t)(e.row0 + row / group) * c.q_heads + h * group + row % group) * D;
-            const int see = have ? max(0, min(e.len, e.len - e.n + row / group + 1)) : 0;
+        const int t = warp >> 2, tr = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t o_at = tmem + lanes + (uint32_t)(C::O_COL + t * 128);
+        bool ok = true;
+        for (int before = 0, mine = 0; ok && walk.more();) {     // pages of the pieces before: of all, and of this tile
+            const ManyPiece x = walk.next(c, p);
+            if (t >= x.tiles) { before += x.n; continue; }
+            const int row = x.r0 + t * kTileRows + tr;
+            const bool have = row < x.e.n * group;
+            const int see = have ? max(0, min(x.e.len, x.e.len - x.e.n + row / group + 1)) - x.p0 * kRows : 0;     // counted from the piece's first key
             int least = have ? see : INT32_MAX;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
-            const float unit = p.units[row_tile(c, p, b, h, r0 / kTileRows + t) * kTileRows + tr];
-            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-            const uint32_t o_at = tmem + lanes + (uint32_t)(C::O_COL + t * 128);
+            const float unit = p.units[row_tile(c, p, x.b, x.h, x.r0 / kTileRows + t) * kTileRows + tr];
             float m = -INFINITY, l = 0.f;                        // m: what the row's weights are relative to
             int j = 0;
-            for (; j < n; ++j) {
-                const int buf = t * 2 + (j & 1);
+            for (; j < x.n; ++j) {
+                const int buf = t * 2 + ((mine + j) & 1);
                 const uint32_t s_at = tmem + lanes + (uint32_t)(C::S_COL + buf * 64);
-                if (!warp_wait(s_full + 8 * buf, (uint32_t)(j >> 1) & 1u, abort_s)) { *abort_s = 1; break; }
+                if (!warp_wait(s_full + 8 * buf, (uint32_t)((mine + j) >> 1) & 1u, abort_s)) { *abort_s = 1; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 float s[64];
                 tmem_ld64(s_at, s);
-                const int seen = there[j & 7] ? see - j * kRows : 0;             // keys of the page that the row sees
-                if (there[j & 7] == 0 || (j + 1) * kRows > least) {
+                const int held = valid_s[(before + j) & 7], seen = held != 0 ? see - j * kRows : 0;             // keys of the page that the row sees
+                if (held == 0 || (j + 1) * kRows > least) {
 #pragma unroll
                     for (int i = 0; i < 64; ++i) if (i >= seen) s[i] = -INFINITY;
                 }
-                float mx[4] = {s[0], s[1], s[2], s[3]};
+                float mx[4] = {fmaxf(s[0], s[1]), fmaxf(s[2], s[3]), fmaxf(s[4], s[5]), fmaxf(s[6], s[7])};
 #pragma unroll
-                for (int i = 4; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+                for (int i = 8; i < 64; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], s[i], s[i + 1]);
                 const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * unit;
                 const bool grow = mn > m + kGrow || (m == -INFINITY && mn != -INFINITY);
                 float alpha = 1.0f;
                 if (grow) { alpha = at::ex2(m - mn); l *= alpha; m = mn; }
                 const float off = m == -INFINITY ? kLift : kLift - m;
                 uint32_t pk[32], pl[X == 2 ? 32 : 1];
-                float sum[2] = {0.f, 0.f};
+                uint64_t sum = 0;
+                const uint64_t unit2 = pair_of_floats(unit, unit), off2 = pair_of_floats(off, off);
 #pragma unroll
                 for (int i = 0; i < 64; i += 2) {
-                    const float a = at::ex2(fmaf(s[i], unit, off)), bb = at::ex2(fmaf(s[i + 1], unit, off));
-                    sum[0] += a;
-                    sum[1] += bb;
+                    const uint64_t x2 = fma2(pair_of_floats(s[i], s[i + 1]), unit2, off2);
+                    const float a = at::ex2(low_of(x2)), bb = at::ex2(high_of(x2));
+                    sum = add2(sum, pair_of_floats(a, bb));
                     pk[i >> 1] = half_pair(a, bb);
                     if constexpr (X == 2) {
                         const float2 r = Num<__half>::two(pk[i >> 1]);
                         pl[i >> 1] = half_pair(a - r.x, bb - r.y);
                     }
                 }
-                l += sum[0] + sum[1];
+                l += low_of(sum) + high_of(sum);
                 if (j > 0 && __any_sync(0xffffffffu, grow)) {    // O once P V of the page before is through
-                    if (!warp_wait(o_done + 8 * (buf ^ 1), (uint32_t)((j - 1) >> 1) & 1u, abort_s)) { *abort_s = 1; break; }
+                    if (!warp_wait(o_done + 8 * (buf ^ 1), (uint32_t)((mine + j - 1) >> 1) & 1u, abort_s)) { *abort_s = 1; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
                     for (int d = 0; d < D; d += 32) {
-                        uint32_t x[32];
-                        tc::tmem_ld32(o_at + d, x);
+                        uint32_t y[32];
+                        tc::tmem_ld32(o_at + d, y);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * alpha);
-                        tmem_st32(o_at + d, x);
+                        for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * alpha);
+                        tmem_st32(o_at + d, y);
                     }
                 }
                 tmem_st32(s_at, pk);
@@ -283,30 +402,44 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 warp_arrive(p_full + 8 * buf);
             }
-            const bool done = j == n && (n == 0 || warp_wait(o_done + 8 * (t * 2 + ((n - 1) & 1)), (uint32_t)((n - 1) >> 1) & 1u, abort_s));
-            if (!done) *abort_s = 1;
+            before += x.n;
+            mine += x.n;
+            ok = j == x.n && warp_wait(o_done + 8 * (t * 2 + ((mine - 1) & 1)), (uint32_t)((mine - 1) >> 1) & 1u, abort_s);
+            if (!ok) { *abort_s = 1; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (done) {
+            const int head = x.h * group + row % group;
+            if (x.from_start && x.to_end) {
                 const float inv = l > 0.f ? 1.0f / l : l != l ? l : 0.f;
-                T* out = (T*)p.out + at;
+                T* out = (T*)p.out + ((size_t)(x.e.row0 + row / group) * c.q_heads + head) * D;
 #pragma unroll 1
                 for (int d = 0; d < D; d += 32) {
-                    uint32_t x[32];
-                    if (n > 0) tc::tmem_ld32(o_at + d, x);
-                    else
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) x[i] = 0u;
+                    uint32_t y[32];
+                    tc::tmem_ld32(o_at + d, y);
                     if (have)
 #pragma unroll
                         for (int i = 0; i < 32; i += 8) {
-                            uint32_t y[4];
+                            uint32_t z[4];
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) y[k] = Num<T>::pack(__uint_as_float(x[i + 2 * k]) * inv, __uint_as_float(x[i + 2 * k + 1]) * inv);
-                            *reinterpret_cast<uint4*>(out + d + i) = make_uint4(y[0], y[1], y[2], y[3]);
+                            for (int k = 0; k < 4; ++k) z[k] = Num<T>::pack(__uint_as_float(y[i + 2 * k]) * inv, __uint_as_float(y[i + 2 * k + 1]) * inv);
+                            *reinterpret_cast<uint4*>(out + d + i) = make_uint4(z[0], z[1], z[2], z[3]);
                         }
                 }
-                if (have && p.stats != nullptr) p.stats[stat_row(c, p, b, row / group, h * group + row % group)] = make_float2(m == -INFINITY ? m : m - kLift, l);
+                if (have && p.stats != nullptr) p.stats[stat_row(c, p, x.b, row / group, head)] = make_float2(m == -INFINITY ? m : m - kLift, l);
+            } else {                                             // [piece][channels / 4][256 rows][4]: neighbouring lanes side by side
+                const size_t piece = (size_t)(2 * blockIdx.x + (x.from_start ? 1 : 0));
+                float4* to = reinterpret_cast<float4*>(p.many_part) + piece * (D / 4) * kManyRows + t * kTileRows + tr;
+#pragma unroll 1
+                for (int d = 0; d < D; d += 32) {
+                    uint32_t y[32];
+                    tc::tmem_ld32(o_at + d, y);
+                    if (have)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            to[(d + i) / 4 * kManyRows] = make_float4(__uint_as_float(y[i]), __uint_as_float(y[i + 1]), __uint_as_float(y[i + 2]), __uint_as_float(y[i + 3]));
+                }
+                if (have) p.many_stats[piece * kManyRows + t * kTileRows + tr] = make_float2(m, l);
             }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");     // the next piece's products go where these were read
         }
     } else if (warp < 12) {
         const int dt = tid - 8 * 32;
@@ -314,7 +447,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
         auto convert = [&](auto values, int j, uint32_t full) {  // K or V of page j, by all four warps
             constexpr bool V = decltype(values)::value;
             const uint8_t* page = sm + C::RAW_AT + (j % C::RAW) * L::BYTES;
-            const int valid = there[j & 7] ? min(kRows, e.len - j * kRows) : 0;
+            const int valid = valid_s[j & 7];
             unsigned char* to = sm + (V ? C::V_AT + (j % C::VS) * C::VB : C::K_AT + (j % C::KS) * C::KB);
             const uint32_t* codes = reinterpret_cast<const uint32_t*>(page + (V ? L::V_CODES : L::K_CODES));
             const __half2* pars = reinterpret_cast<const __half2*>(page + (V ? L::V_PARAMS : L::K_PARAMS));
@@ -345,8 +478,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             warp_arrive(full);
         };
         int i = 0;
-        for (; i < n + C::LEAD; ++i) {
-            if (i < n) {
+        for (; i < pages + C::LEAD; ++i) {
+            if (i < pages) {
                 if (!wait(raw_full + 8 * (i % C::RAW), (uint32_t)(i / C::RAW) & 1u)) break;
                 if (i >= C::KS && !wait(k_empty + 8 * (i % C::KS), (uint32_t)(i / C::KS - 1) & 1u)) break;
                 convert(std::false_type(), i, k_full + 8 * (i % C::KS));
@@ -357,35 +490,35 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             convert(std::true_type(), j, v_full + 8 * (j % C::VS));
             warp_arrive(raw_empty + 8 * (j % C::RAW));
         }
-        if (i < n + C::LEAD) *abort_s = 1;
+        if (i < pages + C::LEAD) *abort_s = 1;
     } else if (warp == 14) {
-        if (lane == 0 && n > 0) {
-            tc::mbar_expect_tx(q_full, nt * C::Q_BYTES);
-            for (int t = 0; t < nt; ++t) bulk_copy(base + C::Q_AT + t * C::Q_BYTES, p.images + row_tile(c, p, b, h, r0 / kTileRows + t) * C::Q_BYTES, C::Q_BYTES, q_full);
-        }
-        __syncwarp();
-        int lane_page = -1;
-        for (int j = 0; j < n; ++j) {
-            if ((j & 31) == 0) {                                 // a lane knows one page of 32
-                const bool in = j + lane < n;
-                lane_page = in ? c.page_table[(size_t)b * c.max_pages + j + lane] : -1;
-                if ((unsigned)lane_page >= (unsigned)c.n_pages) { if (in) raise(c, kBadPage); lane_page = -1; }
-            }
-            const int page = __shfl_sync(0xffffffffu, lane_page, j & 31);
-            const uint32_t bar = raw_full + 8 * (j % C::RAW);
-            if (j >= C::RAW && !warp_wait(raw_empty + 8 * (j % C::RAW), (uint32_t)(j / C::RAW - 1) & 1u, abort_s)) { *abort_s = 1; break; }
-            if (lane == 0) {
-                there[j & 7] = page >= 0;
-                if (page >= 0) {
-                    tc::mbar_expect_tx(bar, L::BYTES);
-                    bulk_copy(base + C::RAW_AT + (j % C::RAW) * L::BYTES, tile_of<D>(c, page, h), L::BYTES, bar);
-                } else {
-                    mbar_arrive(bar);
+        bool ok = true;
+        for (int j = 0; ok && walk.more();) {
+            const ManyPiece x = walk.next(c, p);
+            const int held = (x.e.len + kRows - 1) / kRows;      // pages; a row that sees nothing has one that is nobody's
+            int lane_page = -1;
+            for (int i = 0; i < x.n; ++i, ++j) {
+                if ((i & 31) == 0) {                             // a lane knows one page of 32
+                    const bool in = i + lane < x.n && x.p0 + i + lane < held;
+                    lane_page = in ? c.page_table[(size_t)x.b * c.max_pages + x.p0 + i + lane] : -1;
+                    if ((unsigned)lane_page >= (unsigned)c.n_pages) { if (in) raise(c, kBadPage); lane_page = -1; }
                 }
+                const int page = __shfl_sync(0xffffffffu, lane_page, i & 31);
+                const uint32_t bar = raw_full + 8 * (j % C::RAW);
+                if (j >= C::RAW && !warp_wait(raw_empty + 8 * (j % C::RAW), (uint32_t)(j / C::RAW - 1) & 1u, abort_s)) { *abort_s = 1; ok = false; break; }
+                if (lane == 0) {
+                    valid_s[j & 7] = page >= 0 ? min(kRows, x.e.len - (x.p0 + i) * kRows) : 0;
+                    if (page >= 0) {
+                        tc::mbar_expect_tx(bar, L::BYTES);
+                        bulk_copy(base + C::RAW_AT + (j % C::RAW) * L::BYTES, tile_of<D>(c, page, x.h), L::BYTES, bar);
+                    } else {
+                        mbar_arrive(bar);
+                    }
+                }
+                __syncwarp();
             }
-            __syncwarp();
         }
-    } else if (warp - 12 < nt) {
+    } else {
         // The whole warp walks the loop, so that addresses and descriptors stay in uniform registers; one lane issues.
         constexpr uint32_t kDescS = at::instr_desc_f16(kTileRows, kRows), kDescO = at::instr_desc_f16(kTileRows, D) | (1u << 16);
         const int t = warp - 12;
@@ -393,49 +526,84 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
         const uint64_t qt = tc::umma_desc(base + C::Q_AT + t * C::Q_BYTES), kd = tc::umma_desc(base + C::K_AT), vd = at::umma_desc_mn(base + C::V_AT, (uint32_t)(kRows * 128), 1024u);
         const uint32_t s0 = tm + (uint32_t)(C::S_COL + t * 128), to = tm + (uint32_t)(C::O_COL + t * 128);
-        auto issue_s = [&](int j) {                              // into the buffer of the page's parity
+        int before = 0, mine = 0, asked = 0;                     // pages of the pieces before, of all and of this tile; its pieces
+        auto issue_s = [&](int j) {                              // of page j of the piece, into the buffer of the tile's page's parity
             if (lead) {
-                const uint64_t kt = kd + (uint64_t)(j % C::KS * (C::KB >> 4));
-                const uint32_t s_to = s0 + (uint32_t)((j & 1) * 64);
+                const int k_slot = (before + j) % C::KS, buf = (mine + j) & 1;
+                const uint64_t kt = kd + (uint64_t)(k_slot * (C::KB >> 4));
+                const uint32_t s_to = s0 + (uint32_t)(buf * 64);
 #pragma unroll
                 for (int i = 0; i < (X >= 1 ? 2 : 1) * (D / 16); ++i) {
                     const int k = i % (D / 16), low = i / (D / 16);
                     at::umma_d(s_to, qt + (uint64_t)((k >> 2) * (kTileRows * 128 >> 4) + (k & 3) * 2), kt + (uint64_t)((low * C::LOW + (k >> 2) * (kRows * 128)) / 16 + (k & 3) * 2), kDescS, i != 0 ? 1u : 0u);
                 }
-                tc::umma_commit(s_full + 8 * (t * 2 + (j & 1)));
-                tc::umma_commit(k_empty + 8 * (j % C::KS));
+                tc::umma_commit(s_full + 8 * (t * 2 + buf));
+                tc::umma_commit(k_empty + 8 * k_slot);
             }
             __syncwarp();
         };
         auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait(bar, parity, abort_s); };
-        bool ok = n > 0 && wait(q_full, 0);
-        for (int j = 0; j < min(n, 2) && ok; ++j) {
-            ok = wait(k_full + 8 * j, 0);
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            issue_s(j);
-        }
-        for (int j = 0; j < n && ok; ++j) {
-            // what the products need besides the weights first: it is there long before them
-            ok = wait(v_full + 8 * (j % C::VS), (uint32_t)(j / C::VS) & 1u) && (j + 2 >= n || wait(k_full + 8 * ((j + 2) % C::KS), (uint32_t)((j + 2) / C::KS) & 1u)) &&
-                 wait(p_full + 8 * (t * 2 + (j & 1)), (uint32_t)(j >> 1) & 1u);
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (lead) {
-                const uint64_t vt = vd + (uint64_t)(j % C::VS * (C::VB >> 4));
-                const uint32_t from = s0 + (uint32_t)((j & 1) * 64);
-#pragma unroll
-                for (int i = 0; i < (X == 2 ? 3 : 1) * (kRows / 16); ++i) {
-                    const int k = i % (kRows / 16), part = i / (kRows / 16);                       // Ph Vh, Pl Vh, Ph Vl
-                    at::umma_ts(to, from + (uint32_t)((part == 1 ? 32 : 0) + 8 * k), vt + (uint64_t)((part == 2 ? C::LOW : 0) / 16 + k * (2048 >> 4)), kDescO, i != 0 || j > 0 ? 1u : 0u);
-                }
-                tc::umma_commit(o_done + 8 * (t * 2 + (j & 1)));
-                tc::umma_commit(v_empty + 8 * (j % C::VS));
+        auto wait_k = [&](int j) { return wait(k_full + 8 * ((before + j) % C::KS), (uint32_t)((before + j) / C::KS) & 1u); };
+        auto wait_v = [&](int j) { return wait(v_full + 8 * ((before + j) % C::VS), (uint32_t)((before + j) / C::VS) & 1u); };
+        auto ask = [&](const ManyPiece& x) {                     // the tile's queries, once no product reads those before
+            if (t < x.tiles && lane == 0) {
+                tc::mbar_expect_tx(q_full + 8 * t, C::Q_BYTES);
+                bulk_copy(base + C::Q_AT + t * C::Q_BYTES, p.images + row_tile(c, p, x.b, x.h, x.r0 / kTileRows + t) * C::Q_BYTES, C::Q_BYTES, q_full + 8 * t);
             }
             __syncwarp();
-            if (j + 2 < n) issue_s(j + 2);                       // behind P V, which reads the weights in that place
+        };
+        bool ok = true, more = true;
+        ManyPiece x = walk.next(c, p);
+        ask(x);
+        while (ok && more) {
+            ManyPiece y = x;
+            more = walk.more();
+            if (more) y = walk.next(c, p);
+            if (t < x.tiles) {
+                ok = wait(q_full + 8 * t, (uint32_t)(asked++) & 1u);
+                for (int j = 0; j < min(x.n, 2) && ok; ++j) {
+                    ok = wait_k(j);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    issue_s(j);
+                }
+                for (int j = 0; j < x.n && ok; ++j) {
+                    const int buf = (mine + j) & 1;
+                    // what the products need besides the weights first: it is there long before them
+                    ok = wait_v(j) && (j + 2 >= x.n || wait_k(j + 2)) && wait(p_full + 8 * (t * 2 + buf), (uint32_t)((mine + j) >> 1) & 1u);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (j == x.n - 1 && more) ask(y);            // weights of the last page: all scores are through
+                    if (lead) {
+                        const int v_slot = (before + j) % C::VS;
+                        const uint64_t vt = vd + (uint64_t)(v_slot * (C::VB >> 4));
+                        const uint32_t from = s0 + (uint32_t)(buf * 64);
+#pragma unroll
+                        for (int i = 0; i < (X == 2 ? 3 : 1) * (kRows / 16); ++i) {
+                            const int k = i % (kRows / 16), part = i / (kRows / 16);                       // Ph Vh, Pl Vh, Ph Vl
+                            at::umma_ts(to, from + (uint32_t)((part == 1 ? 32 : 0) + 8 * k), vt + (uint64_t)((part == 2 ? C::LOW : 0) / 16 + k * (2048 >> 4)), kDescO, i != 0 || j > 0 ? 1u : 0u);
+                        }
+                        tc::umma_commit(o_done + 8 * (t * 2 + buf));
+                        tc::umma_commit(v_empty + 8 * v_slot);
+                    }
+                    __syncwarp();
+                    if (j + 2 < x.n) issue_s(j + 2);             // behind P V, which reads the weights in that place
+                }
+                mine += x.n;
+            } else {                                             // no rows in this tile: keys and values are let go as they come
+                if (more) ask(y);
+                for (int j = 0; j < x.n && ok; ++j) {
+                    ok = wait_k(j);
+                    if (ok && lead) mbar_arrive(k_empty + 8 * ((before + j) % C::KS));
+                    ok = ok && wait_v(j);
+                    if (ok && lead) mbar_arrive(v_empty + 8 * ((before + j) % C::VS));
+                    __syncwarp();
+                }
+            }
+            before += x.n;
+            x = y;
         }
-        if (n > 0 && !ok) {                                      // given up: the products issued end before the block leaves (bounded)
+        if (!ok) {                                               // given up: the products issued end before the block leaves (bounded)
             *abort_s = 1;
             volatile int go_on = 0;
             if (lead) tc::umma_commit(drain + 8 * t);
@@ -448,7 +616,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
     __syncthreads();
     if (*abort_s != 0 && tid == 0) {                             // and the copies land
         volatile int go_on = 0;
-        (void)tc::mbar_wait(q_full, 0, &go_on);
+        for (int i = 0; i < 2; ++i) { (void)tc::mbar_wait(q_full + 8 * i, 0, &go_on); (void)tc::mbar_wait(q_full + 8 * i, 1, &go_on); }
         for (int i = 0; i < C::RAW; ++i) { (void)tc::mbar_wait(raw_full + 8 * i, 0, &go_on); (void)tc::mbar_wait(raw_full + 8 * i, 1, &go_on); }
         raise(c, kWait);
     }
@@ -457,6 +625,54 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
+}
+
+// Rows whose pages attend_many dealt over several blocks: maximum, sum and values of their pieces put together.  Block (w - 1, s) looks at
+// the boundary ahead of block w; if that is the first one inside a block of rows it joins 16 channels of those, a thread a row.
+// grid (blocks of attend_many - 1, D / 16).
+template <typename T, int D>
+__global__ void __launch_bounds__(kManyRows) attend_join_kernel(const Cache c, const AttnParams p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int pairs = c.batch * p.many_tiles, all = p.many_starts[pairs], step = many_step(p, all), w = blockIdx.x + 1, group = c.q_heads / c.kv_heads;
+    const int64_t u = (int64_t)w * step;
+    if (u >= all) return;
+    const int pair = pair_of(p.many_starts, pairs, 0, (int)u), b = pair / p.many_tiles, tile = pair - b * p.many_tiles;
+    const Entry e = entry_of(c, p, b);
+    const int each = many_pages(p, e, group, tile), in = (int)u - p.many_starts[pair], h = in / each, at = (int)u - (in - h * each);       // at: the rows' first unit
+    const int row = tile * kManyRows + threadIdx.x, i = row / group, head = h * group + row - i * group;
+    if (at == u || at < (w - 1) * step || row >= e.n * group) return;
+    const int last = (at + each - 1) / step;                     // blocks w - 1 .. last
+    auto slot = [&](int k) { return (size_t)(2 * k + (k == w - 1 ? 1 : 0)); };
+    const float2* stats = p.many_stats + threadIdx.x;
+    float top = -INFINITY, sum = 0.f;
+    for (int k = w - 1; k <= last; ++k) top = fmaxf(top, stats[slot(k) * kManyRows].x);
+    float v[16];
+#pragma unroll
+    for (int d = 0; d < 16; ++d) v[d] = 0.f;
+    const float4* part = reinterpret_cast<const float4*>(p.many_part) + (size_t)blockIdx.y * 4 * kManyRows + threadIdx.x;
+    for (int k = w - 1; k <= last; ++k) {
+        const float2 s = stats[slot(k) * kManyRows];
+        const float f = s.x == -INFINITY && s.y == s.y ? 0.f : at::ex2(s.x - top);           // a sum that is no number stays one
+        const float4* from = part + slot(k) * (D / 4) * kManyRows;
+        sum = fmaf(s.y, f, sum);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float4 y = from[q * kManyRows];
+            v[4 * q] = fmaf(y.x, f, v[4 * q]);
+            v[4 * q + 1] = fmaf(y.y, f, v[4 * q + 1]);
+            v[4 * q + 2] = fmaf(y.z, f, v[4 * q + 2]);
+            v[4 * q + 3] = fmaf(y.w, f, v[4 * q + 3]);
+        }
+    }
+    const float inv = sum > 0.f ? 1.0f / sum : sum != sum ? sum : 0.f;
+    uint32_t z[8];
+#pragma unroll
+    for (int d = 0; d < 8; ++d) z[d] = Num<T>::pack(v[2 * d] * inv, v[2 * d + 1] * inv);
+    uint4* out = reinterpret_cast<uint4*>((T*)p.out + ((size_t)(e.row0 + i) * c.q_heads + head) * D + blockIdx.y * 16);
+    out[0] = make_uint4(z[0], z[1], z[2], z[3]);
+    out[1] = make_uint4(z[4], z[5], z[6], z[7]);
+    if (blockIdx.y == 0 && p.stats != nullptr) p.stats[stat_row(c, p, b, i, head)] = make_float2(top == -INFINITY ? top : top - kLift, sum);
 }
 
 template <int D>
