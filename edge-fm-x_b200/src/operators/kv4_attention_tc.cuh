@@ -122,10 +122,45 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+// 2^x of two numbers without the exponential unit: x = n + f, n the nearest integer (it is in the low bits of x + 1.5 2^23), 2^f on
+// [-1/2, 1/2] by the polynomial of degree 4 of least largest relative error, 2^-18.5 (found by linear programming over 4001 Chebyshev
+// points), n added to the exponent.  Below 2^-125 it stays there.
+__device__ __forceinline__ void ex2_pair(uint64_t x, float& a, float& b) {
+    const uint64_t big = pair_of_floats(12582912.0f, 12582912.0f);
+    x = pair_of_floats(fmaxf(low_of(x), -125.0f), fmaxf(high_of(x), -125.0f));
+    const uint64_t n = add2(x, big), f = fma2(add2(n, pair_of_floats(-12582912.0f, -12582912.0f)), pair_of_floats(-1.0f, -1.0f), x);
+    uint64_t y = fma2(f, pair_of_floats(0.00957053154706955f, 0.00957053154706955f), pair_of_floats(0.05591866374015808f, 0.05591866374015808f));
+    y = fma2(y, f, pair_of_floats(0.24024735391139984f, 0.24024735391139984f));
+    y = fma2(y, f, pair_of_floats(0.6931216716766357f, 0.6931216716766357f));
+    y = fma2(y, f, pair_of_floats(0.9999992847442627f, 0.9999992847442627f));
+    a = __uint_as_float((uint32_t)y + ((uint32_t)n << 23));
+    b = __uint_as_float((uint32_t)(y >> 32) + ((uint32_t)(n >> 32) << 23));
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
+}
+// Three waits at once: polled one behind the other a wait that is over takes some 200 cycles each.
+struct Phase { uint32_t bar, parity; };
+__device__ __forceinline__ bool warp_wait(const Phase& a, const Phase& b, const Phase& c, volatile int* abort_flag) {
+    for (int i = 0; i < kSpins; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n"
+            ".reg .pred p, q, r;\n"
+            "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+            "mbarrier.test_wait.parity.shared::cta.b64 q, [%3], %4;\n"
+            "mbarrier.test_wait.parity.shared::cta.b64 r, [%5], %6;\n"
+            "and.pred p, p, q;\n"
+            "and.pred p, p, r;\n"
+            "selp.u32 %0, 1, 0, p;\n"
+            "}\n"
+            : "=r"(ok) : "r"(a.bar), "r"(a.parity), "r"(b.bar), "r"(b.parity), "r"(c.bar), "r"(c.parity) : "memory");
+        if (__all_sync(0xffffffffu, ok)) return true;
+        if ((i & 0xff) == 0xff && __any_sync(0xffffffffu, *abort_flag != 0)) return false;
+    }
+    return false;
 }
 __device__ __forceinline__ uint32_t elect_one() {
     uint32_t lead;
@@ -375,7 +410,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
 #pragma unroll
                 for (int i = 0; i < 64; i += 2) {
                     const uint64_t x2 = fma2(pair_of_floats(s[i], s[i + 1]), unit2, off2);
-                    const float a = at::ex2(low_of(x2)), bb = at::ex2(high_of(x2));
+                    float a, bb;
+                    if (X == 0 && (i & 6) == 6) {                // a quarter by arithmetic: the exponential unit is what the rest waits for
+                        ex2_pair(x2, a, bb);
+                    } else {
+                        a = at::ex2(low_of(x2));
+                        bb = at::ex2(high_of(x2));
+                    }
                     sum = add2(sum, pair_of_floats(a, bb));
                     pk[i >> 1] = half_pair(a, bb);
                     if constexpr (X == 2) {
@@ -543,8 +584,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             __syncwarp();
         };
         auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait(bar, parity, abort_s); };
-        auto wait_k = [&](int j) { return wait(k_full + 8 * ((before + j) % C::KS), (uint32_t)((before + j) / C::KS) & 1u); };
-        auto wait_v = [&](int j) { return wait(v_full + 8 * ((before + j) % C::VS), (uint32_t)((before + j) / C::VS) & 1u); };
+        auto k_of = [&](int j) { return Phase{k_full + 8 * ((before + j) % C::KS), (uint32_t)((before + j) / C::KS) & 1u}; };
+        auto v_of = [&](int j) { return Phase{v_full + 8 * ((before + j) % C::VS), (uint32_t)((before + j) / C::VS) & 1u}; };
+        auto wait_k = [&](int j) { return wait(k_of(j).bar, k_of(j).parity); };
+        auto wait_v = [&](int j) { return wait(v_of(j).bar, v_of(j).parity); };
         auto ask = [&](const ManyPiece& x) {                     // the tile's queries, once no product reads those before
             if (t < x.tiles && lane == 0) {
                 tc::mbar_expect_tx(q_full + 8 * t, C::Q_BYTES);
@@ -569,8 +612,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
                 }
                 for (int j = 0; j < x.n && ok; ++j) {
                     const int buf = (mine + j) & 1;
-                    // what the products need besides the weights first: it is there long before them
-                    ok = wait_v(j) && (j + 2 >= x.n || wait_k(j + 2)) && wait(p_full + 8 * (t * 2 + buf), (uint32_t)((mine + j) >> 1) & 1u);
+                    const Phase weights{p_full + 8 * (t * 2 + buf), (uint32_t)((mine + j) >> 1) & 1u};
+                    ok = warp_wait(v_of(j), j + 2 < x.n ? k_of(j + 2) : weights, weights, abort_s);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     if (j == x.n - 1 && more) ask(y);            // weights of the last page: all scores are through
