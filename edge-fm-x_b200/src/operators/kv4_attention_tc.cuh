@@ -844,26 +844,35 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
         }
     } else if (warp < 12) {
         const int tr = tid - 256;
+        struct Row { float2 s; float unit; int seen; };
+        auto look = [&](int i) {                                 // a row's parameters, a step ahead of their use
+            const int row = first_row + i * C::ROWS + tr;
+            const bool have = i < n && row < rows;
+            const int qr = have ? row / group : 0, head = h * group + (have ? row - qr * group : 0);
+            Row x;
+            x.s = have ? p.stats[stat_row(c, p, b, qr, head)] : make_float2(-INFINITY, 0.f);
+            x.unit = have ? p.units[row_tile(c, p, b, h, first_row / C::ROWS + i) * kTileRows + tr] : 1.0f;         // not 0: times -inf
+            x.seen = min(e.len, e.len - e.n + qr + 1);
+            return x;
+        };
+        Row x = look(0);
         int i = 0;
         for (; i < n; ++i) {
-            const int st = i & 1, row = first_row + i * C::ROWS + tr;
+            const int st = i & 1;
+            const Row now = x;
+            x = look(i + 1);
             // the products and the sums of two steps before have read this place
             if (i >= 2 && !(wait(q_empty + 8 * st, (uint32_t)(i / 2 - 1) & 1u) && wait(s_empty + 8 * st, (uint32_t)(i / 2 - 1) & 1u))) break;
-            const bool have = row < rows;
-            const int qr = have ? row / group : 0, head = h * group + (have ? row % group : 0);
-            const float2 s = have ? p.stats[stat_row(c, p, b, qr, head)] : make_float2(-INFINITY, 0.f);
-            const size_t tile = row_tile(c, p, b, h, first_row / C::ROWS + i);
             if (tr == 0) {                                       // the operand as it is, the rows' parameters by these four warps
                 tc::mbar_expect_tx(q_full + 8 * st, C::Q_BYTES);
-                bulk_copy(base + C::Q_AT + st * C::Q_BYTES, p.images + tile * C::Q_BYTES, C::Q_BYTES, q_full + 8 * st);
+                bulk_copy(base + C::Q_AT + st * C::Q_BYTES, p.images + row_tile(c, p, b, h, first_row / C::ROWS + i) * C::Q_BYTES, C::Q_BYTES, q_full + 8 * st);
             }
-            const float unit = p.units[tile * kTileRows + tr];
-            const bool sees = s.x != -INFINITY;                  // a row that sees nothing: weights of 0
+            const bool sees = now.s.x != -INFINITY;              // a row that sees nothing: weights of 0
             float* par = reinterpret_cast<float*>(sm + C::PAR_AT) + st * 4 * C::ROWS + tr;
-            par[0] = unit;
-            par[C::ROWS] = sees ? -s.x : 0.f;
-            par[2 * C::ROWS] = sees ? 1.0f / s.y : 0.f;
-            reinterpret_cast<int*>(par)[3 * C::ROWS] = sees ? min(e.len, e.len - e.n + qr + 1) : 0;
+            par[0] = now.unit;
+            par[C::ROWS] = sees ? -now.s.x : 0.f;
+            par[2 * C::ROWS] = sees ? 1.0f / now.s.y : 0.f;
+            reinterpret_cast<int*>(par)[3 * C::ROWS] = sees ? now.seen : 0;
             warp_arrive(q_full + 8 * st);
         }
         if (i < n) *abort_s = 1;
