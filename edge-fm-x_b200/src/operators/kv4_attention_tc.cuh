@@ -722,14 +722,14 @@ template <int D>
 struct WeightsCfg {
     static constexpr int G = D / 64, KEYS = 128, ROWS = 128, K_PART = Tile<D>::V_CODES;       // keys of a block, packed rows of a step; codes and parameters of a page's keys
     static constexpr int K_BYTES = KEYS * 128 * G, Q_BYTES = ROWS * 128 * G;                 // K: of its high and of its low half
-    static constexpr int K_AT = 0, Q_AT = 2 * K_BYTES, PAR_AT = Q_AT + 2 * Q_BYTES, SUM_AT = PAR_AT + 2 * 4 * ROWS * 4, RAW_AT = SUM_AT + KEYS * 4, BARS = RAW_AT + 2 * K_PART;
+    static constexpr int K_AT = 0, Q_AT = 2 * K_BYTES, PAR_AT = Q_AT + 2 * Q_BYTES, SUM_AT = PAR_AT + 2 * 3 * ROWS * 4, RAW_AT = SUM_AT + KEYS * 4, BARS = RAW_AT + 2 * K_PART;
     static constexpr size_t SMEM = BARS + 96 + 1024;
 };
 constexpr int kWeightThreads = 13 * 32;
 
 // Summed weights where scores were not kept: S^T = K Q^T once more, 128 keys against 128 packed rows at a time, keys as a pair high + low of
 // fp16 so that scores have 32-bit accuracy.  A key is a lane of tensor memory and two threads of warps 0-7, each of which adds up its weights
-// 2^(s - m) / l over half the rows of a step, in order: no atomics, no shuffles.  Warps 8-11 bring the rows' operand and (unit, m, 1 / l),
+// 2^(s - m - log2 l) over half the rows of a step, in order: no atomics, no shuffles.  Warps 8-11 bring the rows' operand and (unit, m + log2 l),
 // warp 12 issues the products.
 // grid (blocks of 128 cached rows, kv heads, batch).  Bound: exponentials and tensor pipe alike (128 x 128 of them in 1024 cycles, two products of K = D).
 template <typename T, int D>
@@ -740,8 +740,8 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
     extern __shared__ unsigned char weights_smem[];
     const uint32_t raw_base = tc::smem_u32(weights_smem), base = (raw_base + 1023u) & ~1023u;
     unsigned char* sm = weights_smem + (base - raw_base);
-    const uint32_t bars = base + C::BARS, raw_full = bars, q_full = bars + 8, q_empty = bars + 24, s_full = bars + 40, s_empty = bars + 56, drain = bars + 72;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::BARS + 80);
+    const uint32_t bars = base + C::BARS, raw_full = bars, q_full = bars + 8, q_empty = bars + 24, s_full = bars + 40, s_empty = bars + 56, drain = bars + 72, k_full = bars + 80;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::BARS + 88);
     volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int tid = threadIdx.x, warp = tid >> 5, h = blockIdx.y, b = blockIdx.z, group = c.q_heads / c.kv_heads, key0 = blockIdx.x * C::KEYS;
 
@@ -753,6 +753,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
     for (int i = 0; i < 2; ++i) page[i] = key0 + i * kRows < e.len ? page_of(c, b, key0 / kRows + i) : -1;
     if (tid == 0) {
         tc::mbar_init(raw_full, 1);
+        tc::mbar_init(k_full, 8);
         tc::mbar_init(drain, 1);
         for (int i = 0; i < 2; ++i) { tc::mbar_init(q_full + 8 * i, 5); tc::mbar_init(q_empty + 8 * i, 1); tc::mbar_init(s_full + 8 * i, 1); tc::mbar_init(s_empty + 8 * i, 8); }
         *abort_s = 0;
@@ -766,14 +767,19 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(tmem_slot)), "r"(256) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (!warp_wait(raw_full, 0, abort_s)) *abort_s = 1;
-    if (warp < 8 && *abort_s == 0) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    pdl_launch_dependents();                                     // not before this block has its tensor memory
+    if (warp < 8) {                                              // the keys, while the other warps fetch rows
+        const bool came = warp_wait(raw_full, 0, abort_s);
+        if (!came) *abort_s = 1;
 #pragma unroll
         for (int it = 0; it < 2; ++it) {
             const int r = it * 64 + (tid >> 2), x = tid & 3, pr = r % kRows;     // row of the block, of its page; quarter of its groups
             const uint8_t* raw = sm + C::RAW_AT + it * C::K_PART;
-            const bool have = page[it] >= 0 && key0 + r < e.len;
+            const bool have = came && page[it] >= 0 && key0 + r < e.len;
             uint32_t w[G][2];
             quarter_words<D, false>(reinterpret_cast<const uint32_t*>(raw + L::K_CODES), pr, x, w);
 #pragma unroll
@@ -790,12 +796,8 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
             }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        warp_arrive(k_full);
     }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = *tmem_slot;
-    pdl_launch_dependents();                                     // not before this block has its tensor memory
     pdl_wait();
 
     const int rows = e.n * group, first_row = max(0, key0 - (e.len - e.n)) * group / C::ROWS * C::ROWS;       // rows before do not see the block
@@ -803,13 +805,13 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
     auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait(bar, parity, abort_s); };
     if (warp < 8) {
         const int key = key0 + (tid & 127), half = warp >> 2;         // which half of a step's rows
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint64_t sum[2] = {0, 0};
         int i = 0;
         for (; i < n; ++i) {
             const int st = i & 1, r0 = first_row + i * C::ROWS;
             if (!wait(s_full + 8 * st, (uint32_t)(i >> 1) & 1u)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const float* par = reinterpret_cast<const float*>(sm + C::PAR_AT) + st * 4 * C::ROWS;      // [unit | -m | 1 / l | rows seen][row]
+            const float* par = reinterpret_cast<const float*>(sm + C::PAR_AT) + st * 3 * C::ROWS;      // [unit | -m - log2 l | rows seen][row]
             const bool interior = e.len - e.n + r0 / group >= key0 + C::KEYS - 1;          // the step's first row sees every key
             {
                 const int q = half * 64;
@@ -817,16 +819,14 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
                 tmem_ld64(tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(st * C::ROWS + q), s);
                 if (!interior) {
 #pragma unroll
-                    for (int k = 0; k < 64; ++k) if (key >= reinterpret_cast<const int*>(par)[3 * C::ROWS + q + k]) s[k] = -INFINITY;
+                    for (int k = 0; k < 64; ++k) if (key >= reinterpret_cast<const int*>(par)[2 * C::ROWS + q + k]) s[k] = -INFINITY;
                 }
 #pragma unroll
                 for (int k = 0; k < 64; k += 4) {
-                    const float4 u = *reinterpret_cast<const float4*>(par + q + k), m = *reinterpret_cast<const float4*>(par + C::ROWS + q + k),
-                                 l = *reinterpret_cast<const float4*>(par + 2 * C::ROWS + q + k);
-                    sum[0] = fmaf(at::ex2(fmaf(s[k], u.x, m.x)), l.x, sum[0]);
-                    sum[1] = fmaf(at::ex2(fmaf(s[k + 1], u.y, m.y)), l.y, sum[1]);
-                    sum[2] = fmaf(at::ex2(fmaf(s[k + 2], u.z, m.z)), l.z, sum[2]);
-                    sum[3] = fmaf(at::ex2(fmaf(s[k + 3], u.w, m.w)), l.w, sum[3]);
+                    const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(par + q + k), m = *reinterpret_cast<const ulonglong2*>(par + C::ROWS + q + k);
+                    const uint64_t x = fma2(pair_of_floats(s[k], s[k + 1]), u.x, m.x), y = fma2(pair_of_floats(s[k + 2], s[k + 3]), u.y, m.y);
+                    sum[0] = add2(sum[0], pair_of_floats(at::ex2(low_of(x)), at::ex2(high_of(x))));
+                    sum[1] = add2(sum[1], pair_of_floats(at::ex2(low_of(y)), at::ex2(high_of(y))));
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -834,7 +834,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
         }
         if (i < n) *abort_s = 1;
         float* other = reinterpret_cast<float*>(sm + C::SUM_AT);
-        const float mine = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        const float mine = (low_of(sum[0]) + high_of(sum[0])) + (low_of(sum[1]) + high_of(sum[1]));
         if (half == 1) other[tid & 127] = mine;
         asm volatile("bar.sync 1, 256;" ::: "memory");
         const int pg = page[(tid & 127) >> 6];
@@ -868,11 +868,10 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
                 bulk_copy(base + C::Q_AT + st * C::Q_BYTES, p.images + row_tile(c, p, b, h, first_row / C::ROWS + i) * C::Q_BYTES, C::Q_BYTES, q_full + 8 * st);
             }
             const bool sees = now.s.x != -INFINITY;              // a row that sees nothing: weights of 0
-            float* par = reinterpret_cast<float*>(sm + C::PAR_AT) + st * 4 * C::ROWS + tr;
+            float* par = reinterpret_cast<float*>(sm + C::PAR_AT) + st * 3 * C::ROWS + tr;
             par[0] = now.unit;
-            par[C::ROWS] = sees ? -now.s.x : 0.f;
-            par[2 * C::ROWS] = sees ? 1.0f / now.s.y : 0.f;
-            reinterpret_cast<int*>(par)[3 * C::ROWS] = sees ? now.seen : 0;
+            par[C::ROWS] = sees ? -now.s.x - log2f(now.s.y) : -INFINITY;
+            reinterpret_cast<int*>(par)[2 * C::ROWS] = sees ? now.seen : 0;
             warp_arrive(q_full + 8 * st);
         }
         if (i < n) *abort_s = 1;
@@ -880,7 +879,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
         constexpr uint32_t kDesc = at::instr_desc_f16(C::KEYS, C::ROWS);
         const uint32_t lead = elect_one(), tm = __shfl_sync(0xffffffffu, tmem, 0);
         const uint64_t kd = tc::umma_desc(base + C::K_AT), qd = tc::umma_desc(base + C::Q_AT);
-        bool ok = true;
+        bool ok = n == 0 || wait(k_full, 0);
         for (int i = 0; i < n && ok; ++i) {
             const int st = i & 1;
             ok = (i < 2 || wait(s_empty + 8 * st, (uint32_t)(i / 2 - 1) & 1u)) && wait(q_full + 8 * st, (uint32_t)(i >> 1) & 1u);
