@@ -187,7 +187,7 @@ AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
         const int64_t tiles_all = std::min<int64_t>((int64_t)c->batch * p.many_tiles, c->batch + (int64_t)a->max_rows * (c->q_heads / c->kv_heads) / kv4::kManyRows);
         p.many_units = tiles_all * c->kv_heads * pages;
         p.many_blocks = (int)std::min<int64_t>(kSms, (p.many_units + kv4::kManyStep - 1) / kv4::kManyStep);
-        p.many_starts = round_up((int64_t)c->batch * p.many_tiles + 1, 4);
+        p.many_starts = round_up((int64_t)c->batch * p.many_tiles + 2, 4);
         p.many_stats = 2 * 2 * (int64_t)p.many_blocks * kv4::kManyRows;
         p.many_part = 2 * (int64_t)p.many_blocks * kv4::kManyRows * c->head_dim;
     }

@@ -32,7 +32,7 @@ struct AttnParams {
     float* units;             // [batch, kv_heads, row_tiles][128] what their scores are multiplied with; where many rows are a sequence's
     int row_tiles;
     int many_tiles, many_blocks;      // blocks of 256 packed rows a sequence may have; blocks of attend_many
-    int32_t* many_starts;     // [batch x many_tiles + 1] its units ahead, and all of them
+    int32_t* many_starts;     // [batch x many_tiles + 2] its units ahead, all of them, and those of each if blocks of rows stay whole
     float2* many_stats;       // [2 many_blocks][256] and
     float* many_part;         // [2 many_blocks][D / 4][256][4] what part_stats and part are, of its pieces
     float* scores;            // [batch, kv_heads, 8 nt][score_ld] scores in units of log2; null: not wanted

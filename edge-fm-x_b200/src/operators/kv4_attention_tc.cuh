@@ -228,39 +228,58 @@ __device__ __forceinline__ int many_pages(const AttnParams& p, const Entry& e, i
     const int last = min(rows, (tile + 1) * kManyRows) - 1;
     return max(1, (min(e.len, e.len - e.n + last / group + 1) + kRows - 1) / kRows);
 }
-__device__ __forceinline__ int many_step(const AttnParams& p, int all) { return max(kManyStep, (all + p.many_blocks - 1) / p.many_blocks); }
-// many_starts[b * many_tiles + tile]: units ahead, by one block of kTileRows threads
+// Joining costs as much as some ten pages of a block.  Where every (block of rows, kv head) can have an SM and none has that many more than
+// its even share they stay whole: they all get as many units as the longest then, which many_starts has behind the sums (otherwise 0).
+// 8 sequences with 256 new rows on 1000, 16 query heads on 2 of 128 (128 blocks of 20 pages): 46 us whole, 57 dealt evenly; 4 of them
+// (64 blocks, 8 pages an SM) 45 dealt evenly.
+constexpr int kJoinPages = 10;
+__device__ __forceinline__ int many_step(const AttnParams& p, int all, int whole) { return whole > 0 ? whole : max(kManyStep, (all + p.many_blocks - 1) / p.many_blocks); }
+// many_starts[b * many_tiles + tile]: units ahead; all; units of each, if they stay whole.  By one block of kTileRows threads
 __device__ __forceinline__ void lay_out_units(const Cache& c, const AttnParams& p) {
-    __shared__ int64_t sums[kTileRows / 32];
+    __shared__ int64_t sums[kTileRows / 32], counts[kTileRows / 32];
+    __shared__ int most_s;
     const int group = c.q_heads / c.kv_heads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t pairs = (int64_t)c.batch * p.many_tiles, per = (pairs + kTileRows - 1) / kTileRows, lo = min(pairs, (int64_t)threadIdx.x * per), hi = min(pairs, lo + per);
-    int64_t own = 0;
+    if (threadIdx.x == 0) most_s = 0;
+    __syncthreads();
+    int64_t own = 0, count = 0;                                  // units, and blocks of rows that have any; most: of one
+    int most = 0;
     auto walk = [&](auto&& visit) {
         int b = (int)(lo / p.many_tiles), tile = (int)(lo % p.many_tiles);
         Entry e{};
         if (lo < hi) e = entry_of(c, p, b);
         for (int64_t i = lo; i < hi; ++i) {
-            visit(i, many_pages(p, e, group, tile) * c.kv_heads);
+            visit(i, many_pages(p, e, group, tile));
             if (++tile == p.many_tiles) {
                 tile = 0;
                 if (++b < c.batch) e = entry_of(c, p, b);
             }
         }
     };
-    walk([&](int64_t, int n) { own += n; });
-    int64_t upto = own;
+    walk([&](int64_t, int n) { own += (int64_t)n * c.kv_heads; count += n > 0 ? c.kv_heads : 0; most = max(most, n); });
+    atomicMax(&most_s, most);
+    int64_t upto = own, upto_n = count;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o), n = __shfl_up_sync(0xffffffffu, upto_n, o);
+        if (lane >= o) { upto += v; upto_n += n; }
     }
-    if (lane == 31) sums[warp] = upto;
+    if (lane == 31) { sums[warp] = upto; counts[warp] = upto_n; }
     __syncthreads();
-    int64_t all = 0;
-    for (int w = 0; w < kTileRows / 32; ++w) { if (w < warp) upto += sums[w]; all += sums[w]; }
-    int64_t at = upto - own;                                     // row counts that lie may add up to more than the caller's sizes allow: cut off there
-    walk([&](int64_t i, int n) { p.many_starts[i] = (int)min(at, kMostUnits); at += n; });
-    if (threadIdx.x == 0) p.many_starts[pairs] = (int)min(all, kMostUnits);
+    int64_t all = 0, all_n = 0;
+    for (int w = 0; w < kTileRows / 32; ++w) {
+        if (w < warp) { upto += sums[w]; upto_n += counts[w]; }
+        all += sums[w];
+        all_n += counts[w];
+    }
+    const bool whole = all_n <= p.many_blocks && most_s <= (all + p.many_blocks - 1) / p.many_blocks + kJoinPages;
+    // row counts that lie may add up to more than the caller's sizes allow: cut off there
+    int64_t at = whole ? (upto_n - count) * most_s : upto - own;
+    walk([&](int64_t i, int n) { p.many_starts[i] = (int)min(at, kMostUnits); at += (int64_t)(whole && n > 0 ? most_s : n) * c.kv_heads; });
+    if (threadIdx.x == 0) {
+        p.many_starts[pairs] = (int)min(whole ? all_n * most_s : all, kMostUnits);
+        p.many_starts[pairs + 1] = whole ? most_s : 0;
+    }
 }
 // Of a (sequence, block of rows) whose units begin at or before `from`, the one that has unit u, by a warp: 32 at a time.
 __device__ __forceinline__ int pair_of(const int32_t* starts, int pairs, int from, int u) {
@@ -280,9 +299,10 @@ __device__ __forceinline__ int pair_of(const int32_t* starts, int pairs, int fro
 // Pages [p0, p0 + n) of a (sequence, block of rows, kv head), as a warp walks a block's range of units.
 struct ManyPiece { Entry e; int b, h, r0, tiles, p0, n; bool from_start, to_end; };
 struct ManyWalk {
-    int u, u1, pair, base, pairs;
+    int u, u1, pair, base, pairs, whole;
     __device__ __forceinline__ ManyWalk(const Cache& c, const AttnParams& p, int block) : pair(0), base(0), pairs(c.batch * p.many_tiles) {
-        const int all = p.many_starts[pairs], step = many_step(p, all);
+        whole = p.many_starts[pairs + 1];
+        const int all = p.many_starts[pairs], step = many_step(p, all, whole);
         u = (int)min((int64_t)all, (int64_t)block * step);
         u1 = min(all, u + step);
     }
@@ -294,15 +314,15 @@ struct ManyWalk {
         x.b = pair / p.many_tiles;
         const int tile = pair - x.b * p.many_tiles, group = c.q_heads / c.kv_heads;
         x.e = entry_of(c, p, x.b);
-        const int each = many_pages(p, x.e, group, tile), in = u - base;
-        x.h = in / each;
-        x.p0 = in - x.h * each;
+        const int each = many_pages(p, x.e, group, tile), stride = whole > 0 ? whole : each, in = u - base;
+        x.h = in / stride;
+        x.p0 = in - x.h * stride;
         x.n = __shfl_sync(0xffffffffu, min(each - x.p0, u1 - u), 0);
         x.r0 = tile * kManyRows;
         x.tiles = x.e.n * group - x.r0 > kTileRows ? 2 : 1;
         x.from_start = x.p0 == 0;
         x.to_end = x.p0 + x.n == each;
-        u += x.n;
+        u += whole > 0 ? whole : x.n;
         return x;
     }
 };
@@ -346,8 +366,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
 
     pdl_wait();
     ManyWalk walk(c, p, blockIdx.x);
-    const int pages = walk.u1 - walk.u;                          // of all pieces
-    if (pages <= 0) return;
+    if (!walk.more()) return;
+    const int pages = walk.whole > 0 ? ManyWalk(walk).next(c, p).n : walk.u1 - walk.u;      // of all pieces
     if (tid == 0) {
         for (int i = 0; i < C::RAW; ++i) { tc::mbar_init(raw_full + 8 * i, 1); tc::mbar_init(raw_empty + 8 * i, 4); }
         for (int i = 0; i < 2; ++i) { tc::mbar_init(q_full + 8 * i, 1); tc::mbar_init(drain + 8 * i, 1); }
@@ -677,7 +697,8 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kManyRows) attend_join_kernel(const Cache c, const AttnParams p) {
     pdl_wait();
     pdl_launch_dependents();
-    const int pairs = c.batch * p.many_tiles, all = p.many_starts[pairs], step = many_step(p, all), w = blockIdx.x + 1, group = c.q_heads / c.kv_heads;
+    const int pairs = c.batch * p.many_tiles, all = p.many_starts[pairs], step = many_step(p, all, 0), w = blockIdx.x + 1, group = c.q_heads / c.kv_heads;
+    if (p.many_starts[pairs + 1] > 0) return;                    // they stayed whole
     const int64_t u = (int64_t)w * step;
     if (u >= all) return;
     const int pair = pair_of(p.many_starts, pairs, 0, (int)u), b = pair / p.many_tiles, tile = pair - b * p.many_tiles;
