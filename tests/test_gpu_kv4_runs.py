@@ -31,6 +31,14 @@ def test_attention_wide_groups_and_short_portions(qh, kh, d, dtype, counts, lens
     run_attention(c, counts, lens, dtype, mass, shared_tiles=True)
 
 
+@pytest.mark.parametrize("counts,lens", [([128] * 8, [400 + 7 * i for i in range(8)]), ([128] * 8, [150, 150, 900, 150, 150, 150, 150, 150]), ([300, 2, 40], [2000, 2, 1200])])
+@pytest.mark.parametrize("mass", [False, True])
+def test_attention_even_and_uneven_blocks_of_rows(counts, lens, mass):
+    """Blocks of rows of much the same length, which stay whole, and one far longer than the rest, which does not."""
+    c = kv.KV4(16, 2, 128, lens, None, "bf16", seed=3).fill()
+    run_attention(c, counts, lens, "bf16", mass, shared_tiles=True)
+
+
 def test_attention_more_pages_than_a_warp_asks_for_at_once():
     """64 sequences of up to 7100 rows on the same pages: every warp has more than 32 of a row's."""
     B, kh, d, L = 64, 8, 64, 7100
