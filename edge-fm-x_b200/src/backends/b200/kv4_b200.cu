@@ -84,7 +84,7 @@ efm_status device_info(const char* call, int device, DeviceInfo& info) {
         if (e == cudaSuccess) e = cudaDeviceGetAttribute(&smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);
         if (e != cudaSuccess) return cuda_fail(nullptr, e, call);
         if (major != 10 || minor != 0) return fail(nullptr, EFM_ERR_CUDA, std::string(call) + ": needs an sm_100 device");
-        e = cudaFuncSetAttribute(kv4::evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem - kEvictSmemReserve);
+        e = cudaFuncSetAttribute(kv4::evict_select_kernel<kv4::kKeepMany>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem - kEvictSmemReserve);
         if (e == cudaSuccess) e = more_smem<__nv_bfloat16, 64>();
         if (e == cudaSuccess) e = more_smem<__nv_bfloat16, 128>();
         if (e == cudaSuccess) e = more_smem<__half, 64>();
@@ -404,7 +404,9 @@ efm_status efm_b200_op_kv4_evict(const efm_kv4_cache* cache, const efm_kv4_evict
         p.keys_cap = (int)std::min<int64_t>(capacity(cache), (info.smem - kEvictSmemReserve) / 4);
         Launcher L = on_stream(stream);
         const kv4::Cache c = device_cache(cache);
-        L.launch(kv4::evict_select_kernel, dim3(cache->kv_heads, cache->batch), dim3(kv4::kEvictThreads), (size_t)p.keys_cap * 4, c, p);
+        const dim3 heads(cache->kv_heads, cache->batch);
+        if (capacity(cache) <= kv4::kKeepFew * kv4::kEvictThreads) L.launch(kv4::evict_select_kernel<kv4::kKeepFew>, heads, dim3(kv4::kEvictThreads), (size_t)p.keys_cap * 4, c, p);
+        else L.launch(kv4::evict_select_kernel<kv4::kKeepMany>, heads, dim3(kv4::kEvictThreads), (size_t)p.keys_cap * 4, c, p);
         if (!p.inline_moves) {
             const int per = kv4::kMoveThreads / 16, all = (p.most_moves + per - 1) / per;
             const int parts = (int)std::min<int64_t>(all, std::max<int64_t>(1, (int64_t)8 * info.sms / ((int64_t)cache->batch * cache->kv_heads)));

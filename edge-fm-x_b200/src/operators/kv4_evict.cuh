@@ -26,7 +26,9 @@ struct EvictParams {
 
 constexpr int kEvictThreads = 512, kEvictWarps = kEvictThreads / 32, kBins = 256, kCopies = 8, kMoveThreads = 256;
 constexpr int kInlineMoves = 256;         // rows: two rounds of a block's 128 rows, below the cost of a launch
-constexpr int kKeep = 10;                 // rows a thread holds in registers: 5120 a round
+// Rows a thread holds in registers, a round's 512: 5120 a round, or 1024 where a sequence cannot have more, which leaves out most of what
+// is unrolled over them.
+constexpr int kKeepMany = 10, kKeepFew = 2;
 
 // Ascending order of masses as unsigned numbers: NaN 0, protected rows the largest.
 __device__ __forceinline__ uint32_t evict_key(float mass, bool always) {
@@ -77,6 +79,7 @@ __device__ __forceinline__ void move_rows(const Cache& c, const EvictParams& p, 
 
 // grid (kv heads, batch).  Barriers cost more than arithmetic here: rows are counted by ballots, and every warp adds up the warps' counts
 // for itself.
+template <int kKeep>
 __global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const Cache c, const EvictParams p) {
     extern __shared__ uint32_t keys[];
     __shared__ int hist[kBins * kCopies], counts[2][kKeep * kEvictWarps + 1], digit_sums[2][kEvictWarps], found[2], newest_s;
@@ -106,8 +109,8 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const Ca
             }
         return;
     }
-    // One walk over the rows: keys into shared memory where they fit (a longer sequence computes them again), those of the first 5120 in
-    // registers.  Where the outputs are other arrays every row below the budget is copied: the free ones are written by their moves.
+    // One walk over the rows: keys into shared memory where they fit (a longer sequence computes them again), those of the first round
+    // in registers.  Where the outputs are other arrays every row below the budget is copied: the free ones are written by their moves.
     const bool cached = n <= p.keys_cap;
     int at[kKeep], newest = INT32_MIN;
     uint32_t key[kKeep];
@@ -186,7 +189,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const Ca
     }
     const uint32_t border = prefix;
 
-    // Ties, then free rows below the budget and kept ones behind it, numbered in the order of the rows: round by round of 5120, within a
+    // Ties, then free rows below the budget and kept ones behind it, numbered in the order of the rows: round by round, within a
     // round by (row of the thread, warp), within a warp by lane.
     int2* moves = p.moves + (size_t)(b * c.kv_heads + h) * p.most_moves;
     int ties = 0, holes = 0, extra = 0;                          // of the rounds before
