@@ -628,7 +628,7 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
                         v[ch + 2] = fmaf(o[g][y][t][2 + k], back, pc[g][t][k]) * inv;
                     }
                     if (alone) {
-                        *reinterpret_cast<uint4*>((T*)p.out + at + g * 64 + 8 * r) = make_uint4(Num<T>::pack(v[0], v[1]), Num<T>::pack(v[2], v[3]), Num<T>::pack(v[4], v[5]), Num<T>::pack(v[6], v[7]));
+                        *reinterpret_cast<uint4*>((T*)p.out + at + g * 64 + 8 * r) = make_uint4(within2<T>(v[0], v[1]), within2<T>(v[2], v[3]), within2<T>(v[4], v[5]), within2<T>(v[6], v[7]));
                     } else {
                         float4* dst = reinterpret_cast<float4*>(p.part + ((size_t)piece * R + rr) * D + g * 64 + 8 * r);
                         dst[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -767,7 +767,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
             }
             T* dst = (T*)p.out + ((size_t)(e.row0 + i) * c.q_heads + head) * D + lane * E;
 #pragma unroll
-            for (int k = 0; k < E; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = Num<T>::pack(v[k] * inv, v[k + 1] * inv);
+            for (int k = 0; k < E; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = within2<T>(v[k] * inv, v[k + 1] * inv);
             if (lane == 0 && p.stats != nullptr && mass_blocks == 0) p.stats[stat_row(c, p, b, i, head)] = st;
         }
         return;
@@ -806,7 +806,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
         if ((int)threadIdx.x < Q) {
             for (int k = 1; k < LANES; ++k) { const float4 y = v_s[k * Q + threadIdx.x]; v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w; }
             const float inv = st.y > 0.f ? 1.0f / st.y : st.y != st.y ? st.y : 0.f;
-            *reinterpret_cast<uint2*>((T*)p.out + ((size_t)(e.row0 + i) * c.q_heads + head) * D + d) = make_uint2(Num<T>::pack(v.x * inv, v.y * inv), Num<T>::pack(v.z * inv, v.w * inv));
+            *reinterpret_cast<uint2*>((T*)p.out + ((size_t)(e.row0 + i) * c.q_heads + head) * D + d) = make_uint2(within2<T>(v.x * inv, v.y * inv), within2<T>(v.z * inv, v.w * inv));
             if (threadIdx.x == 0 && d == 0 && p.stats != nullptr && mass_blocks == 0) p.stats[stat_row(c, p, b, i, head)] = st;
         }
         __syncthreads();

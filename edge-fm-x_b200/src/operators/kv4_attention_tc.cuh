@@ -56,6 +56,27 @@ __device__ __forceinline__ uint4 four(const __half2 (&x)[4]) {
     const uint32_t* u = reinterpret_cast<const uint32_t*>(x);
     return make_uint4(u[0], u[1], u[2], u[3]);
 }
+// Parameters whose products or sums could leave fp16's range (scale above 2048 or minimum beyond 32768): both tests in one addition.
+__device__ __forceinline__ bool wide_range(__half2 par) {
+    return (((*reinterpret_cast<const uint32_t*>(&par) & 0x7fff7fffu) + 0x07ff17ffu) & 0x80008000u) != 0u;
+}
+// (a whole warp asks once for all that it converts: a branch a word made attend_many a third slower)
+// Their values by way of fp32, up to 65504 (the parameters' rounding may take them 80 beyond), and what is left of them.
+__device__ __forceinline__ void wide_values(uint32_t w, __half2 par, uint4& high, uint4& low) {
+    const float s = __low2float(par), m = __high2float(par);
+    __half2 n[4], h[4];
+    half_codes(w, n);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 c = __half22float2(n[i]);
+        const float a = fmaf(c.x, s, m), b = fmaf(c.y, s, m);
+        h[i] = __floats2half2_rn(fminf(a, 65504.0f), fminf(b, 65504.0f));
+        const float2 f = __half22float2(h[i]);
+        n[i] = __floats2half2_rn(a - f.x, b - f.y);
+    }
+    high = four(h);
+    low = four(n);
+}
 // min + scale * code of a word's eight codes, rounded once
 __device__ __forceinline__ uint4 half_values(uint32_t w, __half2 par) {
     const __half2 s = __low2half2(par), m = __high2half2(par);
@@ -481,7 +502,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
                         for (int i = 0; i < 32; i += 8) {
                             uint32_t z[4];
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) z[k] = Num<T>::pack(__uint_as_float(y[i + 2 * k]) * inv, __uint_as_float(y[i + 2 * k + 1]) * inv);
+                            for (int k = 0; k < 4; ++k) z[k] = within2<T>(__uint_as_float(y[i + 2 * k]) * inv, __uint_as_float(y[i + 2 * k + 1]) * inv);
                             *reinterpret_cast<uint4*>(out + d + i) = make_uint4(z[0], z[1], z[2], z[3]);
                         }
                 }
@@ -512,29 +533,40 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             unsigned char* to = sm + (V ? C::V_AT + (j % C::VS) * C::VB : C::K_AT + (j % C::KS) * C::KB);
             const uint32_t* codes = reinterpret_cast<const uint32_t*>(page + (V ? L::V_CODES : L::K_CODES));
             const __half2* pars = reinterpret_cast<const __half2*>(page + (V ? L::V_PARAMS : L::K_PARAMS));
+            __half2 par[2][G];
+            bool wide = false;
 #pragma unroll
-            for (int it = 0; it < 2; ++it) {
-                const int r = it * 32 + (dt >> 2), x = dt & 3;                   // row, quarter of its groups
-                uint32_t w[G][2];
-                quarter_words<D, V>(codes, r, x, w);
+            for (int it = 0; it < 2; ++it)
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    __half2 par = pars[r * G + g];
-                    if (r >= valid) par = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        uint4* dst = reinterpret_cast<uint4*>(to + g * (kRows * 128) + r * 128 + (((2 * x + i) ^ (r & 7)) << 4));
-                        if constexpr (V ? X == 2 : X >= 1) {
-                            uint4 high, low;
-                            half_pairs(w[g][i], par, high, low);
-                            *dst = high;
-                            dst[C::LOW / 16] = low;
-                        } else {
-                            *dst = half_values(w[g][i], par);
-                        }
-                    }
+                    const int r = it * 32 + (dt >> 2);
+                    par[it][g] = pars[r * G + g];
+                    if (r >= valid) par[it][g] = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+                    wide = wide || wide_range(par[it][g]);
                 }
-            }
+            auto words = [&](auto by_fp32) {
+#pragma unroll
+                for (int it = 0; it < 2; ++it) {
+                    const int r = it * 32 + (dt >> 2), x = dt & 3;               // row, quarter of its groups
+                    uint32_t w[G][2];
+                    quarter_words<D, V>(codes, r, x, w);
+#pragma unroll
+                    for (int g = 0; g < G; ++g)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            uint4* dst = reinterpret_cast<uint4*>(to + g * (kRows * 128) + r * 128 + (((2 * x + i) ^ (r & 7)) << 4));
+                            constexpr bool pair = V ? X == 2 : X >= 1;
+                            uint4 high, low;
+                            if constexpr (decltype(by_fp32)::value) wide_values(w[g][i], par[it][g], high, low);
+                            else if constexpr (pair) half_pairs(w[g][i], par[it][g], high, low);
+                            else high = half_values(w[g][i], par[it][g]);
+                            *dst = high;
+                            if constexpr (pair) dst[C::LOW / 16] = low;
+                        }
+                }
+            };
+            if (!__any_sync(0xffffffffu, wide)) words(std::false_type());
+            else words(std::true_type());
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             warp_arrive(full);
         };
@@ -732,7 +764,7 @@ __global__ void __launch_bounds__(kManyRows) attend_join_kernel(const Cache c, c
     const float inv = sum > 0.f ? 1.0f / sum : sum != sum ? sum : 0.f;
     uint32_t z[8];
 #pragma unroll
-    for (int d = 0; d < 8; ++d) z[d] = Num<T>::pack(v[2 * d] * inv, v[2 * d + 1] * inv);
+    for (int d = 0; d < 8; ++d) z[d] = within2<T>(v[2 * d] * inv, v[2 * d + 1] * inv);
     uint4* out = reinterpret_cast<uint4*>((T*)p.out + ((size_t)(e.row0 + i) * c.q_heads + head) * D + blockIdx.y * 16);
     out[0] = make_uint4(z[0], z[1], z[2], z[3]);
     out[1] = make_uint4(z[4], z[5], z[6], z[7]);
@@ -796,26 +828,38 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
     if (warp < 8) {                                              // the keys, while the other warps fetch rows
         const bool came = warp_wait(raw_full, 0, abort_s);
         if (!came) *abort_s = 1;
+        __half2 par[2][G];
+        bool wide = false;
 #pragma unroll
-        for (int it = 0; it < 2; ++it) {
-            const int r = it * 64 + (tid >> 2), x = tid & 3, pr = r % kRows;     // row of the block, of its page; quarter of its groups
-            const uint8_t* raw = sm + C::RAW_AT + it * C::K_PART;
-            const bool have = came && page[it] >= 0 && key0 + r < e.len;
-            uint32_t w[G][2];
-            quarter_words<D, false>(reinterpret_cast<const uint32_t*>(raw + L::K_CODES), pr, x, w);
+        for (int it = 0; it < 2; ++it)
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                const __half2 par = have ? reinterpret_cast<const __half2*>(raw + L::K_PARAMS)[pr * G + g] : __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    uint4* dst = reinterpret_cast<uint4*>(sm + C::K_AT + g * (C::KEYS * 128) + r * 128 + (((2 * x + i) ^ (r & 7)) << 4));
-                    uint4 high, low;
-                    half_pairs(w[g][i], par, high, low);
-                    dst[0] = high;
-                    dst[C::K_BYTES / 16] = low;
-                }
+                const int r = it * 64 + (tid >> 2);              // row of the block
+                const bool have = came && page[it] >= 0 && key0 + r < e.len;
+                par[it][g] = have ? reinterpret_cast<const __half2*>(sm + C::RAW_AT + it * C::K_PART + L::K_PARAMS)[r % kRows * G + g] : __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+                wide = wide || wide_range(par[it][g]);
             }
-        }
+        auto words = [&](auto by_fp32) {
+#pragma unroll
+            for (int it = 0; it < 2; ++it) {
+                const int r = it * 64 + (tid >> 2), x = tid & 3;                 // quarter of its groups
+                uint32_t w[G][2];
+                quarter_words<D, false>(reinterpret_cast<const uint32_t*>(sm + C::RAW_AT + it * C::K_PART + L::K_CODES), r % kRows, x, w);
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        uint4* dst = reinterpret_cast<uint4*>(sm + C::K_AT + g * (C::KEYS * 128) + r * 128 + (((2 * x + i) ^ (r & 7)) << 4));
+                        uint4 high, low;
+                        if constexpr (decltype(by_fp32)::value) wide_values(w[g][i], par[it][g], high, low);
+                        else half_pairs(w[g][i], par[it][g], high, low);
+                        dst[0] = high;
+                        dst[C::K_BYTES / 16] = low;
+                    }
+            }
+        };
+        if (!__any_sync(0xffffffffu, wide)) words(std::false_type());
+        else words(std::true_type());
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         warp_arrive(k_full);
     }

@@ -7,6 +7,8 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace efm {
@@ -71,6 +73,16 @@ template <> struct Num<__half> {
         return *reinterpret_cast<uint32_t*>(&p);
     }
 };
+
+// A held value as T: fp16 ends at 65504, which the rounding of minimum and scale may take a value 80 beyond.
+template <typename T>
+__device__ __forceinline__ float within(float x) {
+    if constexpr (std::is_same<T, __half>::value) asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(65504.0f));
+    return x;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t within2(float a, float b) { return Num<T>::pack(within<T>(a), within<T>(b)); }
 
 struct AppendParams {
     int max_rows;
@@ -251,7 +263,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const Cache c, c
         void* want = kind == 1 ? p.k_held : p.v_held;
         if (want != nullptr) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = __fadd_rn(m, __fmul_rn(s, code[e]));
+            for (int e = 0; e < 8; ++e) x[e] = within<T>(__fadd_rn(m, __fmul_rn(s, code[e])));
             put(want);
         }
         if (page < 0 || !have) continue;
@@ -271,7 +283,7 @@ __device__ __forceinline__ uint4 word_values(uint32_t w, __half2 par) {
     const float s = __low2float(par), m = __high2float(par);
     float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(m, __fmul_rn(s, (float)((w >> (4 * nibble(i))) & 15u)));
+    for (int i = 0; i < 8; ++i) x[i] = within<T>(__fadd_rn(m, __fmul_rn(s, (float)((w >> (4 * nibble(i))) & 15u))));
     return make_uint4(Num<T>::pack(x[0], x[1]), Num<T>::pack(x[2], x[3]), Num<T>::pack(x[4], x[5]), Num<T>::pack(x[6], x[7]));
 }
 

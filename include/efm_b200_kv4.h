@@ -13,6 +13,8 @@
  * A group is 64 neighbouring channels of a row and head; a channel stands for min + scale * code, computed in fp32.  Of x:
  *     NaN counts as 0, anything beyond +-65504 as +-65504;  scale = fp16((max - min) * (1/15)), min = fp16(min), maximum and minimum of the group;
  *     code = rint((x - min) / scale), ties to even, clamped to 0 .. 15;  scale 0: code 0.
+ * The rounding of min and scale may take a value up to 80 beyond 65504; as fp16 (outputs of that type, and where attention has many rows,
+ * v and without mass k) it is 65504.
  * Eight channels c0 .. c7 share a 32-bit word, as nibbles c0 c2 c4 c6 c1 c3 c5 c7 from the lowest bits up.  Words of a value row are in
  * the order of the channels; the words of a key row (G = D/64 groups) in the order [quarter of a group 0..3][group 0..G-1][word 0..1].
  * Pages of a sequence are any pool pages; page k of its page_table row holds cache rows [64 k, 64 k + 64).

@@ -303,3 +303,62 @@ def test_the_same_token_number_twice():
     for h in range(kh):
         rows = kv.evicted(index[h], mass[h], 150, 3, 4)
         assert c.rows_of(c.index, 0, 150)[h].tolist() == index[h][rows].tolist() and np.array_equal(c.rows_of(c.mass, 0, 150)[h], mass[h][rows])
+
+
+def extreme(c, b, seed):
+    """Every row of sequence b from values as large as fp16 goes: some groups span all of it, some lie at its upper end, some at its lower."""
+    rng, d = np.random.default_rng(seed), c.d
+    pages = c.np_table[b, :-(-c.lens.tolist()[b] // 64)]
+    pool = c.pool.cpu().numpy()
+    for page in pages:
+        tile = np.full((c.kh, kv.tile_bytes(d)), 255, np.uint8)
+        for key, (a, e), (p0, p1) in ((True, *kv.parts(d)[:2]), (False, *kv.parts(d)[2:])):
+            x = rng.standard_normal((c.kh, 64, d // 64, 64))
+            x = x / np.abs(x).max(-1, keepdims=True)
+            kind = rng.integers(0, 4, (c.kh, 64, d // 64, 1))
+            x = np.choose(kind, [x * 65504 * 1.2, 65504 - np.abs(x) * 500, np.abs(x) * 500 - 65504, x * 30000])
+            _, codes, scale, low = kv.snap(x.reshape(c.kh, 64, d))
+            nib = np.zeros((c.kh, 64, d), np.uint8)
+            nib[..., kv.nibble_place(d, key)] = codes
+            tile[:, a:e] = (nib[..., 0::2] | (nib[..., 1::2] << 4)).reshape(c.kh, -1)
+            tile[:, p0:p1] = np.ascontiguousarray(np.stack((scale, low), -1).astype(np.float16)).view(np.uint8).reshape(c.kh, -1)
+        pool[page] = tile
+    c.pool.copy_(torch.from_numpy(pool))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("counts,kh", [([1, 2], 2), ([130, 200], 16)])
+@pytest.mark.parametrize("mass", [False, True])
+def test_values_at_the_ends_of_fp16(dtype, counts, kh, mass):
+    """Parameters whose value lies beyond 65504 by their rounding, or whose scale times a code does: finite everywhere, and near the formula,
+    with values that stop at 65504 where the header allows it."""
+    lens = [190, 200]
+    c = kv.KV4(2 * kh, kh, 64, lens, None, dtype, seed=8).fill()
+    for b in range(2):
+        extreme(c, b, b)
+    q = c.normal(sum(counts), 2 * kh, 64, scale=2e-6)                         # scores of some units
+    out = torch.zeros_like(q)
+    m = torch.zeros(c.n_pages, kh, 64, device=c.dev) if mass else None
+    c.do("attention", c.attention_args(counts, c.lens, q, out, mass=m))
+    assert c.status.item() == 0 and torch.isfinite(out.float()).all()
+    row = 0
+    for b, n in enumerate(counts):
+        k, v = c.held(b, lens[b])
+        x = host(q[row:row + n])
+        ok, end = False, 65504.0
+        for kk, vv in ((k, v), (k, np.minimum(v, end)), (np.minimum(k, end), np.minimum(v, end)))[:3 if n > 2 else 1]:
+            ref, _, size = kv.attend(x, kk, vv, 1 / 8, c.spread(b, lens[b]))
+            ok |= np.abs(host(out[row:row + n]) - ref) <= attention_bound(dtype, ref, size, x, kk, 1 / 8, n > 2)
+        assert ok.all()
+        if mass:
+            w = kv.attend(x, k, v, 1 / 8)[1]
+            want = w.reshape(kh, 2 * n, lens[b]).sum(1)
+            assert np.abs(c.rows_of(m, b, lens[b]) - want).max() <= 2.0 ** -15 * max(1.0, want.max())
+        row += n
+    held = [torch.zeros(2, 256, kh, 64, dtype=c.dtype, device=c.dev) for _ in range(2)]
+    c.do("read", kv.Read(C.sizeof(kv.Read), 0, 256, 0, c.lens.data_ptr(), held[0].data_ptr(), held[1].data_ptr()))
+    for b in range(2):
+        for got, want in zip(held, c.held(b, lens[b])):
+            want = np.minimum(want.swapaxes(0, 1), 65504.0 if dtype == "fp16" else np.inf)
+            assert torch.isfinite(got.float()).all()
+            assert (np.abs(host(got[b, :lens[b]]) - want) <= HALF_STEP[dtype] * np.abs(want) * (1 + 1e-6) + 1e-6).all()
