@@ -109,7 +109,8 @@ void by_type(const efm_kv4_cache* c, F&& f) {
 }
 
 // Every kernel of this file waits for its predecessor before it touches anything an earlier launch may have written, so all of them start
-// ahead of the predecessor's end: a decode step of three launches took 25 us without and 17 with.
+// ahead of the predecessor's end (a kernel lets its successor start once its own wait is over, so that all but the predecessor has ended by
+// then): append, attention and weights of one token on 1450 rows take 13.8 us with and 15.0 without, in a replayed graph.
 Launcher on_stream(void* stream) {
     Launcher L;
     L.stream = (cudaStream_t)stream;
@@ -168,7 +169,8 @@ AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
     p.few_rows = few_rows_of(c);
     p.many_tiles = rows > p.few_rows ? (int)((rows + kv4::kManyRows - 1) / kv4::kManyRows) : 0;
     const int64_t R = 8 * p.nt, tiles = (std::min<int64_t>(rows, p.few_rows) + R - 1) / R, pages = std::max(1, (p.max_len + kRows - 1) / kRows);
-    // a page at a time, or caches of up to four pages whole: nothing is left to join then, which saves the smallest calls a launch
+    // A page at a time, or caches of up to four pages whole: nothing is left to join then, which saves the smallest calls a launch.  Append and
+    // attention of a token, 14/2 heads of 64: 8.2 us whole, 9.6 by pages on two pages; 10.3 and 10.2 on four; 11.2 and 10.3 on five.
     p.unit_shift = pages <= 1 << kWholeShift ? kWholeShift : 0;
     p.units = (pages + (1 << p.unit_shift) - 1 >> p.unit_shift) * tiles * c->kv_heads * c->batch;
     p.blocks = (int)std::max<int64_t>(1, std::min<int64_t>(kSms * (p.nt == 1 ? 3 : 2), (p.units + kv4::kWarps - 1) / kv4::kWarps));

@@ -1,7 +1,7 @@
 // Many query rows against a 4-bit cache on the 5th-generation tensor cores.
 //
-// Block = 256 packed rows (new rows x heads of a group) of one sequence and kv head, as two tiles of 128 that share the keys and values;
-// 15 warps:
+// A block has 256 packed rows (new rows x heads of a group) of one sequence and kv head at a time, as two tiles of 128 that share the keys and
+// values; 15 warps:
 //   warps 0-3, 4-7   softmax of a tile, a thread per row: S from tensor memory, p = 2^(s - m), P back into tensor memory as fp16, where the
 //                    product takes it as its A operand.  O stays in tensor memory; it is scaled only when a row's maximum has grown by
 //                    more than 2^8 since it was last, which a row's first pages see and later ones hardly;
@@ -10,14 +10,17 @@
 //                    operands' 128-byte-swizzled layout: K-major rows of K, and the same rows of V read MN-major;
 //   warps 12, 13     one lane of each issues a tile's products: S = Q K^T (M 128, N 64, K = head size), O += P V (M 128, N = head size, K 64).  S has two
 //                    buffers a tile and runs two pages ahead of P V; weights take the place of the scores they came from.  A wait costs
-//                    that warp some 250 cycles even when it is over; one warp for both tiles left the tensor pipe idle half the time.
+//                    that warp some 200 cycles even when it is over, so it polls for all that a page needs at once; one warp for both
+//                    tiles left the tensor pipe idle half the time.
 // q is scaled by a power of two per row to be exact in fp16.  k, v and p are rounded to fp16 (2^-11), well below the half step of a bf16
 // output (2^-8).  Where that would show they are pairs high + low: k where row sums are wanted that summed weights are divided by (X 1:
 // S = Q (Kh + Kl)), and all of them for fp16 outputs (X 2: O += Ph Vh + Pl Vh + Ph Vl as well).
 // A barrier is waited for by parity, which tells a phase from its neighbours only: every barrier here is either waited for in each of its
 // phases by whoever its next phase needs, or (o_done) has a copy per page parity, whose next phase needs the waiting thread's weights of
 // two pages later.
-// Bound: tensor pipe (4 rows keys D flops), and close to it the exponentials and the conversion of the codes.
+// Bound: the softmax warps (some 2000 cycles a page: 1600 of arithmetic, the rest waits), ahead of the tensor pipe (1280) and the exponential
+// unit (770 after a quarter of the exponentials went to arithmetic).  2048 rows, 28 heads on 4 kv heads of 128, behind 12289: 405 - 440 us by
+// the card's clock, 890 - 960 TFLOP/s of 4 rows keys D.
 #pragma once
 #include <type_traits>
 
@@ -723,7 +726,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
 }
 
 // Rows whose pages attend_many dealt over several blocks: maximum, sum and values of their pieces put together.  Block (w - 1, s) looks at
-// the boundary ahead of block w; if that is the first one inside a block of rows it joins 16 channels of those, a thread a row.
+// the boundary ahead of block w; if that is the first one inside a block of rows it joins 16 channels of those, a thread a row.  Bound: 39 MB of
+// pieces through L2 where every block leaves two; 8 us behind its predecessor.
 // grid (blocks of attend_many - 1, D / 16).
 template <typename T, int D>
 __global__ void __launch_bounds__(kManyRows) attend_join_kernel(const Cache c, const AttnParams p) {
@@ -784,7 +788,9 @@ constexpr int kWeightThreads = 13 * 32;
 // fp16 so that scores have 32-bit accuracy.  A key is a lane of tensor memory and two threads of warps 0-7, each of which adds up its weights
 // 2^(s - m - log2 l) over half the rows of a step, in order: no atomics, no shuffles.  Warps 8-11 bring the rows' operand and (unit, m + log2 l),
 // warp 12 issues the products.
-// grid (blocks of 128 cached rows, kv heads, batch).  Bound: exponentials and tensor pipe alike (128 x 128 of them in 1024 cycles, two products of K = D).
+// grid (blocks of 128 cached rows, kv heads, batch).  Bound: exponentials and tensor pipe alike (1024 cycles a step each, of 1500 - 1600), and
+// 4 us of a block's life before its first step.  16 sequences of 1 .. 256 rows on up to 2056, 16 heads on 2 of 128: 43 us.  Two blocks an SM
+// with one buffer for the rows: 54.
 template <typename T, int D>
 __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const Cache c, const AttnParams p) {
     using C = WeightsCfg<D>;

