@@ -368,7 +368,6 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
                 else L.launch(kv4::attend_many_kernel<T, D, 0>, many, threads, kv4::ManyCfg<D, 0>::SMEM, c, p);
                 if (plan.many_blocks > 1) L.launch(kv4::attend_join_kernel<T, D>, dim3(plan.many_blocks - 1, D / 16), dim3(kv4::kManyRows), 0, c, p);
             }
-            L.pdl = rows > 0;                          // what follows reads lengths ahead of its wait: not as a call's first launch
             if (join.x > 0 && plan.nt == 1) L.launch(kv4::attend_merge_kernel<T, D, 8>, join, block, 0, c, p, masses);
             if (join.x > 0 && plan.nt == 2) L.launch(kv4::attend_merge_kernel<T, D, 16>, join, block, 0, c, p, masses);
             if (p.mass_out != nullptr && !plan.scores)

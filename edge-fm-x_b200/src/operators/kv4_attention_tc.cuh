@@ -804,9 +804,9 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
     volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int tid = threadIdx.x, warp = tid >> 5, h = blockIdx.y, b = blockIdx.z, group = c.q_heads / c.kv_heads, key0 = blockIdx.x * C::KEYS;
 
-    // lengths, pages and keys are nobody's to write since before the first kernel of this call
+    pdl_wait();                                                  // lengths, pages and keys are what earlier launches wrote
     const Entry e = entry_of(c, p, b);
-    if (key0 >= e.len) { pdl_wait(); return; }
+    if (key0 >= e.len) return;
     int page[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) page[i] = key0 + i * kRows < e.len ? page_of(c, b, key0 / kRows + i) : -1;
@@ -869,7 +869,6 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         warp_arrive(k_full);
     }
-    pdl_wait();
 
     const int rows = e.n * group, first_row = max(0, key0 - (e.len - e.n)) * group / C::ROWS * C::ROWS;       // rows before do not see the block
     const int n = rows > first_row ? (rows - first_row + C::ROWS - 1) / C::ROWS : 0;
