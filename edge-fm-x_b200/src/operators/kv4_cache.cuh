@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const Cache c, c
     constexpr int LANES = D / 8, HEADS = 32 / LANES;         // lanes of a head, heads of a warp
     using L = Tile<D>;
     __shared__ float2 rot[D / 2];
-    __shared__ int place_s, page_s;                          // cache row and page of the row; place -1: nobody's row
+    __shared__ int place_s, page_s, falls_s;                 // cache row and page of the row; place -1: nobody's row; row counts fall somewhere
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LANES, c0 = sub * 8;
     const int cap = c.max_pages * kRows;
     const int tq = p.q != nullptr ? (c.q_heads + HEADS - 1) / HEADS : 0, tk = (c.kv_heads + HEADS - 1) / HEADS;
@@ -154,27 +154,34 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const Cache c, c
         const T* src = kind == 0 ? (const T*)p.q + row * p.q_stride : kind == 1 ? (const T*)p.k + row * p.k_stride : (const T*)p.v + row * p.v_stride;
         return *reinterpret_cast<const uint4*>(src + (size_t)h * D + c0);
     };
-    if (tid == 0) place_s = -1;
+    if (tid == 0) { place_s = -1; falls_s = 0; }
     __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
     int task = blockIdx.y * tasks_per_block + warp;
     uint4 next = row < p.max_rows ? fetch(task) : make_uint4(0u, 0u, 0u, 0u);             // on its way while the row's place is looked up
-    for (int b = tid; b < c.batch; b += kAppendThreads) {
-        const int lo = p.cu_rows[b], hi = p.cu_rows[b + 1];
-        const bool mine = row >= lo && row < hi && row < p.max_rows, tells = row == 0 && blockIdx.y == 0;
-        if (!mine && !tells) continue;
+    const bool tells = row == 0 && blockIdx.y == 0;
+    bool full = false;
+    auto look = [&](int b, int lo, int hi) {                 // rows [lo, hi) are sequence b's
+        const bool mine = row >= lo && row < hi;
+        if (!mine && !tells) return;
         const int have = held(c, p.lens_in, b, cap);
         if (tells) {
-            const int n = max(0, min(hi, p.max_rows) - max(min(lo, p.max_rows), 0));
-            p.lens_out[b] = min(cap - have, n) + have;
-            if (n > cap - have) raise(c, kFull);
+            p.lens_out[b] = min(cap - have, hi - lo) + have;
+            full = full || hi - lo > cap - have;
         }
         if (mine) {
             const int64_t behind = have + ((int64_t)row - lo);
             place_s = behind < cap ? (int)behind : cap;
             page_s = behind < cap ? page_of(c, b, (int)behind / kRows) : -1;
         }
+    };
+    auto cut = [&](int at) { return min(max(at, 0), p.max_rows); };
+    for (int b = tid; b < c.batch; b += kAppendThreads) {
+        const int lo = p.cu_rows[b], hi = p.cu_rows[b + 1];
+        if (hi < lo) falls_s = 1;
+        if (tells && (lo < 0 || hi < lo || hi > p.max_rows)) raise(c, kBadCount);
+        look(b, cut(lo), cut(hi));
     }
     const int half = p.rot_dims / 2;
     if (half > 0 && row < p.max_rows)
@@ -185,6 +192,20 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const Cache c, c
             rot[i] = make_float2((float)co, (float)s);
         }
     __syncthreads();
+    if (falls_s) {                                           // counts that fall would give a row to several sequences: their running maximum counts
+        full = false;
+        if (tid == 0) {
+            place_s = -1;
+            for (int b = 0, lo = 0; b < c.batch; ++b) {
+                lo = max(lo, cut(p.cu_rows[b]));
+                const int hi = max(lo, cut(p.cu_rows[b + 1]));
+                look(b, lo, hi);
+                lo = hi;
+            }
+        }
+        __syncthreads();
+    }
+    if (full) raise(c, kFull);
     if (place_s < 0) return;
     const int place = place_s, page = page_s, r = place % kRows;
     const bool turns = c0 < p.rot_dims, second = c0 >= half;

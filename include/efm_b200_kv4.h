@@ -39,7 +39,8 @@ enum { EFM_KV4_ROT_HALVES = 0, EFM_KV4_ROT_NEIGHBOURS = 1 };
 enum {
     EFM_KV4_BAD_PAGE = 1,     /* a page number outside [0, n_pages): its rows are not written, and count as absent when read */
     EFM_KV4_FULL = 2,         /* append: a sequence has no more page_table columns; the row is dropped and not counted */
-    EFM_KV4_BAD_COUNT = 4,    /* a length or row count beyond what the call was given (max_len, max_new) or negative: cut to it */
+    EFM_KV4_BAD_COUNT = 4,    /* a length or row count beyond what the call was given (max_len, max_new, max_rows) or negative: cut to it; where
+                               * cu_rows falls, append takes its running maximum, so that a row stays with the first sequence that names it */
     EFM_KV4_WAIT = 8          /* a bounded wait for a copy or product inside a kernel gave up; the call's outputs are void */
 };
 
