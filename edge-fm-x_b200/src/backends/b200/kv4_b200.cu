@@ -2,6 +2,7 @@
 #include <efm_b200_kv4.h>
 
 #include <atomic>
+#include <cstdlib>
 #include <exception>
 
 #include "../../operators/kv4_attention.cuh"
@@ -57,17 +58,51 @@ private:
 struct DeviceInfo { int sms = 0, smem = 0; };
 constexpr int kEvictSmemReserve = 12 * 1024;          // static shared memory of the ordering kernel, rounded up
 
+// Kernels whose waits give up after a few polls, for tests of what a call does then: EFM_B200_KV4_HASTY, a sum of 1 (attend_few), 2
+// (attend_many) and 4 (attend_weights), looked at if it was there at the first call.
+int hasty() {
+    static const bool set = std::getenv("EFM_B200_KV4_HASTY") != nullptr;
+    const char* e = set ? std::getenv("EFM_B200_KV4_HASTY") : nullptr;
+    return e != nullptr ? std::atoi(e) : 0;
+}
+// Kernels of attention that wait inside.
+template <typename T, int D>
+struct AttendKernels {
+    using Kernel = void (*)(const kv4::Cache, const kv4::AttnParams);
+    static constexpr int X = std::is_same<T, __half>::value ? 2 : 0, XM = X == 0 ? 1 : 2;      // of attend_many without and with mass
+    Kernel few1, few2, many, many_mass, weights;
+    template <int POLLS>
+    static AttendKernels of() {
+        return {kv4::attend_few_kernel<T, D, 1, POLLS>, kv4::attend_few_kernel<T, D, 2, POLLS>, kv4::attend_many_kernel<T, D, X, POLLS>, kv4::attend_many_kernel<T, D, XM, POLLS>,
+                kv4::attend_weights_kernel<T, D, POLLS>};
+    }
+    static AttendKernels now() {
+        AttendKernels k = of<kv4::kPolls>();
+        if constexpr (kHasHasty) {
+            const AttendKernels h = of<kv4::kHasty>();
+            const int which = hasty();
+            if (which & 1) { k.few1 = h.few1; k.few2 = h.few2; }
+            if (which & 2) { k.many = h.many; k.many_mass = h.many_mass; }
+            if (which & 4) k.weights = h.weights;
+        }
+        return k;
+    }
+    cudaError_t more_smem() const {
+        auto set = [](Kernel kernel, size_t bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes); };
+        cudaError_t e = set(few1, kv4::FewCfg<D, 1>::SMEM);
+        if (e == cudaSuccess) e = set(few2, kv4::FewCfg<D, 2>::SMEM);
+        if (e == cudaSuccess) e = set(weights, kv4::WeightsCfg<D>::SMEM);
+        if (e == cudaSuccess) e = set(many, kv4::ManyCfg<D, X>::SMEM);
+        if (e == cudaSuccess) e = set(many_mass, kv4::ManyCfg<D, XM>::SMEM);
+        return e;
+    }
+    static constexpr bool kHasHasty = (X == 0 && D == 128) || (X == 2 && D == 64);             // forms that are enough for those tests
+};
 template <typename T, int D>
 cudaError_t more_smem() {
-    cudaError_t e = cudaFuncSetAttribute(kv4::attend_few_kernel<T, D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::FewCfg<D, 1>::SMEM);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_few_kernel<T, D, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::FewCfg<D, 2>::SMEM);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_weights_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::WeightsCfg<D>::SMEM);
-    if constexpr (std::is_same<T, __half>::value) {
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_many_kernel<T, D, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::ManyCfg<D, 2>::SMEM);
-    } else {
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_many_kernel<T, D, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::ManyCfg<D, 0>::SMEM);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4::attend_many_kernel<T, D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kv4::ManyCfg<D, 1>::SMEM);
-    }
+    using K = AttendKernels<T, D>;
+    cudaError_t e = K::template of<kv4::kPolls>().more_smem();
+    if constexpr (K::kHasHasty) { if (e == cudaSuccess) e = K::template of<kv4::kHasty>().more_smem(); }
     return e;
 }
 
@@ -140,11 +175,12 @@ struct AttnPlan {
     int max_new, max_len, nt, blocks, unit_shift, few_rows;
     int many_tiles, many_blocks;                      // blocks of 256 packed rows a sequence may have; blocks that deal with them
     int64_t many_units, many_starts, many_stats, many_part;
+    int64_t lost;                                     // a word a block of either kernel
     bool joined;                                      // pieces of a row may lie in several blocks
     bool scores;                                      // attend_few leaves its scores for the summed weights
     int64_t units, stats, part_stats, part, score_ld, score, image, image_units, starts;
     int row_tiles;                                    // tiles of 128 packed rows a sequence may have as operands; 0: nobody asks for them
-    int64_t bytes() const { return 4 * (stats + part_stats + part + score + image + image_units + starts + many_starts + many_stats + many_part); }
+    int64_t bytes() const { return 4 * (stats + part_stats + part + score + image + image_units + starts + many_starts + many_stats + many_part + lost); }
 };
 constexpr int kSms = 148;                              // of the GPU these kernels are built for
 constexpr int kWholeShift = 2;
@@ -193,8 +229,36 @@ AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
         p.many_stats = 2 * 2 * (int64_t)p.many_blocks * kv4::kManyRows;
         p.many_part = 2 * (int64_t)p.many_blocks * kv4::kManyRows * c->head_dim;
     }
+    p.lost = rows > 0 ? round_up(p.blocks + p.many_blocks, 4) : 0;
     p.score = p.scores ? (int64_t)c->batch * c->kv_heads * R * p.score_ld : 0;
     return p;
+}
+
+template <typename T, int D>
+void launch_attention(Launcher& L, const efm_kv4_cache* cache, const AttnPlan& plan, const kv4::AttnParams& p) {
+    using K = AttendKernels<T, D>;
+    const K k = K::now();
+    const dim3 block(kv4::kWarps * 32);
+    const kv4::Cache c = device_cache(cache);
+    const int64_t rows = (int64_t)plan.max_new * (cache->q_heads / cache->kv_heads);
+    // as many merging blocks as find room at once
+    const int64_t jobs = std::min<int64_t>(rows, plan.few_rows) * (D / 32), room = std::max<int64_t>(1, 8 * kSms / ((int64_t)cache->batch * cache->kv_heads));
+    const int merges = plan.joined ? (int)std::min(jobs, room) : 0, masses = plan.scores ? (plan.max_len + kv4::kMassTokens - 1) / kv4::kMassTokens : 0;
+    const dim3 join(merges + masses, cache->kv_heads, cache->batch);
+    if (rows > 0 && plan.nt == 1) L.launch(k.few1, dim3(plan.blocks), block, kv4::FewCfg<D, 1>::SMEM, c, p);
+    if (rows > 0 && plan.nt == 2) L.launch(k.few2, dim3(plan.blocks), block, kv4::FewCfg<D, 2>::SMEM, c, p);
+    if (plan.row_tiles > 0) L.launch(kv4::attend_query_kernel<T, D>, dim3(plan.row_tiles + 1, cache->kv_heads, cache->batch), dim3(kv4::kTileRows), 0, c, p);
+    if (plan.many_tiles > 0) {
+        const dim3 many(plan.many_blocks), threads(kv4::kManyThreads);
+        if (p.mass_out != nullptr) L.launch(k.many_mass, many, threads, kv4::ManyCfg<D, K::XM>::SMEM, c, p);
+        else L.launch(k.many, many, threads, kv4::ManyCfg<D, K::X>::SMEM, c, p);
+        if (plan.many_blocks > 1) L.launch(kv4::attend_join_kernel<T, D>, dim3(plan.many_blocks - 1, D / 16), dim3(kv4::kManyRows), 0, c, p);
+    }
+    if (join.x > 0 && plan.nt == 1) L.launch(kv4::attend_merge_kernel<T, D, 8>, join, block, 0, c, p, masses);
+    if (join.x > 0 && plan.nt == 2) L.launch(kv4::attend_merge_kernel<T, D, 16>, join, block, 0, c, p, masses);
+    if (p.mass_out != nullptr && !plan.scores)
+        L.launch(k.weights, dim3((plan.max_len + kv4::WeightsCfg<D>::KEYS - 1) / kv4::WeightsCfg<D>::KEYS, cache->kv_heads, cache->batch), dim3(kv4::kWeightThreads),
+                 kv4::WeightsCfg<D>::SMEM, c, p);
 }
 
 efm_status check_evict(const char* call, const efm_kv4_evict* a) {
@@ -346,33 +410,13 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
         p.many_starts = p.starts + plan.starts;
         p.many_stats = (float2*)(p.many_starts + plan.many_starts);
         p.many_part = (float*)p.many_stats + plan.many_stats;
+        p.lost = (int32_t*)(p.many_part + plan.many_part);
+        p.few_blocks = plan.blocks; p.n_lost = plan.lost > 0 ? plan.blocks + plan.many_blocks : 0;
         Launcher L = on_stream(stream);
         by_type(cache, [&](auto t, auto d) {
             using T = decltype(t);
             constexpr int D = decltype(d)::value;
-            const dim3 block(kv4::kWarps * 32);
-            const kv4::Cache c = device_cache(cache);
-            const int64_t rows = (int64_t)plan.max_new * (cache->q_heads / cache->kv_heads);
-            // as many merging blocks as find room at once
-            const int64_t jobs = std::min<int64_t>(rows, plan.few_rows) * (D / 32), room = std::max<int64_t>(1, 8 * kSms / ((int64_t)cache->batch * cache->kv_heads));
-            const int merges = plan.joined ? (int)std::min(jobs, room) : 0, masses = plan.scores ? (plan.max_len + kv4::kMassTokens - 1) / kv4::kMassTokens : 0;
-            const dim3 join(merges + masses, cache->kv_heads, cache->batch);
-            if (rows > 0 && plan.nt == 1) L.launch(kv4::attend_few_kernel<T, D, 1>, dim3(plan.blocks), block, kv4::FewCfg<D, 1>::SMEM, c, p);
-            if (rows > 0 && plan.nt == 2) L.launch(kv4::attend_few_kernel<T, D, 2>, dim3(plan.blocks), block, kv4::FewCfg<D, 2>::SMEM, c, p);
-            if (plan.row_tiles > 0) L.launch(kv4::attend_query_kernel<T, D>, dim3(plan.row_tiles + 1, cache->kv_heads, cache->batch), dim3(kv4::kTileRows), 0, c, p);
-            if (plan.many_tiles > 0) {
-                const dim3 many(plan.many_blocks);
-                const dim3 threads(kv4::kManyThreads);
-                if constexpr (std::is_same<T, __half>::value) L.launch(kv4::attend_many_kernel<T, D, 2>, many, threads, kv4::ManyCfg<D, 2>::SMEM, c, p);
-                else if (p.mass_out != nullptr) L.launch(kv4::attend_many_kernel<T, D, 1>, many, threads, kv4::ManyCfg<D, 1>::SMEM, c, p);
-                else L.launch(kv4::attend_many_kernel<T, D, 0>, many, threads, kv4::ManyCfg<D, 0>::SMEM, c, p);
-                if (plan.many_blocks > 1) L.launch(kv4::attend_join_kernel<T, D>, dim3(plan.many_blocks - 1, D / 16), dim3(kv4::kManyRows), 0, c, p);
-            }
-            if (join.x > 0 && plan.nt == 1) L.launch(kv4::attend_merge_kernel<T, D, 8>, join, block, 0, c, p, masses);
-            if (join.x > 0 && plan.nt == 2) L.launch(kv4::attend_merge_kernel<T, D, 16>, join, block, 0, c, p, masses);
-            if (p.mass_out != nullptr && !plan.scores)
-                L.launch(kv4::attend_weights_kernel<T, D>, dim3((plan.max_len + kv4::WeightsCfg<D>::KEYS - 1) / kv4::WeightsCfg<D>::KEYS, cache->kv_heads, cache->batch),
-                         dim3(kv4::kWeightThreads), kv4::WeightsCfg<D>::SMEM, c, p);
+            launch_attention<T, D>(L, cache, plan, p);
         });
         return launched(call, L);
     });

@@ -28,6 +28,8 @@ struct AttnParams {
     float2* part_stats;       // [8 nt][2 warps] the same of the keys a warp had, and
     float* part;              // [2 warps][8 nt][D] its weighted values: slot 0 is the piece its range begins with, slot 1 the one it ends with
     int32_t* starts;          // [batch + 1] units ahead of every sequence, and all of them
+    int32_t* lost;            // [n_lost] of attend_few's blocks, then of attend_many's: 1 where a wait gave up.  Weights are not summed then
+    int few_blocks, n_lost;
     uint8_t* images;          // [batch, kv_heads, row_tiles][128 x D fp16] packed rows as operands, and
     float* units;             // [batch, kv_heads, row_tiles][128] what their scores are multiplied with; where many rows are a sequence's
     int row_tiles;
@@ -57,10 +59,12 @@ __device__ __forceinline__ size_t stat_row(const Cache& c, const AttnParams& p, 
 
 constexpr int kWarps = 4;
 
-// Wait of a whole warp for a phase, bounded; false when it gave up.
-constexpr int kSpins = 1 << 25;
+// Wait of a whole warp for a phase, bounded; false when it gave up.  The limit (some seconds) is a constant: read from the parameters it
+// cost attend_many 5 %, attend_few 3, of which warps that poll take issue slots from the others.  kHasty: for tests of what follows.
+constexpr int kPolls = 1 << 25, kHasty = 2;
+template <int POLLS>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-    for (int i = 0; i < kSpins; ++i) {
+    for (int i = 0; i < POLLS; ++i) {
         uint32_t ok;
         asm volatile(
             "{\n"
@@ -283,7 +287,7 @@ struct FewCfg {
 // Bound: instruction issue, 1280 a page of 64 x 128 (a third of them on the integer pipe, which takes the codes apart, half floating point),
 // of which three blocks an SM, as many as registers allow, reach 57 % of the slots; then bytes.  One token, 28 heads on 4 kv heads of 128, on
 // 131000 rows: 28 us, 2.8 TB/s; on 64 caches of 300 .. 4000: 31 us, 2.7 TB/s.
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, int POLLS = kPolls>
 __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few_kernel(const Cache c, const AttnParams p) {
     using L = Tile<D>;
     using C = FewCfg<D, NT>;
@@ -305,6 +309,7 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
     pdl_launch_dependents();
     // the warps' ranges of the units, and the sequences they begin in
     const int me = blockIdx.x * kWarps + warp;
+    if (threadIdx.x == 0) p.lost[blockIdx.x] = 0;
     int all = 0, b = 0, start = 0;                                               // b: sequence, start: unit that it begins with
     Entry e0;
     if (c.batch == 1) {
@@ -441,12 +446,13 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
 
         for (int i = 0; i < x.mine; ++i) {
             const int st = (slot + i) % C::STAGES, first = (x.p0 + i) * kRows;
-            if (!warp_wait(bar0 + 8 * st, (uint32_t)((slot + i) / C::STAGES) & 1u, abort_s)) {      // given up: copies in flight land first (bounded)
+            if (!warp_wait<POLLS>(bar0 + 8 * st, (uint32_t)((slot + i) / C::STAGES) & 1u, abort_s)) {      // given up: the warp's copies in flight land first (bounded)
                 *abort_s = 1;
                 if (lane == 0) {
                     volatile int go_on = 0;
-                    for (int k = 0; k < C::STAGES; ++k) { (void)tc::mbar_wait(bar0 + 8 * k, 0, &go_on); (void)tc::mbar_wait(bar0 + 8 * k, 1, &go_on); }
+                    for (int k = slot + i; k < slot + min(x.mine, i + C::STAGES); ++k) (void)tc::mbar_wait(bar0 + 8 * (k % C::STAGES), (uint32_t)(k / C::STAGES) & 1u, &go_on);
                     raise(c, kWait);
+                    p.lost[blockIdx.x] = 1;
                 }
                 return;
             }
@@ -700,11 +706,13 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
         const int t0 = blockIdx.x * kMassTokens;
         if (t0 >= e.len) return;
         const Pieces x = rows > 0 ? pieces_of(p, sh, Deal{p.starts[b], p.starts[c.batch]}, h, 0) : Pieces{0, 0};
+        bool lost = false;
+        for (int i = x.w0 / kWarps + (int)threadIdx.x; rows > 0 && i <= x.w1 / kWarps; i += kWarps * 32) lost = lost || p.lost[i] != 0;
         for (int row = warp; row < rows; row += kWarps) {
             const float2 s = x.w0 == x.w1 ? p.stats[stat_row(c, p, b, row / group, h * group + row % group)] : merged_stats(p, x, row);
             if (lane == 0) st_s[row] = s.x == -INFINITY ? make_float2(0.f, 0.f) : make_float2(s.x, 1.0f / s.y);
         }
-        __syncthreads();
+        if (__syncthreads_or(lost)) return;                      // not all scores are there
         constexpr int PER = kMassTokens / (kWarps * 32);
         float w[PER];
         const float* from = p.scores + ((size_t)b * c.kv_heads + h) * R * p.score_ld + t0 + threadIdx.x;

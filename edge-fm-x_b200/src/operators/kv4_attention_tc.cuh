@@ -41,7 +41,7 @@ struct ManyCfg {
     static constexpr int KB = X >= 1 ? 2 * LOW : LOW, VB = X == 2 ? 2 * LOW : LOW;       // bytes of a stage
     static constexpr int Q_AT = 0, K_AT = 2 * Q_BYTES, V_AT = K_AT + KS * KB, RAW_AT = V_AT + VS * VB, BARS = RAW_AT + RAW * Tile<D>::BYTES;
     static constexpr int S_COL = 0, O_COL = 256;                                         // S of (tile, page parity): 64 columns each, P in its place; O: 128 a tile
-    static constexpr size_t SMEM = BARS + 336 + 1024;
+    static constexpr size_t SMEM = BARS + 352 + 1024;
 };
 
 // Pairs of fp16 codes of a word, in the order of the channels: as in low_pair / high_pair, without the 8.
@@ -167,8 +167,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 // Three waits at once: polled one behind the other a wait that is over takes some 200 cycles each.
 struct Phase { uint32_t bar, parity; };
+template <int POLLS>
 __device__ __forceinline__ bool warp_wait(const Phase& a, const Phase& b, const Phase& c, volatile int* abort_flag) {
-    for (int i = 0; i < kSpins; ++i) {
+    for (int i = 0; i < POLLS; ++i) {
         uint32_t ok;
         asm volatile(
             "{\n"
@@ -371,7 +372,7 @@ __global__ void __launch_bounds__(kTileRows) attend_query_kernel(const Cache c, 
 }
 
 // grid: one block an SM, each with its share of the units (above)
-template <typename T, int D, int X>
+template <typename T, int D, int X, int POLLS = kPolls>
 __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cache c, const AttnParams p) {
     using C = ManyCfg<D, X>;
     using L = Tile<D>;
@@ -386,9 +387,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::BARS + 288);
     volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* valid_s = reinterpret_cast<volatile int*>(tmem_slot + 2);      // [8] rows held of the block's page number j % 8; 0: not one of the pool's
+    volatile int* asked_s = valid_s + 8;                         // copies that warps 12, 13 and 14 asked for
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = c.q_heads / c.kv_heads;
 
     pdl_wait();
+    if (tid == 0) p.lost[p.few_blocks + blockIdx.x] = 0;
     ManyWalk walk(c, p, blockIdx.x);
     if (!walk.more()) return;
     const int pages = walk.whole > 0 ? ManyWalk(walk).next(c, p).n : walk.u1 - walk.u;      // of all pieces
@@ -431,7 +434,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             for (; j < x.n; ++j) {
                 const int buf = t * 2 + ((mine + j) & 1);
                 const uint32_t s_at = tmem + lanes + (uint32_t)(C::S_COL + buf * 64);
-                if (!warp_wait(s_full + 8 * buf, (uint32_t)((mine + j) >> 1) & 1u, abort_s)) { *abort_s = 1; break; }
+                if (!warp_wait<POLLS>(s_full + 8 * buf, (uint32_t)((mine + j) >> 1) & 1u, abort_s)) { *abort_s = 1; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 float s[64];
                 tmem_ld64(s_at, s);
@@ -470,7 +473,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
                 }
                 l += low_of(sum) + high_of(sum);
                 if (j > 0 && __any_sync(0xffffffffu, grow)) {    // O once P V of the page before is through
-                    if (!warp_wait(o_done + 8 * (buf ^ 1), (uint32_t)((mine + j - 1) >> 1) & 1u, abort_s)) { *abort_s = 1; break; }
+                    if (!warp_wait<POLLS>(o_done + 8 * (buf ^ 1), (uint32_t)((mine + j - 1) >> 1) & 1u, abort_s)) { *abort_s = 1; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
                     for (int d = 0; d < D; d += 32) {
@@ -489,7 +492,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             }
             before += x.n;
             mine += x.n;
-            ok = j == x.n && warp_wait(o_done + 8 * (t * 2 + ((mine - 1) & 1)), (uint32_t)((mine - 1) >> 1) & 1u, abort_s);
+            ok = j == x.n && warp_wait<POLLS>(o_done + 8 * (t * 2 + ((mine - 1) & 1)), (uint32_t)((mine - 1) >> 1) & 1u, abort_s);
             if (!ok) { *abort_s = 1; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int head = x.h * group + row % group;
@@ -528,7 +531,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
         }
     } else if (warp < 12) {
         const int dt = tid - 8 * 32;
-        auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait(bar, parity, abort_s); };
+        auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait<POLLS>(bar, parity, abort_s); };
         auto convert = [&](auto values, int j, uint32_t full) {  // K or V of page j, by all four warps
             constexpr bool V = decltype(values)::value;
             const uint8_t* page = sm + C::RAW_AT + (j % C::RAW) * L::BYTES;
@@ -589,7 +592,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
         if (i < pages + C::LEAD) *abort_s = 1;
     } else if (warp == 14) {
         bool ok = true;
-        for (int j = 0; ok && walk.more();) {
+        int j = 0;
+        while (ok && walk.more()) {
             const ManyPiece x = walk.next(c, p);
             const int held = (x.e.len + kRows - 1) / kRows;      // pages; a row that sees nothing has one that is nobody's
             int lane_page = -1;
@@ -601,7 +605,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
                 }
                 const int page = __shfl_sync(0xffffffffu, lane_page, i & 31);
                 const uint32_t bar = raw_full + 8 * (j % C::RAW);
-                if (j >= C::RAW && !warp_wait(raw_empty + 8 * (j % C::RAW), (uint32_t)(j / C::RAW - 1) & 1u, abort_s)) { *abort_s = 1; ok = false; break; }
+                if (j >= C::RAW && !warp_wait<POLLS>(raw_empty + 8 * (j % C::RAW), (uint32_t)(j / C::RAW - 1) & 1u, abort_s)) { *abort_s = 1; ok = false; break; }
                 if (lane == 0) {
                     valid_s[j & 7] = page >= 0 ? min(kRows, x.e.len - (x.p0 + i) * kRows) : 0;
                     if (page >= 0) {
@@ -614,6 +618,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
                 __syncwarp();
             }
         }
+        if (lane == 0) asked_s[2] = j;
     } else {
         // The whole warp walks the loop, so that addresses and descriptors stay in uniform registers; one lane issues.
         constexpr uint32_t kDescS = at::instr_desc_f16(kTileRows, kRows), kDescO = at::instr_desc_f16(kTileRows, D) | (1u << 16);
@@ -622,7 +627,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
         const uint64_t qt = tc::umma_desc(base + C::Q_AT + t * C::Q_BYTES), kd = tc::umma_desc(base + C::K_AT), vd = at::umma_desc_mn(base + C::V_AT, (uint32_t)(kRows * 128), 1024u);
         const uint32_t s0 = tm + (uint32_t)(C::S_COL + t * 128), to = tm + (uint32_t)(C::O_COL + t * 128);
-        int before = 0, mine = 0, asked = 0;                     // pages of the pieces before, of all and of this tile; its pieces
+        int before = 0, mine = 0, begun = 0, asked = 0;          // pages of the pieces before, of all and of this tile; its pieces; copies of queries
         auto issue_s = [&](int j) {                              // of page j of the piece, into the buffer of the tile's page's parity
             if (lead) {
                 const int k_slot = (before + j) % C::KS, buf = (mine + j) & 1;
@@ -638,7 +643,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             }
             __syncwarp();
         };
-        auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait(bar, parity, abort_s); };
+        auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait<POLLS>(bar, parity, abort_s); };
         auto k_of = [&](int j) { return Phase{k_full + 8 * ((before + j) % C::KS), (uint32_t)((before + j) / C::KS) & 1u}; };
         auto v_of = [&](int j) { return Phase{v_full + 8 * ((before + j) % C::VS), (uint32_t)((before + j) / C::VS) & 1u}; };
         auto wait_k = [&](int j) { return wait(k_of(j).bar, k_of(j).parity); };
@@ -648,6 +653,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
                 tc::mbar_expect_tx(q_full + 8 * t, C::Q_BYTES);
                 bulk_copy(base + C::Q_AT + t * C::Q_BYTES, p.images + row_tile(c, p, x.b, x.h, x.r0 / kTileRows + t) * C::Q_BYTES, C::Q_BYTES, q_full + 8 * t);
             }
+            asked += t < x.tiles ? 1 : 0;
             __syncwarp();
         };
         bool ok = true, more = true;
@@ -658,7 +664,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             more = walk.more();
             if (more) y = walk.next(c, p);
             if (t < x.tiles) {
-                ok = wait(q_full + 8 * t, (uint32_t)(asked++) & 1u);
+                ok = wait(q_full + 8 * t, (uint32_t)(begun++) & 1u);
                 for (int j = 0; j < min(x.n, 2) && ok; ++j) {
                     ok = wait_k(j);
                     if (!ok) break;
@@ -668,7 +674,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
                 for (int j = 0; j < x.n && ok; ++j) {
                     const int buf = (mine + j) & 1;
                     const Phase weights{p_full + 8 * (t * 2 + buf), (uint32_t)((mine + j) >> 1) & 1u};
-                    ok = warp_wait(v_of(j), j + 2 < x.n ? k_of(j + 2) : weights, weights, abort_s);
+                    ok = warp_wait<POLLS>(v_of(j), j + 2 < x.n ? k_of(j + 2) : weights, weights, abort_s);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     if (j == x.n - 1 && more) ask(y);            // weights of the last page: all scores are through
@@ -701,22 +707,25 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             before += x.n;
             x = y;
         }
-        if (!ok) {                                               // given up: the products issued end before the block leaves (bounded)
-            *abort_s = 1;
-            volatile int go_on = 0;
-            if (lead) tc::umma_commit(drain + 8 * t);
-            __syncwarp();
-            (void)tc::mbar_wait(drain + 8 * t, 0, &go_on);
-        }
+        if (!ok) *abort_s = 1;
+        if (lane == 0) asked_s[t] = asked;
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (*abort_s != 0 && tid == 0) {                             // and the copies land
+    if (*abort_s != 0) {                                         // given up: products and copies on their way end before the block leaves (bounded)
         volatile int go_on = 0;
-        for (int i = 0; i < 2; ++i) { (void)tc::mbar_wait(q_full + 8 * i, 0, &go_on); (void)tc::mbar_wait(q_full + 8 * i, 1, &go_on); }
-        for (int i = 0; i < C::RAW; ++i) { (void)tc::mbar_wait(raw_full + 8 * i, 0, &go_on); (void)tc::mbar_wait(raw_full + 8 * i, 1, &go_on); }
-        raise(c, kWait);
+        if (warp == 12 || warp == 13) {
+            const int t = warp - 12, asked = asked_s[t];
+            if (elect_one()) tc::umma_commit(drain + 8 * t);     // the lane that issued the products
+            __syncwarp();
+            (void)tc::mbar_wait(drain + 8 * t, 0, &go_on);
+            if (asked > 0) (void)tc::mbar_wait(q_full + 8 * t, (uint32_t)(asked - 1) & 1u, &go_on);
+        } else if (warp == 14) {
+            const int asked = asked_s[2];
+            for (int j = max(0, asked - C::RAW); j < asked; ++j) (void)tc::mbar_wait(raw_full + 8 * (j % C::RAW), (uint32_t)(j / C::RAW) & 1u, &go_on);
+        }
+        if (tid == 0) { raise(c, kWait); p.lost[p.few_blocks + blockIdx.x] = 1; }
     }
     __syncthreads();
     if (warp == 12) {
@@ -780,7 +789,7 @@ struct WeightsCfg {
     static constexpr int G = D / 64, KEYS = 128, ROWS = 128, K_PART = Tile<D>::V_CODES;       // keys of a block, packed rows of a step; codes and parameters of a page's keys
     static constexpr int K_BYTES = KEYS * 128 * G, Q_BYTES = ROWS * 128 * G;                 // K: of its high and of its low half
     static constexpr int K_AT = 0, Q_AT = 2 * K_BYTES, PAR_AT = Q_AT + 2 * Q_BYTES, SUM_AT = PAR_AT + 2 * 3 * ROWS * 4, RAW_AT = SUM_AT + KEYS * 4, BARS = RAW_AT + 2 * K_PART;
-    static constexpr size_t SMEM = BARS + 96 + 1024;
+    static constexpr size_t SMEM = BARS + 112 + 1024;
 };
 constexpr int kWeightThreads = 13 * 32;
 
@@ -791,7 +800,7 @@ constexpr int kWeightThreads = 13 * 32;
 // grid (blocks of 128 cached rows, kv heads, batch).  Bound: exponentials and tensor pipe alike (1024 cycles a step each, of 1500 - 1600), and
 // 4 us of a block's life before its first step.  16 sequences of 1 .. 256 rows on up to 2056, 16 heads on 2 of 128: 43 us.  Two blocks an SM
 // with one buffer for the rows: 54.
-template <typename T, int D>
+template <typename T, int D, int POLLS = kPolls>
 __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const Cache c, const AttnParams p) {
     using C = WeightsCfg<D>;
     using L = Tile<D>;
@@ -801,12 +810,14 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
     unsigned char* sm = weights_smem + (base - raw_base);
     const uint32_t bars = base + C::BARS, raw_full = bars, q_full = bars + 8, q_empty = bars + 24, s_full = bars + 40, s_empty = bars + 56, drain = bars + 72, k_full = bars + 80;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::BARS + 88);
-    volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int *abort_s = reinterpret_cast<volatile int*>(tmem_slot + 1), *brought_s = abort_s + 1;      // brought_s: steps that warps 8-11 have brought
     const int tid = threadIdx.x, warp = tid >> 5, h = blockIdx.y, b = blockIdx.z, group = c.q_heads / c.kv_heads, key0 = blockIdx.x * C::KEYS;
 
     pdl_wait();                                                  // lengths, pages and keys are what earlier launches wrote
     const Entry e = entry_of(c, p, b);
     if (key0 >= e.len) return;
+    bool lost = false;
+    for (int i = tid; i < p.n_lost && tid < 256; i += 256) lost = lost || p.lost[i] != 0;
     int page[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) page[i] = key0 + i * kRows < e.len ? page_of(c, b, key0 / kRows + i) : -1;
@@ -832,7 +843,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
     const uint32_t tmem = *tmem_slot;
     pdl_launch_dependents();                                     // not before this block has its tensor memory
     if (warp < 8) {                                              // the keys, while the other warps fetch rows
-        const bool came = warp_wait(raw_full, 0, abort_s);
+        const bool came = warp_wait<POLLS>(raw_full, 0, abort_s);
         if (!came) *abort_s = 1;
         __half2 par[2][G];
         bool wide = false;
@@ -872,7 +883,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
 
     const int rows = e.n * group, first_row = max(0, key0 - (e.len - e.n)) * group / C::ROWS * C::ROWS;       // rows before do not see the block
     const int n = rows > first_row ? (rows - first_row + C::ROWS - 1) / C::ROWS : 0;
-    auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait(bar, parity, abort_s); };
+    auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait<POLLS>(bar, parity, abort_s); };
     if (warp < 8) {
         const int key = key0 + (tid & 127), half = warp >> 2;         // which half of a step's rows
         uint64_t sum[2] = {0, 0};
@@ -902,13 +913,13 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             warp_arrive(s_empty + 8 * st);
         }
-        if (i < n) *abort_s = 1;
+        if (i < n || lost) *abort_s = 1;                         // lost: not all rows' sums were there
         float* other = reinterpret_cast<float*>(sm + C::SUM_AT);
         const float mine = (low_of(sum[0]) + high_of(sum[0])) + (low_of(sum[1]) + high_of(sum[1]));
         if (half == 1) other[tid & 127] = mine;
         asm volatile("bar.sync 1, 256;" ::: "memory");
         const int pg = page[(tid & 127) >> 6];
-        if (half == 0 && i == n && key < e.len && pg >= 0) {
+        if (half == 0 && *abort_s == 0 && key < e.len && pg >= 0) {              // both halves, and the keys, were there
             const size_t at = row_slot(c, pg, h, key % kRows);
             p.mass_out[at] = p.mass_in[at] + (mine + other[tid]);
         }
@@ -945,6 +956,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
             warp_arrive(q_full + 8 * st);
         }
         if (i < n) *abort_s = 1;
+        if ((tid & 31) == 0) brought_s[warp - 8] = i;
     } else {
         constexpr uint32_t kDesc = at::instr_desc_f16(C::KEYS, C::ROWS);
         const uint32_t lead = elect_one(), tm = __shfl_sync(0xffffffffu, tmem, 0);
@@ -968,22 +980,27 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
             }
             __syncwarp();
         }
-        if (!ok) {                                               // given up: the products issued end before the block leaves (bounded)
-            *abort_s = 1;
-            volatile int go_on = 0;
-            if (lead) tc::umma_commit(drain);
-            __syncwarp();
-            (void)tc::mbar_wait(drain, 0, &go_on);
-        }
+        if (!ok) *abort_s = 1;
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (*abort_s != 0 && tid == 0) {                             // and the copies land
+    if (*abort_s != 0) {                                         // given up: products and copies on their way end before the block leaves (bounded)
         volatile int go_on = 0;
-        (void)tc::mbar_wait(raw_full, 0, &go_on);
-        for (int i = 0; i < min(n, 2); ++i) { (void)tc::mbar_wait(q_full + 8 * i, 0, &go_on); (void)tc::mbar_wait(q_full + 8 * i, 1, &go_on); }
-        raise(c, kWait);
+        const int brought = brought_s[0];                        // warp 8 asked for the rows; the other three arrive for the steps that they did not come to
+        if (warp > 8 && warp < 12 && (tid & 31) == 0)
+            for (int i = brought_s[warp - 8]; i < brought; ++i) mbar_arrive(q_full + 8 * (i & 1));
+        if (warp == 8)
+            for (int i = max(0, brought - 2); i < brought; ++i) (void)tc::mbar_wait(q_full + 8 * (i & 1), (uint32_t)(i >> 1) & 1u, &go_on);
+        if (warp == 12) {
+            if (elect_one()) tc::umma_commit(drain);             // the lane that issued the products
+            __syncwarp();
+            (void)tc::mbar_wait(drain, 0, &go_on);
+        }
+        if (tid == 0) {
+            (void)tc::mbar_wait(raw_full, 0, &go_on);
+            raise(c, kWait);
+        }
     }
     __syncthreads();
     if (warp == 12) {

@@ -41,7 +41,8 @@ enum {
     EFM_KV4_FULL = 2,         /* append: a sequence has no more page_table columns; the row is dropped and not counted */
     EFM_KV4_BAD_COUNT = 4,    /* a length or row count beyond what the call was given (max_len, max_new, max_rows) or negative: cut to it; where
                                * cu_rows falls, append takes its running maximum, so that a row stays with the first sequence that names it */
-    EFM_KV4_WAIT = 8          /* a bounded wait for a copy or product inside a kernel gave up; the call's outputs are void */
+    EFM_KV4_WAIT = 8          /* attention: a bounded wait for a copy or product inside a kernel gave up; out is void, mass_out has what it had
+                               * or, row by row, the whole sum */
 };
 
 typedef struct efm_kv4_cache {
