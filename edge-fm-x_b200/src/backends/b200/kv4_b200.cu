@@ -178,7 +178,9 @@ struct AttnPlan {
     int64_t lost;                                     // a word a block of either kernel
     bool joined;                                      // pieces of a row may lie in several blocks
     bool scores;                                      // attend_few leaves its scores for the summed weights
-    int64_t units, stats, part_stats, part, score_ld, score, image, image_units, starts;
+    int64_t units, stats, part_stats, part, score, image, image_units, starts;
+    bool by_rows;                                     // stats and operands in the order of the call's rows, not so many a sequence
+    int score_pages;                                  // scores: pages a sequence; 0: by the pool's pages
     int row_tiles;                                    // tiles of 128 packed rows a sequence may have as operands; 0: nobody asks for them
     int64_t bytes() const { return 4 * (stats + part_stats + part + score + image + image_units + starts + many_starts + many_stats + many_part + lost); }
 };
@@ -212,14 +214,20 @@ AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
     p.blocks = (int)std::max<int64_t>(1, std::min<int64_t>(kSms * (p.nt == 1 ? 3 : 2), (p.units + kv4::kWarps - 1) / kv4::kWarps));
     p.joined = pages > 1 << p.unit_shift;
     p.scores = a->mass_out != nullptr && rows <= R;
-    p.stats = a->mass_out != nullptr ? round_up(2 * (int64_t)c->batch * p.max_new * c->q_heads, 4) : 0;
+    // Whatever a batch could have if every sequence were its longest is more than the call's buffers and the pool can hold: 64 sequences of
+    // 28 query heads of 128 with 2048 rows or one, 2111 in all, would have 954 MB of operands (by rows: 23), and 64 tokens with weights on up to
+    // 131072 rows 1074 MB of scores, where a pool of 147 MB has 33 MB of them (with mass no page is two sequences').
+    p.by_rows = a->max_rows < (int64_t)c->batch * p.max_new;
+    p.stats = a->mass_out != nullptr ? round_up(2 * (p.by_rows ? (int64_t)a->max_rows : (int64_t)c->batch * p.max_new) * c->q_heads, 4) : 0;
     const int64_t pieces = p.joined ? 2 * (int64_t)p.blocks * kv4::kWarps * R : 0;      // two a warp: the one it begins in and the one it ends in
     p.part_stats = 2 * pieces;
     p.part = pieces * c->head_dim;
     p.starts = round_up(c->batch + 1, 4);
-    p.score_ld = round_up(p.max_len, kRows);                   // every part a multiple of 16 bytes
     p.row_tiles = p.many_tiles > 0 || (a->mass_out != nullptr && !p.scores) ? (int)((rows + kv4::kTileRows - 1) / kv4::kTileRows) : 0;
-    p.image_units = (int64_t)c->batch * c->kv_heads * p.row_tiles * kv4::kTileRows;
+    if (p.row_tiles > 0) {                            // every part a multiple of 16 bytes
+        const int64_t tiles_of_rows = (int64_t)a->max_rows * (c->q_heads / c->kv_heads) / kv4::kTileRows + c->batch;
+        p.image_units = (p.by_rows ? tiles_of_rows : (int64_t)c->batch * p.row_tiles) * c->kv_heads * kv4::kTileRows;
+    }
     p.image = p.image_units * c->head_dim / 2;
     if (p.many_tiles > 0) {                           // no more blocks of rows than one a sequence and those that all rows fill
         const int64_t tiles_all = std::min<int64_t>((int64_t)c->batch * p.many_tiles, c->batch + (int64_t)a->max_rows * (c->q_heads / c->kv_heads) / kv4::kManyRows);
@@ -230,7 +238,8 @@ AttnPlan plan_attention(const efm_kv4_cache* c, const efm_kv4_attention* a) {
         p.many_part = 2 * (int64_t)p.many_blocks * kv4::kManyRows * c->head_dim;
     }
     p.lost = rows > 0 ? round_up(p.blocks + p.many_blocks, 4) : 0;
-    p.score = p.scores ? (int64_t)c->batch * c->kv_heads * R * p.score_ld : 0;
+    p.score_pages = c->batch * pages <= c->n_pages ? (int)pages : 0;
+    p.score = p.scores ? (p.score_pages > 0 ? c->batch * pages : c->n_pages) * c->kv_heads * R * kRows : 0;
     return p;
 }
 
@@ -395,13 +404,13 @@ efm_status efm_b200_op_kv4_attention(const efm_kv4_cache* cache, const efm_kv4_a
         p.cu_rows = a->cu_rows; p.lens = a->lens; p.q = a->q; p.out = a->out;
         p.scale_log2 = a->scale * 1.4426950408889634f;
         p.mass_in = a->mass_in; p.mass_out = a->mass_out;
-        p.few_rows = plan.few_rows; p.warps = plan.blocks * kv4::kWarps; p.unit_shift = plan.unit_shift; p.group_inv = group == 1 ? 0u : (uint32_t)(((1ull << 32) + group - 1) / group); p.rows = plan.max_new;
+        p.few_rows = plan.few_rows; p.warps = plan.blocks * kv4::kWarps; p.unit_shift = plan.unit_shift; p.group_inv = group == 1 ? 0u : (uint32_t)(((1ull << 32) + group - 1) / group); p.rows = plan.by_rows ? 0 : plan.max_new;
         float* ws = (float*)a->workspace;
         p.stats = plan.stats > 0 ? (float2*)ws : nullptr;
         p.part_stats = (float2*)(ws + plan.stats);
         p.part = ws + plan.stats + plan.part_stats;
         p.scores = plan.scores ? p.part + plan.part : nullptr;
-        p.score_ld = plan.score_ld;
+        p.score_pages = plan.score_pages;
         p.row_tiles = plan.row_tiles;
         p.images = (uint8_t*)(ws + plan.stats + plan.part_stats + plan.part + plan.score);
         p.units = (float*)p.images + plan.image;

@@ -23,22 +23,22 @@ struct AttnParams {
     int few_rows;             // sequences with at most this many packed rows (new rows x heads of a group) are attend_few's
     int warps, unit_shift;    // attend_few's warps; pages of a unit of work: 1 << unit_shift
     uint32_t group_inv;       // ceil(2^32 / heads of a group), 0 for one: what packed rows are divided by
-    float2* stats;            // [batch, rows, q_heads] (maximum, sum) of a row's weights, where one warp had all its keys; null: not wanted
-    int rows;                 // new rows a sequence has in stats
+    float2* stats;            // [rows, q_heads] (maximum, sum) of a row's weights, where one warp had all its keys; null: not wanted
+    int rows, row_tiles;      // rows and tiles of 128 packed rows that a sequence has in stats and images; rows 0: they follow each other as
+                              // in the call's buffers, and a sequence's first tile is row0 x group / 128 + b (one has at most n x group / 128 + 1)
     float2* part_stats;       // [8 nt][2 warps] the same of the keys a warp had, and
     float* part;              // [2 warps][8 nt][D] its weighted values: slot 0 is the piece its range begins with, slot 1 the one it ends with
     int32_t* starts;          // [batch + 1] units ahead of every sequence, and all of them
     int32_t* lost;            // [n_lost] of attend_few's blocks, then of attend_many's: 1 where a wait gave up.  Weights are not summed then
     int few_blocks, n_lost;
-    uint8_t* images;          // [batch, kv_heads, row_tiles][128 x D fp16] packed rows as operands, and
-    float* units;             // [batch, kv_heads, row_tiles][128] what their scores are multiplied with; where many rows are a sequence's
-    int row_tiles;
+    uint8_t* images;          // [tiles, kv_heads][128 x D fp16] packed rows as operands, and
+    float* units;             // [tiles, kv_heads][128] what their scores are multiplied with; where many rows are a sequence's
     int many_tiles, many_blocks;      // blocks of 256 packed rows a sequence may have; blocks of attend_many
     int32_t* many_starts;     // [batch x many_tiles + 2] its units ahead, all of them, and those of each if blocks of rows stay whole
     float2* many_stats;       // [2 many_blocks][256] and
     float* many_part;         // [2 many_blocks][D / 4][256][4] what part_stats and part are, of its pieces
-    float* scores;            // [batch, kv_heads, 8 nt][score_ld] scores in units of log2; null: not wanted
-    int64_t score_ld;
+    float* scores;            // [pages, kv_heads][64][8 nt] scores in units of log2; null: not wanted
+    int score_pages;          // pages a sequence has there; 0: they are the pool's
 };
 
 // New rows and cache rows of sequence b, cut to what the call was given.
@@ -53,8 +53,8 @@ __device__ __forceinline__ Entry entry_of(const Cache& c, const AttnParams& p, i
     e.len = held(c, p.lens, b, min(p.max_len, c.max_pages * kRows));
     return e;
 }
-__device__ __forceinline__ size_t stat_row(const Cache& c, const AttnParams& p, int b, int i, int head) {
-    return ((size_t)b * p.rows + i) * c.q_heads + head;
+__device__ __forceinline__ size_t stat_row(const Cache& c, const AttnParams& p, const Entry& e, int b, int i, int head) {
+    return ((p.rows > 0 ? (size_t)b * p.rows : (size_t)e.row0) + i) * c.q_heads + head;
 }
 
 constexpr int kWarps = 4;
@@ -295,6 +295,7 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int sums[kWarps], before_s[kWarps], first_s[kWarps];
     __shared__ Entry entry_s[kWarps];
+    __shared__ volatile int stage_page_s[kWarps][C::STAGES];                     // the page in a stage, -1: none of the pool's
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::RING);
     volatile int* abort_s = reinterpret_cast<volatile int*>(bars + kWarps * C::STAGES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3, group = c.q_heads / c.kv_heads;
@@ -376,9 +377,13 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
         u += last - first;
         return x;
     };
+    auto value_params = [&](const uint8_t* page, int t, uint32_t (&w)[G]) {      // read for the largest scale and again for the values: kept they take 16 registers
+        const uint32_t at = tc::smem_u32(page) + (uint32_t)(L::V_PARAMS + t * G * 4);
+        if constexpr (G == 2) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[G - 1]) : "r"(at));
+        else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(at));
+    };
     auto row_at = [&](const Piece& x, int row) { return ((size_t)(x.e.row0 + by_group(row)) * c.q_heads + x.h * group + row - by_group(row) * group) * D; };
     int lane_page = -1;
-    uint32_t there = 0;                                                          // bit per stage: its page is one of the pool's
     auto request = [&](const Piece& x, int i) {
         if ((i & 31) == 0) {                                                     // a lane knows one page of 32
             const bool in = i + lane < x.mine;
@@ -386,8 +391,8 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
             if ((unsigned)lane_page >= (unsigned)c.n_pages) { if (in) raise(c, kBadPage); lane_page = -1; }
         }
         const int page = __shfl_sync(0xffffffffu, lane_page, i & 31), st = (slot + i) % C::STAGES;
-        there = page >= 0 ? there | 1u << st : there & ~(1u << st);
         if (lane == 0) {
+            stage_page_s[warp][st] = page;
             if (page >= 0) {
                 tc::mbar_expect_tx(bar0 + 8 * st, L::BYTES);
                 bulk_copy(tc::smem_u32(ring) + st * L::BYTES, tile_of<D>(c, page, x.h), L::BYTES, bar0 + 8 * st);
@@ -405,6 +410,7 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
             raw[t] = QueryTile<D>::fetch((const T*)p.q + (have ? row_at(x, row) : 0), have);
         }
         for (int i = 0; i < min(x.mine, C::STAGES); ++i) request(x, i);
+        __syncwarp();
     };
     Piece x = next_piece();
     ask(x);
@@ -456,7 +462,7 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
                 }
                 return;
             }
-            if (there >> st & 1u) {
+            if (stage_page_s[warp][st] >= 0) {
                 uint8_t* page = ring + (size_t)st * L::BYTES;
                 if (x.e.len - first < kRows) clear_rows<D>(page, x.e.len - first, true);
                 float s[4][NT][4];
@@ -472,16 +478,15 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
                                 if (first + u * 16 + token_of(r) + 8 * (k >> 1) >= see[t][k & 1]) s[u][t][k] = -INFINITY;
                 }
                 if (p.scores != nullptr) {
-                    float* to = p.scores + ((size_t)x.b * c.kv_heads + x.h) * R * p.score_ld + first + token_of(r);
+                    const uint32_t at = (uint32_t)(p.score_pages > 0 ? x.b * p.score_pages + x.p0 + i : stage_page_s[warp][st]) * c.kv_heads + x.h;      // no more than the pool's tiles
+                    float* to = p.scores + (size_t)at * (R * kRows) + token_of(r) * R + 2 * j;
 #pragma unroll
-                    for (int t = 0; t < NT; ++t)
+                    for (int u = 0; u < 4; ++u)
 #pragma unroll
-                        for (int k = 0; k < 2; ++k)
-                            if (t * 8 + 2 * j + k < rows)
+                        for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-                                for (int u = 0; u < 4; ++u)
-#pragma unroll
-                                    for (int hf = 0; hf < 2; ++hf) to[(t * 8 + 2 * j + k) * p.score_ld + u * 16 + 8 * hf] = s[u][t][2 * hf + k] * q[t].unit[k];
+                            for (int t = 0; t < NT; ++t)
+                                *reinterpret_cast<float2*>(to + (u * 16 + 8 * hf) * R + t * 8) = make_float2(s[u][t][2 * hf] * q[t].unit[0], s[u][t][2 * hf + 1] * q[t].unit[1]);
                 }
                 float top[NT][2];
 #pragma unroll
@@ -493,21 +498,15 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
                         for (int u = 1; u < 4; ++u) top[t][k] = fmaxf(top[t][k], fmaxf(s[u][t][k], s[u][t][2 + k]));
                     }
                 // parameters of the values; the largest scale is the low half of the largest pair
-                uint32_t vp[4][2][G], big2 = 0;
+                uint32_t big2 = 0;
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf) {
-                        const uint8_t* par = page + L::V_PARAMS + (u * 16 + token_of(r) + 8 * hf) * G * 4;
-                        if constexpr (G == 2) {
-                            const uint2 w = *reinterpret_cast<const uint2*>(par);
-                            vp[u][hf][0] = w.x;
-                            vp[u][hf][1] = w.y;
-                        } else {
-                            vp[u][hf][0] = *reinterpret_cast<const uint32_t*>(par);
-                        }
+                        uint32_t vp[G];
+                        value_params(page, u * 16 + token_of(r) + 8 * hf, vp);
 #pragma unroll
-                        for (int g = 0; g < G; ++g) asm("max.f16x2 %0, %0, %1;" : "+r"(big2) : "r"(vp[u][hf][g]));
+                        for (int g = 0; g < G; ++g) asm("max.f16x2 %0, %0, %1;" : "+r"(big2) : "r"(vp[g]));
                     }
                 int big = (int)(big2 & 0x7fffu);
 #pragma unroll
@@ -554,7 +553,9 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
                 const float unit = __uint_as_float((uint32_t)(127 + 14 - ev) << 23);
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    uint32_t b0[G][NT], b1[G][NT];
+                    uint32_t b0[G][NT], b1[G][NT], va[G], vb[G];
+                    value_params(page, u * 16 + token_of(r), va);
+                    value_params(page, u * 16 + token_of(r) + 8, vb);
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -564,7 +565,7 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
                         }
 #pragma unroll
                     for (int g = 0; g < G; ++g) {
-                        const float2 a = centred(vp[u][0][g]), bb = centred(vp[u][1][g]);
+                        const float2 a = centred(va[g]), bb = centred(vb[g]);
                         const float sa = a.x * unit, sb = bb.x * unit;
 #pragma unroll
                         for (int t = 0; t < NT; ++t) {
@@ -645,7 +646,7 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
                 }
                 if (r == 0) {
                     if (!alone) p.part_stats[(size_t)rr * 2 * p.warps + piece] = make_float2(m[t][k], l[t][k]);
-                    else if (p.stats != nullptr) p.stats[stat_row(c, p, done.b, by_group(row), done.h * group + row - by_group(row) * group)] = make_float2(m[t][k], l[t][k]);
+                    else if (p.stats != nullptr) p.stats[stat_row(c, p, done.e, done.b, by_group(row), done.h * group + row - by_group(row) * group)] = make_float2(m[t][k], l[t][k]);
                 }
             }
     }
@@ -705,25 +706,36 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
     if ((int)blockIdx.x < mass_blocks) {
         const int t0 = blockIdx.x * kMassTokens;
         if (t0 >= e.len) return;
+        constexpr int PER = kMassTokens / (kWarps * 32);
+        int page[PER];
+#pragma unroll
+        for (int k = 0; k < PER; ++k) { const int tk = t0 + threadIdx.x + k * kWarps * 32; page[k] = tk < e.len ? page_of(c, b, tk / kRows) : -1; }
         const Pieces x = rows > 0 ? pieces_of(p, sh, Deal{p.starts[b], p.starts[c.batch]}, h, 0) : Pieces{0, 0};
         bool lost = false;
         for (int i = x.w0 / kWarps + (int)threadIdx.x; rows > 0 && i <= x.w1 / kWarps; i += kWarps * 32) lost = lost || p.lost[i] != 0;
         for (int row = warp; row < rows; row += kWarps) {
-            const float2 s = x.w0 == x.w1 ? p.stats[stat_row(c, p, b, row / group, h * group + row % group)] : merged_stats(p, x, row);
+            const float2 s = x.w0 == x.w1 ? p.stats[stat_row(c, p, e, b, row / group, h * group + row % group)] : merged_stats(p, x, row);
             if (lane == 0) st_s[row] = s.x == -INFINITY ? make_float2(0.f, 0.f) : make_float2(s.x, 1.0f / s.y);
         }
         if (__syncthreads_or(lost)) return;                      // not all scores are there
-        constexpr int PER = kMassTokens / (kWarps * 32);
         float w[PER];
-        const float* from = p.scores + ((size_t)b * c.kv_heads + h) * R * p.score_ld + t0 + threadIdx.x;
+        const float* from[PER];
 #pragma unroll
-        for (int k = 0; k < PER; ++k) w[k] = 0.f;
+        for (int k = 0; k < PER; ++k) {
+            const int tk = t0 + threadIdx.x + k * kWarps * 32;
+            w[k] = 0.f;
+            from[k] = p.scores + ((p.score_pages > 0 ? (size_t)b * p.score_pages + tk / kRows : (size_t)max(page[k], 0)) * c.kv_heads + h) * (R * kRows) + tk % kRows * R;
+        }
         for (int row = 0; row < rows; row += 4) {                // four rows' scores on their way at a time
             float s[4][PER];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int k = 0; k < PER; ++k) s[i][k] = row + i < rows && t0 + (int)threadIdx.x + k * kWarps * 32 < e.len ? from[(row + i) * p.score_ld + k * kWarps * 32] : -INFINITY;
+            for (int k = 0; k < PER; ++k) {
+                const float4 v = page[k] >= 0 ? *reinterpret_cast<const float4*>(from[k] + row) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                s[0][k] = v.x;
+                s[1][k] = row + 1 < rows ? v.y : -INFINITY;
+                s[2][k] = row + 2 < rows ? v.z : -INFINITY;
+                s[3][k] = row + 3 < rows ? v.w : -INFINITY;
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float2 st = st_s[min(row + i, rows - 1)];
@@ -733,10 +745,8 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
         }
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-            const int tk = t0 + threadIdx.x + k * kWarps * 32;
-            const int page = tk < e.len ? page_of(c, b, tk / kRows) : -1;
-            if (page < 0) continue;
-            const size_t at = row_slot(c, page, h, tk % kRows);
+            if (page[k] < 0) continue;
+            const size_t at = row_slot(c, page[k], h, (t0 + threadIdx.x + k * kWarps * 32) % kRows);
             p.mass_out[at] = p.mass_in[at] + w[k];
         }
         return;
@@ -778,7 +788,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
             T* dst = (T*)p.out + ((size_t)(e.row0 + i) * c.q_heads + head) * D + lane * E;
 #pragma unroll
             for (int k = 0; k < E; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = within2<T>(v[k] * inv, v[k + 1] * inv);
-            if (lane == 0 && p.stats != nullptr && mass_blocks == 0) p.stats[stat_row(c, p, b, i, head)] = st;
+            if (lane == 0 && p.stats != nullptr && mass_blocks == 0) p.stats[stat_row(c, p, e, b, i, head)] = st;
         }
         return;
     }
@@ -817,7 +827,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
             for (int k = 1; k < LANES; ++k) { const float4 y = v_s[k * Q + threadIdx.x]; v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w; }
             const float inv = st.y > 0.f ? 1.0f / st.y : st.y != st.y ? st.y : 0.f;
             *reinterpret_cast<uint2*>((T*)p.out + ((size_t)(e.row0 + i) * c.q_heads + head) * D + d) = make_uint2(within2<T>(v.x * inv, v.y * inv), within2<T>(v.z * inv, v.w * inv));
-            if (threadIdx.x == 0 && d == 0 && p.stats != nullptr && mass_blocks == 0) p.stats[stat_row(c, p, b, i, head)] = st;
+            if (threadIdx.x == 0 && d == 0 && p.stats != nullptr && mass_blocks == 0) p.stats[stat_row(c, p, e, b, i, head)] = st;
         }
         __syncthreads();
     }

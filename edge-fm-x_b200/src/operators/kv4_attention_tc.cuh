@@ -239,7 +239,10 @@ __device__ __forceinline__ void quarter_words(const uint32_t* codes, int r, int 
     }
 }
 
-__device__ __forceinline__ size_t row_tile(const Cache& c, const AttnParams& p, int b, int h, int tile) { return ((size_t)b * c.kv_heads + h) * p.row_tiles + tile; }
+__device__ __forceinline__ size_t row_tile(const Cache& c, const AttnParams& p, const Entry& e, int b, int h, int tile) {
+    const size_t first = p.rows > 0 ? (size_t)b * p.row_tiles : (size_t)e.row0 * (c.q_heads / c.kv_heads) / kTileRows + b;
+    return (first + tile) * c.kv_heads + h;
+}
 
 // How attend_many's work is dealt: its units are the pages of every (sequence, block of 256 packed rows, kv head), in that order, block w of
 // the grid has the units [w step, (w + 1) step).  Rows that begin or end inside such a range are joined by attend_join.
@@ -366,7 +369,7 @@ __global__ void __launch_bounds__(kTileRows) attend_query_kernel(const Cache c, 
     const Entry e = entry_of(c, p, b);
     const int rows = e.n * group;
     if ((int)blockIdx.x * kTileRows >= rows) return;
-    const size_t tile = row_tile(c, p, b, h, blockIdx.x);
+    const size_t tile = row_tile(c, p, e, b, h, blockIdx.x);
     const long long at = row < rows ? ((long long)(e.row0 + row / group) * c.q_heads + h * group + row % group) * D : -1;
     p.units[tile * kTileRows + threadIdx.x] = query_rows<T, D>((const T*)p.q, at, p.images + tile * (kTileRows * D * 2), threadIdx.x & ~31, p.scale_log2);
 }
@@ -428,7 +431,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
             int least = have ? see : INT32_MAX;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
-            const float unit = p.units[row_tile(c, p, x.b, x.h, x.r0 / kTileRows + t) * kTileRows + tr];
+            const float unit = p.units[row_tile(c, p, x.e, x.b, x.h, x.r0 / kTileRows + t) * kTileRows + tr];
             float m = -INFINITY, l = 0.f;                        // m: what the row's weights are relative to
             int j = 0;
             for (; j < x.n; ++j) {
@@ -512,7 +515,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
                             *reinterpret_cast<uint4*>(out + d + i) = make_uint4(z[0], z[1], z[2], z[3]);
                         }
                 }
-                if (have && p.stats != nullptr) p.stats[stat_row(c, p, x.b, row / group, head)] = make_float2(m == -INFINITY ? m : m - kLift, l);
+                if (have && p.stats != nullptr) p.stats[stat_row(c, p, x.e, x.b, row / group, head)] = make_float2(m == -INFINITY ? m : m - kLift, l);
             } else {                                             // [piece][channels / 4][256 rows][4]: neighbouring lanes side by side
                 const size_t piece = (size_t)(2 * blockIdx.x + (x.from_start ? 1 : 0));
                 float4* to = reinterpret_cast<float4*>(p.many_part) + piece * (D / 4) * kManyRows + t * kTileRows + tr;
@@ -651,7 +654,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
         auto ask = [&](const ManyPiece& x) {                     // the tile's queries, once no product reads those before
             if (t < x.tiles && lane == 0) {
                 tc::mbar_expect_tx(q_full + 8 * t, C::Q_BYTES);
-                bulk_copy(base + C::Q_AT + t * C::Q_BYTES, p.images + row_tile(c, p, x.b, x.h, x.r0 / kTileRows + t) * C::Q_BYTES, C::Q_BYTES, q_full + 8 * t);
+                bulk_copy(base + C::Q_AT + t * C::Q_BYTES, p.images + row_tile(c, p, x.e, x.b, x.h, x.r0 / kTileRows + t) * C::Q_BYTES, C::Q_BYTES, q_full + 8 * t);
             }
             asked += t < x.tiles ? 1 : 0;
             __syncwarp();
@@ -781,7 +784,7 @@ __global__ void __launch_bounds__(kManyRows) attend_join_kernel(const Cache c, c
     uint4* out = reinterpret_cast<uint4*>((T*)p.out + ((size_t)(e.row0 + i) * c.q_heads + head) * D + blockIdx.y * 16);
     out[0] = make_uint4(z[0], z[1], z[2], z[3]);
     out[1] = make_uint4(z[4], z[5], z[6], z[7]);
-    if (blockIdx.y == 0 && p.stats != nullptr) p.stats[stat_row(c, p, b, i, head)] = make_float2(top == -INFINITY ? top : top - kLift, sum);
+    if (blockIdx.y == 0 && p.stats != nullptr) p.stats[stat_row(c, p, e, b, i, head)] = make_float2(top == -INFINITY ? top : top - kLift, sum);
 }
 
 template <int D>
@@ -931,8 +934,8 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
             const bool have = i < n && row < rows;
             const int qr = have ? row / group : 0, head = h * group + (have ? row - qr * group : 0);
             Row x;
-            x.s = have ? p.stats[stat_row(c, p, b, qr, head)] : make_float2(-INFINITY, 0.f);
-            x.unit = have ? p.units[row_tile(c, p, b, h, first_row / C::ROWS + i) * kTileRows + tr] : 1.0f;         // not 0: times -inf
+            x.s = have ? p.stats[stat_row(c, p, e, b, qr, head)] : make_float2(-INFINITY, 0.f);
+            x.unit = have ? p.units[row_tile(c, p, e, b, h, first_row / C::ROWS + i) * kTileRows + tr] : 1.0f;         // not 0: times -inf
             x.seen = min(e.len, e.len - e.n + qr + 1);
             return x;
         };
@@ -946,7 +949,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) attend_weights_kernel(const
             if (i >= 2 && !(wait(q_empty + 8 * st, (uint32_t)(i / 2 - 1) & 1u) && wait(s_empty + 8 * st, (uint32_t)(i / 2 - 1) & 1u))) break;
             if (tr == 0) {                                       // the operand as it is, the rows' parameters by these four warps
                 tc::mbar_expect_tx(q_full + 8 * st, C::Q_BYTES);
-                bulk_copy(base + C::Q_AT + st * C::Q_BYTES, p.images + row_tile(c, p, b, h, first_row / C::ROWS + i) * C::Q_BYTES, C::Q_BYTES, q_full + 8 * st);
+                bulk_copy(base + C::Q_AT + st * C::Q_BYTES, p.images + row_tile(c, p, e, b, h, first_row / C::ROWS + i) * C::Q_BYTES, C::Q_BYTES, q_full + 8 * st);
             }
             const bool sees = now.s.x != -INFINITY;              // a row that sees nothing: weights of 0
             float* par = reinterpret_cast<float*>(sm + C::PAR_AT) + st * 3 * C::ROWS + tr;
