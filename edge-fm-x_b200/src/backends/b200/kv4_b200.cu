@@ -187,14 +187,15 @@ struct AttnPlan {
 constexpr int kSms = 148;                              // of the GPU these kernels are built for
 constexpr int kWholeShift = 2;
 // Packed rows of a sequence up to which attend_few takes it, in tiles of 16.  A page costs attend_few 3.7 ns a tile of 128 channels (half
-// of it with 64) once the tiles fill the GPU; attend_many has three launches more and some 8.6 ns a block of 256 rows, however few rows are
-// in it (fp16, with its products in three parts: 14).  Equal at some 90 tiles of all sequences and kv heads (fp16: 190), and where those are
-// many, at 2 (fp16: 3) of each.  Measured (attend_few / attend_many, us): 28 query heads on 4 kv heads of 128, 4000 tokens, 32 rows (56 tiles)
-// 26 / 33, 64 rows (112) 39 / 33; 8 sequences of 2000 tokens with 32 on 4, 6 rows (96) 27 / 31, 12 rows (192) 36 / 33, fp16 16 rows (256) 40 / 41;
-// 64 such, 4 rows (2 tiles each) 72 / 82, 6 rows (3 each) 100 / 84, fp16 8 rows (4 each) 128 / 135; 64 channels, 14 on 2, 256 rows (224) 25 / 28.
+// of it with 64; fp16 a quarter more) once the tiles fill the GPU; attend_many has three launches more and some 8.6 ns a block of 256 rows,
+// however few rows are in it (fp16, with its products in three parts: 14).  Equal at some 90 tiles of all sequences and kv heads (fp16: 140), and
+// where those are many, at 2 (fp16: 3) of each.  Measured (attend_few / attend_many, us): 28 query heads on 4 kv heads of 128, 4000 tokens, 32 rows
+// (56 tiles) 26 / 33, 64 rows (112) 39 / 33, fp16 42 / 44, 96 rows (168) fp16 51 / 48; 8 sequences of 2000 tokens with 32 on 4, 6 rows (96) 27 / 31,
+// 12 rows (192, 3 each) 36 / 33, fp16 42 / 42; 64 such, 4 rows (2 tiles each) 72 / 82, 6 rows (3 each) 100 / 84, fp16 127 / 157; 64 channels, 14 on 2,
+// 256 rows (224) 25 / 28, fp16 39 / 36.
 int few_rows_of(const efm_kv4_cache* c) {
     const bool bf16 = c->dtype == EFM_BF16;
-    const int64_t each = (int64_t)c->batch * c->kv_heads, all = (bf16 ? 90 : 190) * (128 / c->head_dim);
+    const int64_t each = (int64_t)c->batch * c->kv_heads, all = (bf16 ? 90 : 140) * (128 / c->head_dim);
     return (int)(16 * std::max<int64_t>(bf16 ? 2 : 3, all / each));
 }
 

@@ -4,7 +4,8 @@
 //     q . k = sum over groups g of  scale_g (q_g . (code - 8)_g + 8 (sum of q_g)) + min_g (sum of q_g),
 // and code - 8 is exact in fp16.  q is scaled by a power of two per row and is exact there too (bf16 has fewer bits): scores carry fp32
 // rounding only.  Values: o = sum over tokens of (p scale_g) (code - 8) + sum of p c_g, with p scale_g rounded to fp16 below a power of
-// two that keeps the largest scale seen at 2^14 .. 2^15, so that neither large nor small scales leave its range.
+// two that keeps the largest scale seen at 2^14 .. 2^15, so that neither large nor small scales leave its range.  That is 2^-11 of a weight, well
+// below the half step of a bf16 output (2^-8); for fp16 outputs, whose half step it is, p scale_g is a pair high + low (2^-22).
 #pragma once
 #include "gemm_tc.cuh"
 #include "kv4_cache.cuh"
@@ -553,7 +554,8 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
                 const float unit = __uint_as_float((uint32_t)(127 + 14 - ev) << 23);
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    uint32_t b0[G][NT], b1[G][NT], va[G], vb[G];
+                    constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 1;
+                    uint32_t b0[PARTS][G][NT], b1[PARTS][G][NT], va[G], vb[G];
                     value_params(page, u * 16 + token_of(r), va);
                     value_params(page, u * 16 + token_of(r) + 8, vb);
 #pragma unroll
@@ -572,8 +574,15 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
                             const float(&w)[4] = s[u][t];
                             pc[g][t][0] = fmaf(w[0], a.y, fmaf(w[2], bb.y, pc[g][t][0]));
                             pc[g][t][1] = fmaf(w[1], a.y, fmaf(w[3], bb.y, pc[g][t][1]));
-                            b0[g][t] = transposed(half_pair(w[0] * sa, w[1] * sa));
-                            b1[g][t] = transposed(half_pair(w[2] * sb, w[3] * sb));
+                            float x[4] = {w[0] * sa, w[1] * sa, w[2] * sb, w[3] * sb};
+#pragma unroll
+                            for (int y = 0; y < PARTS; ++y) {
+                                const uint32_t h0 = half_pair(x[0], x[1]), h1 = half_pair(x[2], x[3]);
+                                b0[y][g][t] = transposed(h0);
+                                b1[y][g][t] = transposed(h1);
+                                const float2 f0 = Num<__half>::two(h0), f1 = Num<__half>::two(h1);
+                                x[0] -= f0.x; x[1] -= f0.y; x[2] -= f1.x; x[3] -= f1.y;
+                            }
                         }
                     }
                     // columns 2 j, 2 j + 1 (and 8 behind) of the operand are the tokens j, j + 4 (j + 8, j + 12)
@@ -587,10 +596,12 @@ __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few
                             const uint32_t a0[4] = {low_pair(ta), high_pair(ta), low_pair(tb), high_pair(tb)};
                             const uint32_t a1[4] = {low_pair(ta >> 8), high_pair(ta >> 8), low_pair(tb >> 8), high_pair(tb >> 8)};
 #pragma unroll
-                            for (int t = 0; t < NT; ++t) {
-                                mma16816(o[g][2 * hl][t], a0, b0[g][t], b1[g][t]);
-                                mma16816(o[g][2 * hl + 1][t], a1, b0[g][t], b1[g][t]);
-                            }
+                            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                                for (int y = 0; y < PARTS; ++y) {
+                                    mma16816(o[g][2 * hl][t], a0, b0[y][g][t], b1[y][g][t]);
+                                    mma16816(o[g][2 * hl + 1][t], a1, b0[y][g][t], b1[y][g][t]);
+                                }
                         }
                     }
                 }
