@@ -160,9 +160,15 @@ __device__ __forceinline__ void ex2_pair(uint64_t x, float& a, float& b) {
     a = __uint_as_float((uint32_t)y + ((uint32_t)n << 23));
     b = __uint_as_float((uint32_t)(y >> 32) + ((uint32_t)(n >> 32) << 23));
 }
+// Maxima that keep what is no number: ex2_pair does not.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float max2(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
 // Three waits at once: polled one behind the other a wait that is over takes some 200 cycles each.
@@ -446,13 +452,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Cach
 #pragma unroll
                     for (int i = 0; i < 64; ++i) if (i >= seen) s[i] = -INFINITY;
                 }
-                float mx[4] = {fmaxf(s[0], s[1]), fmaxf(s[2], s[3]), fmaxf(s[4], s[5]), fmaxf(s[6], s[7])};
+                float mx[4] = {max2(s[0], s[1]), max2(s[2], s[3]), max2(s[4], s[5]), max2(s[6], s[7])};
 #pragma unroll
                 for (int i = 8; i < 64; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], s[i], s[i + 1]);
-                const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * unit;
-                const bool grow = mn > m + kGrow || (m == -INFINITY && mn != -INFINITY);
+                const float mn = max2(max2(mx[0], mx[1]), max2(mx[2], mx[3])) * unit;
+                const bool grow = !(mn <= m + kGrow);
                 float alpha = 1.0f;
-                if (grow) { alpha = at::ex2(m - mn); l *= alpha; m = mn; }
+                if (grow) { alpha = at::ex2(m - mn); l *= alpha; m = mn + (mn - mn); }       // an infinite maximum has no weights: NaN
                 const float off = m == -INFINITY ? kLift : kLift - m;
                 uint32_t pk[32], pl[X == 2 ? 32 : 1];
                 uint64_t sum = 0;

@@ -75,6 +75,35 @@ def test_append_falling_counts_of_many_sequences():
     assert [g[0] for g in got] == [0, kv.BAD_COUNT] and all(torch.equal(a, b) for a, b in zip(got[0][1], got[1][1]))
 
 
+@pytest.mark.parametrize("counts,mass", [([60] * 6, False), ([60] * 6, True), ([1] * 6, False)])
+@pytest.mark.parametrize("held", [1.0, 0.0])
+def test_scores_beyond_all_numbers_show(counts, mass, held):
+    """An infinite query channel meets one key (of any place in a page) that is positive or 0 there, all others negative: weights of inf - inf, or
+    of 0 inf.  NaN like every row whose scores are no numbers, and no other row changes."""
+    kh, d, L = 16, 64, 60
+    for place in (0, 3, 6, 7, 38, 55):
+        c = kv.KV4(kh, kh, d, [0] * 6, [L] * 6, "bf16", seed=place)
+        x = c.normal(6 * L, kh * d)
+        k = x.clone().view(6, L, kh, d)
+        k[..., 0] = -1.0 - k[..., 0].abs()
+        k[:, place] = 0.0
+        k[:, place, :, 0] = held
+        out = c.ints([0] * 6)
+        c.do("append", c.append_args([L] * 6, out, None, k.view(6 * L, kh * d), x))
+        q = c.normal(sum(counts), kh, d)
+        got = [torch.zeros_like(q) for _ in range(2)]
+        m = torch.zeros(c.n_pages, kh, 64, device=c.dev) if mass else None
+        c.do("attention", c.attention_args(counts, out, q, got[0], mass=m))
+        row = counts[0] - 1                                       # sees every key
+        q[row, 5] = 0.0
+        q[row, 5, 0] = float("inf")
+        c.do("attention", c.attention_args(counts, out, q, got[1], mass=m))
+        torch.cuda.synchronize()
+        assert c.status.item() == 0 and torch.isnan(got[1][row, 5]).all()
+        got[1][row, 5] = got[0][row, 5]
+        assert torch.equal(got[0], got[1])
+
+
 # ---- waits that run out ----------------------------------------------------------------------------------------------------
 def hasty_calls():
     """In a process of its own, since the library looks for the variable once.  Waits give up after a few polls: copies and products on their
