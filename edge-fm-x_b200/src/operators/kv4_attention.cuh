@@ -2,8 +2,8 @@
 //
 // The codes go to the tensor cores as they are: a key is min + scale * code = c + scale * (code - 8) with c = min + 8 scale, so that
 //     q . k = sum over groups g of  scale_g (q_g . (code - 8)_g + 8 (sum of q_g)) + min_g (sum of q_g),
-// and code - 8 is exact in fp16.  q is scaled by a power of two per row and is exact there too (bf16 has fewer bits): scores carry fp32
-// rounding only.  Values: o = sum over tokens of (p scale_g) (code - 8) + sum of p c_g, with p scale_g rounded to fp16 below a power of
+// and code - 8 is exact in fp16.  q is scaled by a power of two per row and is exact there too, but for channels 2^17 (bf16 2^20) below the
+// row's largest, which lose bits below fp16's normal range: scores carry fp32 rounding only.  Values: o = sum over tokens of (p scale_g) (code - 8) + sum of p c_g, with p scale_g rounded to fp16 below a power of
 // two that keeps the largest scale seen at 2^14 .. 2^15, so that neither large nor small scales leave its range.  That is 2^-11 of a weight, well
 // below the half step of a bf16 output (2^-8); for fp16 outputs, whose half step it is, p scale_g is a pair high + low (2^-22).
 #pragma once
@@ -287,7 +287,7 @@ struct FewCfg {
 // single token of up to 8 heads per kv head fills it: m16n8k16 the other way round would leave half of it empty.
 // Bound: instruction issue, 1280 a page of 64 x 128 (a third of them on the integer pipe, which takes the codes apart, half floating point),
 // of which three blocks an SM, as many as registers allow, reach 57 % of the slots; then bytes.  One token, 28 heads on 4 kv heads of 128, on
-// 131000 rows: 28 us, 2.8 TB/s; on 64 caches of 300 .. 4000: 31 us, 2.7 TB/s.
+// 131000 rows: 28 us, 2.8 TB/s; on 64 caches of 300 .. 4000: 30 us, 2.7 TB/s.
 template <typename T, int D, int NT, int POLLS = kPolls>
 __global__ void __launch_bounds__(kWarps * 32, FewCfg<D, NT>::BLOCKS) attend_few_kernel(const Cache c, const AttnParams p) {
     using L = Tile<D>;
@@ -711,6 +711,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
     const int h = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = c.q_heads / c.kv_heads;
     pdl_wait();
     pdl_launch_dependents();
+    const Deal deal{p.starts[b], p.starts[c.batch]};             // on its way with the lengths; of no use where nothing was dealt
     const Entry e = entry_of(c, p, b);
     const Share sh = share_of<R>(c, p, e, group);
     const int rows = sh.tiles > 0 ? e.n * group : 0;
@@ -721,7 +722,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
         int page[PER];
 #pragma unroll
         for (int k = 0; k < PER; ++k) { const int tk = t0 + threadIdx.x + k * kWarps * 32; page[k] = tk < e.len ? page_of(c, b, tk / kRows) : -1; }
-        const Pieces x = rows > 0 ? pieces_of(p, sh, Deal{p.starts[b], p.starts[c.batch]}, h, 0) : Pieces{0, 0};
+        const Pieces x = rows > 0 ? pieces_of(p, sh, deal, h, 0) : Pieces{0, 0};
         bool lost = false;
         for (int i = x.w0 / kWarps + (int)threadIdx.x; rows > 0 && i <= x.w1 / kWarps; i += kWarps * 32) lost = lost || p.lost[i] != 0;
         for (int row = warp; row < rows; row += kWarps) {
@@ -763,7 +764,6 @@ __global__ void __launch_bounds__(kWarps * 32) attend_merge_kernel(const Cache c
         return;
     }
     if (rows == 0) return;
-    const Deal deal{p.starts[b], p.starts[c.batch]};
     const int first = (int)blockIdx.x - mass_blocks, blocks = (int)gridDim.x - mass_blocks;
     constexpr int SLICES = D / 32, Q = 8, LANES = kWarps * 32 / Q;               // threads side by side, each with four channels of every LANES-th piece
     // few pieces, or more rows than there are blocks for: a row a warp, no barriers

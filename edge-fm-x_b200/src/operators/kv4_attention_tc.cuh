@@ -12,15 +12,17 @@
 //                    buffers a tile and runs two pages ahead of P V; weights take the place of the scores they came from.  A wait costs
 //                    that warp some 200 cycles even when it is over, so it polls for all that a page needs at once; one warp for both
 //                    tiles left the tensor pipe idle half the time.
-// q is scaled by a power of two per row to be exact in fp16.  k, v and p are rounded to fp16 (2^-11), well below the half step of a bf16
-// output (2^-8).  Where that would show they are pairs high + low: k where row sums are wanted that summed weights are divided by (X 1:
-// S = Q (Kh + Kl)), and all of them for fp16 outputs (X 2: O += Ph Vh + Pl Vh + Ph Vl as well).
+// q is scaled by a power of two per row to be exact in fp16.  k, v and p are rounded to fp16: v and p by 2^-11 of themselves, below the half step
+// of a bf16 output (2^-8), and a score by 2^-11 of sum |q k| scale at most, as from a 16-bit cache of fp16 keys.  X 0, bf16 outputs without
+// mass: on 2048 rows behind 12289 1.74e-3 from the formula, where rounding the outputs is 1.66e-3 (X 1 1.68e-3, but 540 us instead of 418).
+// Pairs high + low hold more: k where row sums are wanted that summed weights are divided by (X 1: S = Q (Kh + Kl)), and all of them for fp16
+// outputs, whose half step it would be (X 2: O += Ph Vh + Pl Vh + Ph Vl as well).
 // A barrier is waited for by parity, which tells a phase from its neighbours only: every barrier here is either waited for in each of its
 // phases by whoever its next phase needs, or (o_done) has a copy per page parity, whose next phase needs the waiting thread's weights of
 // two pages later.
 // Bound: the softmax warps (some 2000 cycles a page: 1600 of arithmetic, the rest waits), ahead of the tensor pipe (1280) and the exponential
-// unit (770 after a quarter of the exponentials went to arithmetic).  2048 rows, 28 heads on 4 kv heads of 128, behind 12289: 405 - 440 us by
-// the card's clock, 890 - 960 TFLOP/s of 4 rows keys D.
+// unit (770 after a quarter of the exponentials went to arithmetic).  2048 rows, 28 heads on 4 kv heads of 128, behind 12289: 370 - 411 us by
+// the card's clock, 950 - 1060 TFLOP/s of 4 rows keys D; the whole call 400 - 450.
 #pragma once
 #include <type_traits>
 

@@ -134,7 +134,7 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float m, float
 
 // grid (rows, parts of the row's heads); a lane has eight neighbouring channels of a head (one word of codes), a warp 32 / (D / 8) heads
 // of one kind at a time.
-// Bound: instruction issue (78 % of the slots; 330 a warp and 32 / (D / 8) heads, most of them for the fixed roundings), not bytes.  3117 rows
+// Bound: instruction issue (77 % of the slots; 330 a warp and 32 / (D / 8) heads, most of them products and sums of single numbers), not bytes.  3117 rows
 // of 32 + 16 heads of 128 fp16, normed and turned: 30 us, 2.7 TB/s of what has to move.  One row: latency, some 4 us.
 template <typename T, int D>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const Cache c, const AppendParams p, int tasks_per_block) {

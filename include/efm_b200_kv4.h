@@ -89,7 +89,9 @@ typedef struct efm_kv4_append {
 } efm_kv4_append;
 
 /* Attention of new rows over the cache, which holds them already: row i of a sequence's n new rows sees its cache rows
- * [0, lens[b] - n + i].  out = softmax(scale q k^T) v; a row that sees nothing gets zeros. */
+ * [0, lens[b] - n + i].  out = softmax(scale q k^T) v; a row that sees nothing gets zeros.  Outputs are rounded once.  Before that, for EFM_BF16,
+ * weights are rounded to fp16, and where a sequence has many new rows v, and without mass k, too: out may differ in its last bits with and
+ * without mass.  Everything else, and all of it for EFM_F16, has 22 bits or more. */
 typedef struct efm_kv4_attention {
     int32_t struct_size;
     int32_t max_rows;
