@@ -61,7 +61,7 @@ __device__ __forceinline__ size_t stat_row(const Cache& c, const AttnParams& p, 
 constexpr int kWarps = 4;
 
 // Wait of a whole warp for a phase, bounded; false when it gave up.  The limit (some seconds) is a constant: read from the parameters it
-// cost attend_many 5 %, attend_few 3, of which warps that poll take issue slots from the others.  kHasty: for tests of what follows.
+// cost attend_many 5 % and attend_few 3, since warps that poll take issue slots from the others.  kHasty: for tests of what follows.
 constexpr int kPolls = 1 << 25, kHasty = 2;
 template <int POLLS>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
