@@ -3,9 +3,10 @@
 // The codes go to the tensor cores as they are: a key is min + scale * code = c + scale * (code - 8) with c = min + 8 scale, so that
 //     q . k = sum over groups g of  scale_g (q_g . (code - 8)_g + 8 (sum of q_g)) + min_g (sum of q_g),
 // and code - 8 is exact in fp16.  q is scaled by a power of two per row and is exact there too, but for channels 2^17 (bf16 2^20) below the
-// row's largest, which lose bits below fp16's normal range: scores carry fp32 rounding only.  Values: o = sum over tokens of (p scale_g) (code - 8) + sum of p c_g, with p scale_g rounded to fp16 below a power of
-// two that keeps the largest scale seen at 2^14 .. 2^15, so that neither large nor small scales leave its range.  That is 2^-11 of a weight, well
-// below the half step of a bf16 output (2^-8); for fp16 outputs, whose half step it is, p scale_g is a pair high + low (2^-22).
+// row's largest, which lose bits below fp16's normal range: scores carry fp32 rounding only.  Values: o = sum over tokens of
+// (p scale_g) (code - 8) + sum of p c_g, with p scale_g rounded to fp16 below a power of two that keeps the largest scale seen at 2^14 .. 2^15,
+// so that neither large nor small scales leave its range.  That is 2^-11 of a weight, well below the half step of a bf16 output (2^-8); for
+// fp16 outputs, whose half step it is, p scale_g is a pair high + low (2^-22).
 #pragma once
 #include "gemm_tc.cuh"
 #include "kv4_cache.cuh"
